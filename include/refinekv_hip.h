@@ -231,6 +231,92 @@ int rkv_dense_decode(const void* query, const void* keys, int64_t key_head_strid
 int rkv_dense_plan(int64_t heads, int64_t group, int64_t dim, int64_t length, int64_t* splits,
                    size_t* workspace_bytes);
 
+/*
+ * Rotary positions.  Each pair (x0, x1) of a row's rotated part turns by
+ * t = position * rate: y0 = x0 c - x1 s, y1 = x1 c + x0 s with c = scale
+ * cos t, s = scale sin t.  The reference calls the model's own function
+ * (src/refinekv/integrations/transformers.py:485-508).
+ *   query: (tokens, q_heads, dim), key: (tokens, k_heads, dim), dtype RKV_*,
+ *     with token and head strides; q_heads or k_heads 0: absent.
+ *   positions: (tokens,) int64 (wide_positions != 0) or int32.
+ *   rates: (rotary_dim / 2,) float64, WHOLE TURNS per position (radians /
+ *     2 pi) of each pair: dims i and i + rotary_dim / 2, or, interleaved != 0,
+ *     2 i and 2 i + 1.  Dims from rotary_dim (even, at most dim) on pass.
+ *   inverse != 0 turns by -t (the transposed rotation; scale applies alike).
+ *   query_out / key_out may be query / key themselves (in place), else must
+ *   not overlap any input.
+ * The angle is reduced in fp64, the products are fp32, rounded once.
+ */
+int rkv_rotary(const void* query, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
+               const void* key, int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads,
+               int dtype, int64_t tokens, int64_t dim, const void* positions, int wide_positions,
+               const double* rates, int64_t rotary_dim, int interleaved, float scale, int inverse,
+               void* query_out, int64_t qo_token_stride, int64_t qo_head_stride, void* key_out,
+               int64_t ko_token_stride, int64_t ko_head_stride, rkv_stream_t stream);
+
+/*
+ * A KV cache in pages shared by several sequences (no reference counterpart:
+ * its caches hold one sequence, contiguous).  Token t of sequence b lies in
+ * row t % page_size of page block_table[b * table_stride + t / page_size];
+ * page p, KV head h, row r starts p * page_stride + h * head_stride + r *
+ * token_stride elements into keys / values, head_dim dense.  lengths[b]:
+ * the sequence's visible tokens, those of the call at hand included.
+ * block_table and lengths are read on the device: a page outside [0, pages)
+ * is never read or written.
+ */
+typedef struct rkv_paged_cache {
+  void* keys;
+  int64_t key_page_stride, key_head_stride, key_token_stride;
+  void* values;
+  int64_t value_page_stride, value_head_stride, value_token_stride;
+  const int32_t* block_table; /* (sequences, max_blocks) */
+  int64_t table_stride;
+  const int32_t* lengths; /* (sequences,) */
+  int64_t pages, heads, page_size, dim, sequences, max_blocks;
+  int dtype; /* RKV_* */
+} rkv_paged_cache;
+
+/*
+ * New keys and values of the cache's sequences to their pages, keys (and the
+ * same tokens' queries) turned on the way as by rkv_rotary.
+ *   key/value: (tokens, heads, dim) rows with token and head strides, the
+ *     cache's dtype; query: (tokens, q_heads, dim) or q_heads 0.
+ *   token_starts: device int32 (sequences + 1,): sequence b's new tokens are
+ *     rows token_starts[b] .. token_starts[b + 1] - 1 and become its last
+ *     ones, ending at position lengths[b] - 1; NULL: tokens = sequences, one
+ *     each.
+ *   rates NULL with rotary_dim 0: nothing turns.
+ * A row of no sequence or at a negative position (an idle place of a padded
+ * batch) is not stored and its query is copied unturned; a row whose page is
+ * outside the cache or the table is not stored.  Sequences must not append
+ * to the same page row in one call.
+ */
+int rkv_paged_append(const rkv_paged_cache* cache, const void* query, int64_t q_token_stride,
+                     int64_t q_head_stride, int64_t q_heads, void* query_out,
+                     int64_t qo_token_stride, int64_t qo_head_stride, const void* key,
+                     int64_t k_token_stride, int64_t k_head_stride, const void* value,
+                     int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
+                     const int32_t* token_starts, const double* rates, int64_t rotary_dim,
+                     int interleaved, float scale, rkv_stream_t stream);
+
+/*
+ * Attention of one new token per sequence over its visible tokens:
+ *   out[b, h * group + g] = softmax_t(scale query[b, h * group + g] . K[b, h, t]) V[b, h, t]
+ * over t < lengths[b] (rkv_dense_decode for many sequences in pages).
+ *   query: (sequences, heads * group, dim) with sequence and head strides;
+ *   output: the same shape, dense.  bf16 or fp16, dim 32..256 step 32, group
+ *   <= 16; query, output and cache 16-byte aligned, strides multiples of 8.
+ *   workspace: rkv_paged_plan's bytes.
+ * lengths[b] <= 0 gives zeros.  A page outside the cache among the visible
+ * ones, or a length past the table, gives NaN in that sequence's rows.
+ */
+int rkv_paged_decode(const rkv_paged_cache* cache, const void* query, int64_t q_sequence_stride,
+                     int64_t q_head_stride, int64_t group, float scale, void* output,
+                     void* workspace, size_t workspace_bytes, rkv_stream_t stream);
+
+/* Workspace bytes of rkv_paged_decode for this cache on the current device. */
+int rkv_paged_plan(const rkv_paged_cache* cache, int64_t group, size_t* workspace_bytes);
+
 /* Profiling hook with no reference counterpart: when `events` points to 4
  * hipEvent_t handles, later rkv_select / rkv_decode calls on this thread
  * record events[0] before their first kernel and events[k] after their k-th

@@ -1,0 +1,354 @@
+// Rotary positions, alone (rkv_rotary) and on the way into a paged KV cache
+// (rkv_paged_append).
+//
+// A pair (x0, x1) of a head's rotated part turns by t = position * rate_i:
+//   y0 = x0 c - x1 s,  y1 = x1 c + x0 s,  c = a cos t, s = a sin t,
+// with a the table's attention factor.  The half layout pairs dims i and
+// i + r/2, the interleaved one 2i and 2i + 1; dims from r on pass.  Memory
+// bound: every value is read and written once.
+#include "rkv_common.h"
+#include "rkv_internal.h"
+#include "rkv_paged.h"
+
+namespace rkv {
+namespace {
+
+constexpr int kThreads = 256;
+
+// A set of rows (token, head, dim): strides in elements, dim dense.
+struct Rows {
+  const char* src;
+  char* dst;                 // rows, or the cache's pages for keys and values
+  int64_t src_ts, src_hs;    // token and head strides of src, elements
+  int64_t dst_ts, dst_hs;    // of dst (a page's row and head strides in a cache)
+  int64_t dst_ps;            // page stride of dst, elements (cache only)
+  int heads;
+  int paged;                 // dst is the cache's pages
+};
+
+struct RotaryArgs {
+  Rows rows[3];              // queries, keys, values (heads 0: absent)
+  int heads;                 // all of them
+  int64_t tokens;
+  int dim, rotary_dim;
+  const void* positions;     // int32 or int64 per token (null: from the sequences)
+  int wide_positions;
+  const double* rates;       // turns per position of each pair, rotary_dim / 2
+  float scale, sign;         // attention factor; -1 turns back
+  // paged: token t belongs to the sequence b with starts[b] <= t < starts[b + 1]
+  // (null: sequence t), at position lengths[b] - (starts[b + 1] - t)
+  const int32_t* starts;
+  const int32_t* lengths;
+  const int32_t* table;
+  int64_t table_stride;
+  int sequences, max_blocks, pages, shift;
+  int items, turning;        // items of a head's row; those that turn come first
+  int step, gap;             // dims from one turning item to the next, of an item's two vectors
+  int slots, per_block;      // heads that a token's threads hold at a time, a workgroup's tokens
+};
+
+// cos and sin of `turns` whole turns, to an ulp or two of fp32.  The angle of
+// a far position needs more than fp32's 24 bits (131071 * 1 rad has an ulp of
+// 0.008 rad there), so the whole quarter turns are taken off in fp64; what
+// is left, at most pi/4, goes through the Taylor series of sin (to a^9,
+// truncation 2e-9) and cos (to a^10, 2e-10).
+__device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
+  const double quarter = __builtin_rint(turns * 4.0);
+  const float a = (float)((turns - quarter * 0.25) * 6.283185307179586477);
+  const float a2 = a * a;
+  float p = 2.75573192239858907e-06f;                    // 1/9!
+  p = __builtin_fmaf(p, a2, -1.98412698412698413e-04f);  // 1/7!
+  p = __builtin_fmaf(p, a2, 8.33333333333333333e-03f);   // 1/5!
+  p = __builtin_fmaf(p, a2, -1.66666666666666667e-01f);  // 1/3!
+  const float sn = __builtin_fmaf(p * a2, a, a);
+  float q = -2.75573192239858907e-07f;                   // 1/10!
+  q = __builtin_fmaf(q, a2, 2.48015873015873016e-05f);   // 1/8!
+  q = __builtin_fmaf(q, a2, -1.38888888888888889e-03f);  // 1/6!
+  q = __builtin_fmaf(q, a2, 4.16666666666666667e-02f);   // 1/4!
+  q = __builtin_fmaf(q, a2, -0.5f);
+  const float cn = __builtin_fmaf(q, a2, 1.0f);
+  // the low two bits of the whole quarters (their count may pass 32 bits)
+  const int k = (int)(quarter - 4.0 * __builtin_floor(quarter * 0.25));
+  c = k & 1 ? sn : cn;
+  s = k & 1 ? cn : sn;
+  c = k == 1 || k == 2 ? -c : c;
+  s = k >= 2 ? -s : s;
+}
+
+// Where a token's rows go: its position, and its page and row in a cache
+// (page < 0: not in the cache).
+struct Place {
+  int64_t position;
+  int page, row;
+  bool live;  // has a position: its rows turn
+};
+
+__device__ __forceinline__ Place place_of(const RotaryArgs& a, int64_t t) {
+  Place p{0, -1, 0, true};
+  if (a.positions) {
+    p.position = a.wide_positions ? static_cast<const int64_t*>(a.positions)[t]
+                                  : static_cast<const int32_t*>(a.positions)[t];
+    return p;
+  }
+  int64_t b = t, behind = 1;  // tokens of the sequence from this one on
+  if (a.starts) {
+    // the first sequence that ends after t (empty ones end where they start)
+    int lo = 0, hi = a.sequences;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (a.starts[mid + 1] <= t) lo = mid + 1;
+      else hi = mid;
+    }
+    b = lo;
+    if (b >= a.sequences || a.starts[b] > t) return Place{0, -1, 0, false};
+    behind = a.starts[b + 1] - t;
+  }
+  p.position = (int64_t)a.lengths[b] - behind;
+  if (p.position < 0) return Place{0, -1, 0, false};
+  const int64_t block = p.position >> a.shift;
+  if (block < a.max_blocks) {
+    const int page = a.table[b * a.table_stride + block];
+    p.page = page >= 0 && page < a.pages ? page : -1;
+  }
+  p.row = (int)(p.position & ((1 << a.shift) - 1));
+  return p;
+}
+
+// A thread holds one item of a row: two vectors of W dims `gap` apart (the
+// half layout: gap r/2; the interleaved one's pairs where no vector holds
+// whole ones: W 1, gap 1), one vector of W / 2 adjacent pairs (kAdjacent), or
+// one of W dims that pass.  It works out the item's cos and sin once and
+// applies them to every slots-th head of its token.
+template <typename T, int W, bool kAdjacent>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
+  constexpr int kPairs = kAdjacent ? W / 2 : W;
+  constexpr int kSize = sizeof(T);
+  typedef T V __attribute__((ext_vector_type(W)));
+  const int wide = a.items < kThreads ? a.items : kThreads;
+  const int in_block = (int)(threadIdx.x / (uint32_t)(wide * a.slots));
+  const uint32_t rest = threadIdx.x % (uint32_t)(wide * a.slots);
+  const int slot = (int)(rest / (uint32_t)wide);
+  const int64_t t = (int64_t)blockIdx.x * a.per_block + in_block;
+  if (in_block >= a.per_block || t >= a.tokens) return;
+  const Place place = place_of(a, t);
+  for (int item = (int)(rest % (uint32_t)wide); item < a.items; item += kThreads) {
+    const bool turns = item < a.turning;
+    const int d0 = turns ? item * a.step : a.rotary_dim + (item - a.turning) * W;
+    const bool two = turns && !kAdjacent;
+    float c[kPairs], s[kPairs];
+    if (turns && place.live) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        cos_sin((double)place.position * a.rates[item * kPairs + i], c[i], s[i]);
+        c[i] *= a.scale;
+        s[i] *= a.scale * a.sign;
+      }
+    }
+    for (int n = slot; n < a.heads; n += a.slots) {
+      // queries, then keys, then values
+      const bool q = n < a.rows[0].heads, v = n >= a.rows[0].heads + a.rows[1].heads;
+      const int h = n - (q ? 0 : a.rows[0].heads) - (v ? a.rows[1].heads : 0);
+#define PICK(field) (q ? a.rows[0].field : v ? a.rows[2].field : a.rows[1].field)
+      if (PICK(paged) && place.page < 0) continue;
+      const char* src = PICK(src) + (t * PICK(src_ts) + h * PICK(src_hs) + d0) * kSize;
+      char* dst = PICK(dst) + ((PICK(paged) ? place.page * PICK(dst_ps) + place.row * PICK(dst_ts)
+                                            : t * PICK(dst_ts)) + h * PICK(dst_hs) + d0) * kSize;
+#undef PICK
+      V x = *reinterpret_cast<const V*>(src), z = x;
+      if (two) z = *reinterpret_cast<const V*>(src + a.gap * kSize);
+      if (turns && !v && place.live) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+          float x0, x1;
+          if constexpr (kAdjacent) x0 = (float)x[2 * i], x1 = (float)x[2 * i + 1];
+          else x0 = (float)x[i], x1 = (float)z[i];
+          const float y0 = __builtin_fmaf(x0, c[i], -(x1 * s[i]));
+          const float y1 = __builtin_fmaf(x1, c[i], x0 * s[i]);
+          if constexpr (kAdjacent) {
+            x[2 * i] = (T)y0;
+            x[2 * i + 1] = (T)y1;
+          } else {
+            x[i] = (T)y0;
+            z[i] = (T)y1;
+          }
+        }
+      }
+      *reinterpret_cast<V*>(dst) = x;
+      if (two) *reinterpret_cast<V*>(dst + a.gap * kSize) = z;
+    }
+  }
+}
+
+// Bytes of the widest vector (16, 8 or one element) that every row's address
+// and the rotated and passing parts allow.
+int vector_bytes(const RotaryArgs& a, int size, bool interleaved) {
+  const int64_t half = (int64_t)a.rotary_dim / 2;
+  for (int bytes = 16; bytes > size; bytes >>= 1) {
+    const int64_t n = bytes / size;
+    if (bytes < 8 || (interleaved ? a.rotary_dim : half) % n || (a.dim - a.rotary_dim) % n)
+      continue;
+    bool ok = true;
+    for (const Rows& r : a.rows) {
+      if (!r.heads) continue;
+      ok = ok && aligned(r.src, bytes) && aligned(r.dst, bytes) && r.src_ts % n == 0 &&
+           r.src_hs % n == 0 && r.dst_ts % n == 0 && r.dst_hs % n == 0 && r.dst_ps % n == 0;
+    }
+    if (ok) return bytes;
+  }
+  return size;
+}
+
+template <typename T, int W, bool kAdjacent>
+int launch_w(RotaryArgs& a, hipStream_t stream) {
+  const int half = a.rotary_dim / 2;
+  a.turning = half / (kAdjacent ? W / 2 : W);
+  a.items = a.turning + (a.dim - a.rotary_dim) / W;
+  const int wide = a.items < kThreads ? a.items : kThreads;
+  a.slots = kThreads / wide < a.heads ? kThreads / wide : a.heads;
+  a.per_block = kThreads / (wide * a.slots);
+  const int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
+  if (blocks > 0x7fffffff) return set_error(kInvalidArgument, "rotary: too many tokens");
+  rotary_kernel<T, W, kAdjacent><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
+  return check_launch("rotary_kernel");
+}
+
+template <typename T>
+int launch_t(RotaryArgs& a, bool interleaved, hipStream_t stream) {
+  constexpr int kSize = sizeof(T);
+  const int bytes = vector_bytes(a, kSize, interleaved);
+  if (interleaved && bytes > kSize) {
+    a.gap = 0;
+    a.step = bytes / kSize;
+    return bytes == 16 ? launch_w<T, 16 / kSize, true>(a, stream)
+                       : launch_w<T, 8 / kSize, true>(a, stream);
+  }
+  a.gap = interleaved ? 1 : a.rotary_dim / 2;
+  a.step = interleaved ? 2 : bytes / kSize;
+  if (bytes == 16) return launch_w<T, 16 / kSize, false>(a, stream);
+  if (bytes == 8) return launch_w<T, 8 / kSize, false>(a, stream);
+  return launch_w<T, 1, false>(a, stream);
+}
+
+int launch(RotaryArgs& a, int dtype, bool interleaved, hipStream_t stream) {
+  a.heads = 0;
+  for (const Rows& r : a.rows) a.heads += r.heads;
+  if (a.tokens == 0 || a.heads == 0) return kOk;
+  if (dtype == RKV_BF16) return launch_t<__bf16>(a, interleaved, stream);
+  if (dtype == RKV_F16) return launch_t<_Float16>(a, interleaved, stream);
+  return launch_t<float>(a, interleaved, stream);
+}
+
+int check_table(const char* who, const double* rates, int64_t rotary_dim, int64_t dim) {
+  if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > dim || (rotary_dim > 0 && !rates))
+    return set_error(kInvalidArgument, "%s: rotary_dim %lld must be even, at most head_dim %lld, "
+                     "with its rates", who, (long long)rotary_dim, (long long)dim);
+  return kOk;
+}
+
+int check_rows(const char* who, const void* src, const void* dst, int64_t heads, int size) {
+  if (heads < 0 || heads > 65535) return set_error(kInvalidArgument, "%s: bad head count", who);
+  if (heads && (!src || !dst)) return set_error(kInvalidArgument, "%s: null pointer argument", who);
+  if (heads && (!aligned(src, size) || !aligned(dst, size)))
+    return set_error(kInvalidArgument, "%s: rows not aligned to their type", who);
+  return kOk;
+}
+
+Rows plain_rows(const void* src, int64_t ts, int64_t hs, int64_t heads, void* dst, int64_t dst_ts,
+                int64_t dst_hs) {
+  Rows r{};
+  r.src = static_cast<const char*>(src);
+  r.dst = static_cast<char*>(dst);
+  r.src_ts = ts;
+  r.src_hs = hs;
+  r.dst_ts = dst_ts;
+  r.dst_hs = dst_hs;
+  r.heads = (int)heads;
+  return r;
+}
+
+}  // namespace
+}  // namespace rkv
+
+using namespace rkv;
+
+extern "C" int rkv_rotary(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                          int64_t q_heads, const void* key, int64_t k_token_stride,
+                          int64_t k_head_stride, int64_t k_heads, int dtype, int64_t tokens,
+                          int64_t dim, const void* positions, int wide_positions,
+                          const double* rates, int64_t rotary_dim, int interleaved, float scale,
+                          int inverse, void* query_out, int64_t qo_token_stride,
+                          int64_t qo_head_stride, void* key_out, int64_t ko_token_stride,
+                          int64_t ko_head_stride, hipStream_t stream) {
+  const char* who = "rkv_rotary";
+  clear_error();
+  if (!known_dtype(dtype)) return set_error(kUnsupported, "%s: dtype %d", who, dtype);
+  if (tokens < 0 || dim <= 0 || dim > 65535)
+    return set_error(kInvalidArgument, "%s: bad shape", who);
+  if (tokens && !positions) return set_error(kInvalidArgument, "%s: null positions", who);
+  const int size = (int)dtype_bytes(dtype);
+  int rc = check_table(who, rates, rotary_dim, dim);
+  if (!rc) rc = check_rows(who, query, query_out, tokens ? q_heads : 0, size);
+  if (!rc) rc = check_rows(who, key, key_out, tokens ? k_heads : 0, size);
+  if (rc) return rc;
+  RotaryArgs a{};
+  a.rows[0] = plain_rows(query, q_token_stride, q_head_stride, q_heads, query_out,
+                         qo_token_stride, qo_head_stride);
+  a.rows[1] = plain_rows(key, k_token_stride, k_head_stride, k_heads, key_out, ko_token_stride,
+                         ko_head_stride);
+  a.tokens = tokens;
+  a.dim = (int)dim;
+  a.rotary_dim = (int)rotary_dim;
+  a.positions = positions;
+  a.wide_positions = wide_positions;
+  a.rates = rates;
+  a.scale = scale;
+  a.sign = inverse ? -1.0f : 1.0f;
+  return launch(a, dtype, interleaved != 0, stream);
+}
+
+extern "C" int rkv_paged_append(const rkv_paged_cache* cache, const void* query,
+                                int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
+                                void* query_out, int64_t qo_token_stride, int64_t qo_head_stride,
+                                const void* key, int64_t k_token_stride, int64_t k_head_stride,
+                                const void* value, int64_t v_token_stride, int64_t v_head_stride,
+                                int64_t tokens, const int32_t* token_starts, const double* rates,
+                                int64_t rotary_dim, int interleaved, float scale,
+                                hipStream_t stream) {
+  const char* who = "rkv_paged_append";
+  clear_error();
+  int rc = check_cache(who, cache);
+  if (rc) return rc;
+  if (tokens < 0 || (!token_starts && tokens != cache->sequences))
+    return set_error(kInvalidArgument, "%s: without token_starts one token per sequence", who);
+  const int size = (int)dtype_bytes(cache->dtype);
+  rc = check_table(who, rates, rotary_dim, cache->dim);
+  if (!rc) rc = check_rows(who, query, query_out, tokens ? q_heads : 0, size);
+  if (!rc) rc = check_rows(who, key, cache->keys, tokens ? cache->heads : 0, size);
+  if (!rc) rc = check_rows(who, value, cache->values, tokens ? cache->heads : 0, size);
+  if (rc) return rc;
+  RotaryArgs a{};
+  a.rows[0] = plain_rows(query, q_token_stride, q_head_stride, q_heads, query_out,
+                         qo_token_stride, qo_head_stride);
+  a.rows[1] = plain_rows(key, k_token_stride, k_head_stride, cache->heads, cache->keys,
+                         cache->key_token_stride, cache->key_head_stride);
+  a.rows[2] = plain_rows(value, v_token_stride, v_head_stride, cache->heads, cache->values,
+                         cache->value_token_stride, cache->value_head_stride);
+  a.rows[1].dst_ps = cache->key_page_stride;
+  a.rows[2].dst_ps = cache->value_page_stride;
+  a.rows[1].paged = a.rows[2].paged = 1;
+  a.tokens = tokens;
+  a.dim = (int)cache->dim;
+  a.rotary_dim = (int)rotary_dim;
+  a.rates = rates;
+  a.scale = scale;
+  a.sign = 1.0f;
+  a.starts = token_starts;
+  a.lengths = cache->lengths;
+  a.table = cache->block_table;
+  a.table_stride = cache->table_stride;
+  a.sequences = (int)cache->sequences;
+  a.max_blocks = (int)cache->max_blocks;
+  a.pages = (int)cache->pages;
+  a.shift = page_shift(cache->page_size);
+  return launch(a, cache->dtype, interleaved != 0, stream);
+}

@@ -6,14 +6,22 @@ Same public API as the reference package (src/refinekv/__init__.py:3-25);
 
 from .attention import AttentionResult, select_blocks, select_blocks_union, sparse_attention
 from .config import RefineKVConfig
+from .paged import PagedCache, paged_append, paged_decode
+from .rotary import Rotary, RotaryConfig, rotate_heads
 from .summary import BlockSummary, build_summary
 
 __version__ = "0.1.2+mi355x"
 __all__ = [
     "AttentionResult",
     "BlockSummary",
+    "PagedCache",
     "RefineKVConfig",
+    "Rotary",
+    "RotaryConfig",
     "build_summary",
+    "paged_append",
+    "paged_decode",
+    "rotate_heads",
     "select_blocks",
     "select_blocks_union",
     "sparse_attention",

@@ -14,6 +14,7 @@ variable ``REFINEKV_HIP_CHECK=1`` every ``decode`` call checks it (a host
 synchronization per call, so not under graph capture).
 """
 
+import contextlib
 import ctypes
 import os
 
@@ -41,6 +42,14 @@ _u32 = ctypes.c_uint32
 
 class HipUnavailable(RuntimeError):
     pass
+
+
+class _PagedCache(ctypes.Structure):
+    """rkv_paged_cache."""
+    _fields_ = [("keys", _p), ("key_strides", _i64 * 3), ("values", _p),
+                ("value_strides", _i64 * 3), ("block_table", _p), ("table_stride", _i64),
+                ("lengths", _p), ("pages", _i64), ("heads", _i64), ("page_size", _i64),
+                ("dim", _i64), ("sequences", _i64), ("max_blocks", _i64), ("dtype", _int)]
 
 
 def _bind(lib):
@@ -98,6 +107,17 @@ def _bind(lib):
     lib.rkv_dense_decode.restype = _int
     lib.rkv_dense_plan.argtypes = [_i64, _i64, _i64, _i64, _p, _p]
     lib.rkv_dense_plan.restype = _int
+    lib.rkv_rotary.argtypes = [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _int, _i64, _i64, _p,
+                               _int, _p, _i64, _int, _f32, _int, _p, _i64, _i64, _p, _i64, _i64,
+                               _p]
+    lib.rkv_rotary.restype = _int
+    lib.rkv_paged_append.argtypes = [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p,
+                                     _i64, _i64, _i64, _p, _p, _i64, _int, _f32, _p]
+    lib.rkv_paged_append.restype = _int
+    lib.rkv_paged_decode.argtypes = [_p, _p, _i64, _i64, _i64, _f32, _p, _p, _size, _p]
+    lib.rkv_paged_decode.restype = _int
+    lib.rkv_paged_plan.argtypes = [_p, _i64, _p]
+    lib.rkv_paged_plan.restype = _int
     return lib
 
 
@@ -517,6 +537,106 @@ def dense_decode(query, keys, values, length=None, workspace=None, output=None):
         values.stride(1), heads, group, dim, cap, _ptr(length_dev), _ptr(output), _ptr(scratch),
         scratch.numel(), _stream(device))
     _check(rc, "rkv_dense_decode")
+    return output
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions and the paged cache
+# ---------------------------------------------------------------------------
+
+def _dense_rows(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _rows_args(t):
+    """(pointer, token stride, head stride) of (tokens, heads, dim) rows."""
+    if t is None:
+        return None, 0, 0
+    return _ptr(t), t.stride(0), t.stride(1)
+
+
+def _on(device):
+    """The device's guard, for a call on another device than the current one."""
+    return (contextlib.nullcontext() if device.index == torch.cuda.current_device()
+            else torch.cuda.device(device))
+
+
+def rotary(query, key, positions, table, query_out=None, key_out=None, inverse=False):
+    """rkv_rotary on checked (tokens, heads, dim) rows; returns (query, key)."""
+    device, config = query.device, table.config
+    query = _dense_rows(query)
+    if query_out is None:
+        query_out = torch.empty(query.shape, device=device, dtype=query.dtype)
+    if key is not None:
+        key = _dense_rows(key)
+        if key_out is None:
+            key_out = torch.empty(key.shape, device=device, dtype=key.dtype)
+    positions = positions.contiguous()
+    with _on(device):
+        rc = lib().rkv_rotary(
+            *_rows_args(query), query.shape[1], *_rows_args(key),
+            0 if key is None else key.shape[1], DTYPE_CODES[query.dtype], query.shape[0],
+            query.shape[2], _ptr(positions), positions.dtype == torch.int64, _ptr(table.turns),
+            config.rotary_dim, config.interleaved, table.scale, inverse, *_rows_args(query_out),
+            *_rows_args(key_out), _stream(device))
+    _check(rc, "rkv_rotary")
+    return query_out, key_out
+
+
+def _cache_struct(cache):
+    """The C view of a PagedCache, made on its first call; its pointers are
+    taken from the tensors on every call."""
+    view = cache.__dict__.get("_hip_view")
+    if view is None:
+        view = _PagedCache(
+            key_strides=(_i64 * 3)(*cache.keys.stride()[:3]),
+            value_strides=(_i64 * 3)(*cache.values.stride()[:3]),
+            table_stride=cache.block_table.stride(0), pages=cache.pages, heads=cache.heads,
+            page_size=cache.page_size, dim=cache.head_dim, sequences=cache.sequences,
+            max_blocks=cache.max_blocks, dtype=DTYPE_CODES[cache.keys.dtype])
+        cache.__dict__["_hip_view"] = view
+    view.keys, view.values = cache.keys.data_ptr(), cache.values.data_ptr()
+    view.block_table, view.lengths = cache.block_table.data_ptr(), cache.lengths.data_ptr()
+    return view
+
+
+def paged_append(key, value, cache, query=None, table=None, token_starts=None, query_out=None):
+    """rkv_paged_append on checked rows; returns the turned query or None."""
+    device = cache.keys.device
+    key, value = _dense_rows(key), _dense_rows(value)
+    if query is not None:
+        query = _dense_rows(query)
+        if query_out is None:
+            query_out = torch.empty(query.shape, device=device, dtype=query.dtype)
+    if table is None:
+        turns = (None, 0, 0, 1.0)
+    else:
+        turns = (_ptr(table.turns), table.config.rotary_dim, table.config.interleaved, table.scale)
+    view = _cache_struct(cache)
+    with _on(device):
+        rc = lib().rkv_paged_append(
+            ctypes.byref(view), *_rows_args(query), 0 if query is None else query.shape[1],
+            *_rows_args(query_out), *_rows_args(key), *_rows_args(value), key.shape[0],
+            _ptr(token_starts), *turns, _stream(device))
+    _check(rc, "rkv_paged_append")
+    return query_out
+
+
+def paged_decode(query, cache, scaling, workspace=None, output=None):
+    """rkv_paged_decode on a checked (sequences, q_heads, dim) query."""
+    device, group = query.device, query.shape[1] // cache.heads
+    query = _row_aligned(query, 16)
+    if output is None:
+        output = torch.empty(query.shape, device=device, dtype=query.dtype)
+    view, nbytes = _cache_struct(cache), _size()
+    with _on(device):
+        _check(lib().rkv_paged_plan(ctypes.byref(view), group, ctypes.byref(nbytes)),
+               "rkv_paged_plan")
+        scratch = _buffer(workspace, "hip_paged_scratch", (nbytes.value,), device, torch.uint8)
+        rc = lib().rkv_paged_decode(ctypes.byref(view), _ptr(query), query.stride(0),
+                                    query.stride(1), group, scaling, _ptr(output), _ptr(scratch),
+                                    scratch.numel(), _stream(device))
+    _check(rc, "rkv_paged_decode")
     return output
 
 

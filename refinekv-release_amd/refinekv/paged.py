@@ -1,0 +1,217 @@
+"""A KV cache in pages shared by many sequences, and the attention over it.
+
+The reference's caches hold one sequence, contiguous; a server that decodes
+many at once keeps their tokens in pages of one allocation.  ``PagedCache``
+describes such a cache (the tensors are the caller's, and so is the
+allocation of pages), ``paged_append`` writes new keys and values to it,
+turned to their positions on the way, and ``paged_decode`` attends one new
+token per sequence over its visible tokens.  A decode step::
+
+    cache.lengths.add_(1)                 # the new token counts as visible
+    query = paged_append(key, value, cache, query=query, rotary=rotary)
+    output = paged_decode(query, cache, workspace=workspace)
+
+Lengths and block table are read on the device, so one captured HIP graph
+serves every step of a batch.  ROCm tensors use the gfx950 kernels, others
+(and the types and shapes the kernels do not take) torch operations.
+"""
+
+from dataclasses import dataclass
+
+import torch
+
+from .rotary import DTYPES, check_out, pick_backend, rows_overlap
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+@dataclass(frozen=True, eq=False)
+class PagedCache:
+    """Keys and values of ``sequences`` sequences in pages.
+
+    ``keys``/``values``: (pages, kv_heads, page_size, head_dim), head_dim
+    dense, the other strides free (a cache kept as (pages, page_size,
+    kv_heads, head_dim) is passed as its transposed view).  ``block_table``:
+    (sequences, max_blocks) int32, the page of each page_size tokens; entries
+    past a sequence's length are not read.  ``lengths``: (sequences,) int32,
+    the visible tokens, those being appended included; 0 marks an idle place.
+    """
+
+    keys: torch.Tensor
+    values: torch.Tensor
+    block_table: torch.Tensor
+    lengths: torch.Tensor
+
+    def __post_init__(self):
+        keys, values, table, lengths = self.keys, self.values, self.block_table, self.lengths
+        if keys.ndim != 4 or keys.shape != values.shape or min(keys.shape) <= 0:
+            raise ValueError("keys and values must have the same nonempty (pages, kv_heads, "
+                             "page_size, head_dim) shape")
+        if keys.dtype != values.dtype or keys.device != values.device:
+            raise ValueError("keys and values must have the same device and dtype")
+        if not keys.is_floating_point():
+            raise TypeError("keys and values must be floating point")
+        if keys.shape[2] not in PAGE_SIZES:
+            raise ValueError(f"page_size must be one of {PAGE_SIZES}")
+        if keys.shape[3] > 1 and (keys.stride(3) != 1 or values.stride(3) != 1):
+            raise ValueError("keys and values must have a dense head_dim")
+        if table.ndim != 2 or min(table.shape) <= 0 or table.dtype != torch.int32:
+            raise ValueError("block_table must be int32 with a nonempty (sequences, max_blocks) "
+                             "shape")
+        if table.shape[1] > 1 and table.stride(1) != 1:
+            raise ValueError("block_table must have dense rows")
+        if lengths.shape != table.shape[:1] or lengths.dtype != torch.int32:
+            raise ValueError("lengths must be int32 with shape (sequences,)")
+        if not lengths.is_contiguous():
+            raise ValueError("lengths must be contiguous")
+        if table.device != keys.device or lengths.device != keys.device:
+            raise ValueError("block_table and lengths must be on the cache's device")
+
+    @classmethod
+    def empty(cls, pages, kv_heads, page_size, head_dim, sequences, max_blocks, *,
+              dtype=torch.bfloat16, device=None):
+        """A new cache of zeros with no pages assigned (block_table -1)."""
+        shape = (pages, kv_heads, page_size, head_dim)
+        return cls(torch.zeros(shape, dtype=dtype, device=device),
+                   torch.zeros(shape, dtype=dtype, device=device),
+                   torch.full((sequences, max_blocks), -1, dtype=torch.int32, device=device),
+                   torch.zeros(sequences, dtype=torch.int32, device=device))
+
+    @property
+    def pages(self):
+        return self.keys.shape[0]
+
+    @property
+    def heads(self):
+        return self.keys.shape[1]
+
+    @property
+    def page_size(self):
+        return self.keys.shape[2]
+
+    @property
+    def head_dim(self):
+        return self.keys.shape[3]
+
+    @property
+    def sequences(self):
+        return self.block_table.shape[0]
+
+    @property
+    def max_blocks(self):
+        return self.block_table.shape[1]
+
+    @property
+    def capacity(self):
+        """Tokens a sequence's row of the table can address."""
+        return self.max_blocks * self.page_size
+
+
+def _check_rows(name, rows, cache, tokens=None):
+    if (rows.ndim != 3 or rows.shape[1] <= 0 or rows.shape[2] != cache.head_dim
+            or (tokens is not None and rows.shape[0] != tokens)):
+        raise ValueError(f"{name} must have shape (tokens, heads, head_dim) with the cache's "
+                         "head_dim and the key's tokens")
+    if rows.dtype != cache.keys.dtype or rows.device != cache.keys.device:
+        raise ValueError(f"{name} must have the cache's dtype and device")
+
+
+@torch.no_grad()
+def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=None,
+                 query_out=None, backend="auto"):
+    """Write new (tokens, kv_heads, head_dim) keys and values to their
+    sequences' pages, and return the turned queries (None without a query).
+
+    With ``token_starts`` (sequences + 1,) int32, rows token_starts[b] up to
+    token_starts[b + 1] are sequence b's last tokens, ending at position
+    lengths[b] - 1; without it every sequence has one.  With ``rotary`` keys
+    and ``query`` (tokens, q_heads, head_dim) are turned to those positions;
+    ``query_out`` takes the turned queries (it may be the query itself).
+
+    Rows of no sequence (behind the last one) or without a position (an idle
+    place: length 0) are not stored, and their queries are returned unturned.
+    A row whose page is outside the cache, or past the block table, is not
+    stored.  No two rows of a call may fall on the same place: a page written
+    here belongs to one sequence.
+    """
+    _check_rows("key", key, cache)
+    _check_rows("value", value, cache, key.shape[0])
+    if key.shape[1] != cache.heads or value.shape[1] != cache.heads:
+        raise ValueError("key and value must have the cache's heads")
+    device = cache.keys.device
+    if token_starts is not None:
+        if (token_starts.shape != (cache.sequences + 1,) or token_starts.dtype != torch.int32
+                or token_starts.device != device or not token_starts.is_contiguous()):
+            raise ValueError("token_starts must be contiguous int32 with shape (sequences + 1,) "
+                             "on the cache's device")
+    elif key.shape[0] != cache.sequences:
+        raise ValueError("without token_starts there is one token per sequence")
+    if rotary is not None and (rotary.config.head_dim != cache.head_dim
+                               or rotary.device != device):
+        raise ValueError("rotary must have the cache's head_dim and device")
+    if query is not None:
+        if rotary is None:
+            raise ValueError("a query is only taken to be turned: pass rotary")
+        _check_rows("query", query, cache, key.shape[0])
+        if query_out is not None:
+            check_out("query_out", query_out, query, (key, value))
+    elif query_out is not None:
+        raise ValueError("query_out without a query")
+    if pick_backend(key, backend, key.dtype in DTYPES,
+                    "the HIP append needs a bf16, fp16 or fp32 cache") == "hip":
+        from . import _hip
+
+        return _hip.paged_append(key, value, cache, query, rotary, token_starts, query_out)
+    from .reference_paged import append
+
+    turned = append(cache, key, value, query, rotary, token_starts)
+    return turned if query_out is None else query_out.copy_(turned)
+
+
+def _decode_support(query, cache):
+    """None, or why the HIP kernel does not take the call."""
+    from . import _hip
+
+    group = query.shape[1] // cache.heads
+    if cache.keys.dtype not in (torch.bfloat16, torch.float16):
+        return "the HIP paged decode needs a bf16 or fp16 cache"
+    if cache.head_dim not in _hip.SUPPORTED_DIMS or group > _hip.MAX_GROUP:
+        return "the HIP paged decode needs head_dim in 32..256 (multiple of 32) and group <= 16"
+    for t in (cache.keys, cache.values):
+        if t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]):
+            return "the HIP paged decode needs a cache of 16-byte aligned rows"
+    return None
+
+
+@torch.no_grad()
+def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, backend="auto"):
+    """Attention of one new token per sequence over its visible tokens.
+
+    ``query`` (sequences, q_heads, head_dim), q_heads a multiple of the
+    cache's heads (head h's rows are its group h); ``scaling`` defaults to
+    head_dim^-0.5.  Returns a new tensor of the query's shape, or ``output``.
+    ``workspace`` (a dict) keeps the partial results' buffer from call to
+    call; calls that share one must be ordered on one stream.
+
+    A sequence of length 0 gives zeros; one with a page outside the cache
+    among its visible ones, or a length past its table, gives NaN.
+    """
+    _check_rows("query", query, cache, cache.sequences)
+    if query.shape[1] % cache.heads:
+        raise ValueError("query heads must be a multiple of the cache's heads")
+    if output is not None:
+        if (output.shape != query.shape or output.dtype != query.dtype
+                or output.device != query.device or not output.is_contiguous()):
+            raise ValueError("output must be contiguous with the query's shape, dtype and device")
+        if rows_overlap(output, query):
+            raise ValueError("output must not overlap the query")
+    scaling = cache.head_dim ** -0.5 if scaling is None else float(scaling)
+    why = _decode_support(query, cache) if query.is_cuda else None
+    if pick_backend(query, backend, why is None, why) == "hip":
+        from . import _hip
+
+        return _hip.paged_decode(query, cache, scaling, workspace, output)
+    from .reference_paged import decode
+
+    out = decode(query, cache, scaling)
+    return out if output is None else output.copy_(out)
