@@ -1,6 +1,8 @@
 // Attention of one new token per sequence over a paged KV cache:
 //   out[b, h, g] = softmax_t(scale q[b, h, g] . K[t]) V,  t < lengths[b],
 // token t of KV head h at row t % P of page table[b][t / P].
+#include <atomic>
+
 #include "rkv_common.h"
 #include "rkv_internal.h"
 #include "rkv_paged.h"
@@ -8,90 +10,588 @@
 namespace rkv {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kTileTokens = 32;  // tokens a wave takes at a time: two halves of 16
+
+typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+typedef float F32x4 __attribute__((ext_vector_type(4)));
+
+// A type's matrix products (16 x 16 x 32) and its rounding of pairs.
+template <bool kHalf>
+struct Type16;
+template <>
+struct Type16<false> {
+  typedef __bf16 E;
+  typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ F32x4 mma(V8 a, V8 b, F32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Type16<true> {
+  typedef _Float16 E;
+  typedef _Float16 V8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ F32x4 mma(V8 a, V8 b, F32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
 
 struct PagedArgs {
   const char* query;             // (B, H G, D), strides in elements
   int64_t q_bs, q_hs;
   const char* keys;
   const char* values;
-  int64_t k_ps, k_hs, k_ts;      // page, head and token strides, elements
-  int64_t v_ps, v_hs, v_ts;
+  int64_t k_ps, k_hs, v_ps, v_hs;  // page and head strides, elements
+  uint32_t k_ts, v_ts;             // row strides, bytes
   const int32_t* table;
   int64_t table_stride;
   const int32_t* lengths;
   int sequences, heads, group, max_blocks, pages, shift;
-  float scale;
+  float scale;                   // times log2 e: the softmax runs on 2^x
   char* out;                     // (B, H G, D) dense
+  int min_tiles;                 // tiles a wave takes at the least
+  // a row (sequence, KV head) whose tiles lie in several workgroups: their
+  // partial results, [workgroup][0: began before, 1: begins here]
+  int64_t* part_row;             // row, or -1
+  float2* part_ml;               // [..][group]
+  float* part_acc;               // [..][group][D]
 };
 
-template <bool kHalf>
-__device__ __forceinline__ float load16(const char* p) {
-  if constexpr (kHalf) return (float)*reinterpret_cast<const _Float16*>(p);
-  return bf16_to_f32(*reinterpret_cast<const uint16_t*>(p));
+// Dims of a value row that a lane holds: D / 16 of them, as 16-, 8- and
+// 4-byte pieces (of 128, 64 and 32 dims of the row).
+template <int D>
+struct Pieces {
+  static constexpr int k8 = D / 128;
+  static constexpr int k4 = D % 128 >= 64 ? 1 : 0;
+  static constexpr int k2 = D % 64 >= 32 ? 1 : 0;
+  static constexpr int kBlocks = D / 16;  // 16-dim matrix products: 8 k8 + 4 k4 + 2 k2
+  // first dim of lane column i's piece of product m, and the dim in it
+  static __device__ __forceinline__ int dim(int m, int i) {
+    if (m < 8 * k8) return (m / 8) * 128 + i * 8 + m % 8;
+    m -= 8 * k8;
+    if (m < 4 * k4) return 128 * k8 + i * 4 + m;
+    m -= 4 * k4;
+    return 128 * k8 + 64 * k4 + i * 2 + m;
+  }
+};
+
+// One tile's operands as they come from memory.
+template <int D>
+struct Tile {
+  using P = Pieces<D>;
+  U32x4 k[2][D / 32];
+  U32x4 v8[P::k8 ? P::k8 : 1][8];
+  U32x2 v4[8];
+  uint32_t v2[8];
+};
+
+// A buffer view from `base` on, without an upper bound (the caller's offsets
+// stay inside a page); base must be wave-uniform.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t view_at(const char* base) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo),
+                                           (short)0, (int)0x7fffffff, 0x00020000);
 }
 
-// One workgroup per (query head, sequence): 16 lanes share a token's dims, 16
-// such groups take every 16th token with a running maximum and sum, joined at
-// the end in LDS.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// An int of an array that does not change during a launch, at a wave-uniform
+// place: a scalar load.
+__device__ __forceinline__ int scalar_at(const int32_t* p, int64_t i) {
+  typedef __attribute__((address_space(4))) const int32_t ConstI32;
+  return ((ConstI32*)(uintptr_t)p)[i];
+}
+
+// A sequence's length as attended: negative is 0; one past the table is 0 with
+// its row marked bad.
+__device__ __forceinline__ int length_of(const PagedArgs& a, int n, bool& bad) {
+  bad = n > 0 && (n - 1) >> a.shift >= a.max_blocks;
+  return bad || n < 0 ? 0 : n;
+}
+
+// Tiles of a sequence's row: one at least, so that every row has an owner
+// that writes its output.
+__device__ __forceinline__ int tiles_of(int length) {
+  return length > kTileTokens ? (length - 1) / kTileTokens + 1 : 1;
+}
+
+// Where a wave stands in the list of all tiles: sequence by sequence, KV head
+// by KV head, tile by tile.
+struct Cursor {
+  int b, h, tile, tiles, length;
+  bool bad;
+};
+
+__device__ __forceinline__ void next_tile(const PagedArgs& a, Cursor& c) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.h < a.heads) return;
+  c.h = 0;
+  ++c.b;
+  if (c.b < a.sequences) {
+    c.length = length_of(a, scalar_at(a.lengths, c.b), c.bad);
+    c.tiles = tiles_of(c.length);
+  }
+}
+
+// A wave's results of a row that it does not hold whole.
+template <int D>
+struct Part {
+  float acc[kMaxGroup][D];
+  float2 ml[kMaxGroup];
+};
+
+struct PartHead {
+  int64_t row;        // -1: unused
+  int begins, ends;   // the row's first / last tile is in the wave
+};
+
+// Every wave takes an equal, contiguous share of all tiles and walks it alone:
+// the keys and values of the next tile are loading while one is computed,
+// across rows' ends too.  A tile is 32 tokens, all of S^T = K Q^T and
+// O^T = V^T P^T on the matrix cores with the query rows in the columns, so
+// that a lane's maximum, sum and accumulators all belong to query row l % 16:
+//   S^T: A = 16 key rows straight from memory (lane l: row l % 16, dims
+//     8 (l / 16) + 32 j ..), B = the query rows; the result in lane l is
+//     S[t = 4 (l / 16) + r][l % 16], r = 0..3.
+//   O^T: B = P^T, whose k slots 8 (l / 16) + e are tokens 4 (l / 16) + e of
+//     the first half (e < 4) and 4 (l / 16) + e - 4 of the second: the values
+//     that lane l already holds.  A = V^T over the same slots: lane l loads
+//     the same 8 dims of those 8 tokens (16 lanes: a whole row) and
+//     transposes them with byte permutes; the m-th of 8 products takes dim
+//     8 (l % 16) + m for its row l % 16.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kThreads) void paged_kernel(PagedArgs a) {
-  constexpr int CH = D / 16;
-  __shared__ float acc_s[16][D];
-  __shared__ float m_s[16], l_s[16];
-  const int hq = blockIdx.x, b = blockIdx.y, h = hq / a.group;
-  const int c = threadIdx.x % 16, grp = threadIdx.x / 16;
-  const int length = a.lengths[b];
-  const char* q = a.query + (b * a.q_bs + hq * a.q_hs + c * CH) * 2;
-  float qf[CH], acc[CH];
-  for (int i = 0; i < CH; ++i) {
-    qf[i] = load16<kHalf>(q + 2 * i);
-    acc[i] = 0.0f;
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedArgs a) {
+  using T = Type16<kHalf>;
+  using V8 = typename T::V8;
+  using E = typename T::E;
+  using P = Pieces<D>;
+  __shared__ alignas(16) Part<D> parts[kWaves][2];
+  __shared__ PartHead heads_s[kWaves][2];
+  __shared__ int64_t wave_sum[kWaves];
+  __shared__ int64_t start_s[kWaves], count_s[kWaves];
+  __shared__ int seq_s[kWaves];
+  __shared__ int64_t rest_s[kWaves];
+  const int tid = threadIdx.x, lane = tid % kWave;
+  const int wave = uniform(tid / kWave);
+  const int li = lane & 15, lg = lane >> 4;
+
+  // ---- this workgroup's share of the tiles
+  const int per = (a.sequences + kThreads - 1) / kThreads;
+  const int b0 = tid * per, b1 = min(b0 + per, a.sequences);
+  int64_t sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    bool bad;
+    sum += tiles_of(length_of(a, a.lengths[b], bad));
   }
-  float m = kNegInf, l = 0.0f;
-  bool bad = length > a.max_blocks << a.shift;
-  for (int t = grp; t < length && !bad; t += 16) {
-    const int page = a.table[b * a.table_stride + (t >> a.shift)];
-    if (page < 0 || page >= a.pages) {
-      bad = true;
-      break;
+  sum *= a.heads;
+  int64_t before = sum;  // inclusive scan over the workgroup's threads
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int64_t x = __shfl_up(before, o, kWave);
+    before += lane >= o ? x : 0;
+  }
+  if (lane == kWave - 1) wave_sum[wave] = before;
+  if (tid < kWaves * 2) heads_s[tid / 2][tid % 2].row = -1;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += wave_sum[w];
+    total += wave_sum[w];
+  }
+  before -= sum;
+  int64_t waves = (int64_t)gridDim.x * kWaves;
+  const int64_t useful = (total + a.min_tiles - 1) / a.min_tiles;
+  waves = useful < waves ? useful : waves;
+  const int64_t share = total / waves, extra = total % waves;
+  for (int w = 0; w < kWaves; ++w) {
+    const int64_t id = (int64_t)blockIdx.x * kWaves + w;
+    const int64_t first = id * share + (id < extra ? id : extra);
+    const int64_t n = id < waves ? share + (id < extra ? 1 : 0) : 0;
+    if (tid == 0) count_s[w] = n;
+    if (n > 0 && first >= before && first < before + sum) {
+      int64_t rest = first - before;
+      int b = b0;
+      for (;; ++b) {
+        bool bad;
+        const int64_t here = (int64_t)tiles_of(length_of(a, a.lengths[b], bad)) * a.heads;
+        if (rest < here) break;
+        rest -= here;
+      }
+      seq_s[w] = b;
+      rest_s[w] = rest;
     }
-    const int64_t row = t & ((1 << a.shift) - 1);
-    const char* k = a.keys + (page * a.k_ps + h * a.k_hs + row * a.k_ts + c * CH) * 2;
-    const char* v = a.values + (page * a.v_ps + h * a.v_hs + row * a.v_ts + c * CH) * 2;
-    float s = 0.0f;
-    for (int i = 0; i < CH; ++i) s = __builtin_fmaf(qf[i], load16<kHalf>(k + 2 * i), s);
-    s = row16_sum_all(s) * a.scale;
-    const float mn = nanmax(m, s);
-    const float w = m == mn ? 1.0f : exp_hw(m - mn);
-    const float p = s == kNegInf ? 0.0f : exp_hw(s - mn);
-    l = l * w + p;
-    for (int i = 0; i < CH; ++i)
-      acc[i] = __builtin_fmaf(p, load16<kHalf>(v + 2 * i), acc[i] * w);
-    m = mn;
-  }
-  if (bad) l = __builtin_nanf("");
-  for (int i = 0; i < CH; ++i) acc_s[grp][c * CH + i] = acc[i];
-  if (c == 0) {
-    m_s[grp] = m;
-    l_s[grp] = l;
   }
   __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= D) return;
-  float M = kNegInf;
-  for (int j = 0; j < 16; ++j) M = nanmax(M, m_s[j]);
-  float L = 0.0f, o = 0.0f;
-  for (int j = 0; j < 16; ++j) {
-    if (l_s[j] == 0.0f) continue;
-    const float w = m_s[j] == M ? 1.0f : exp_hw(m_s[j] - M);
-    L += l_s[j] * w;
-    o += acc_s[j][d] * w;
+
+  int64_t left = count_s[wave];
+  left = ((int64_t)uniform((int)(left >> 32)) << 32) | (uint32_t)uniform((int)left);
+  if (left > 0) {
+    Cursor cur;
+    cur.b = uniform(seq_s[wave]);
+    cur.length = length_of(a, scalar_at(a.lengths, cur.b), cur.bad);
+    cur.tiles = tiles_of(cur.length);
+    const uint32_t rest = (uint32_t)uniform((int)rest_s[wave]);
+    cur.h = (int)(rest / (uint32_t)cur.tiles);
+    cur.tile = (int)(rest % (uint32_t)cur.tiles);
+
+    F32x4 acc[P::kBlocks];
+    V8 q[D / 32];
+    U32x4 q_next[D / 32];  // the next row's, loading with its first tile
+    float m = kNegInf, l = 0.0f;
+    bool bad_row = false;
+    bool begun = false;  // the row's first tile was this wave's
+
+    auto load_query = [&](const Cursor& c) {
+      const char* qp = a.query + ((int64_t)c.b * a.q_bs + (int64_t)(c.h * a.group + li) * a.q_hs
+                                  + lg * 8) * 2;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+        q_next[j] = li < a.group ? *reinterpret_cast<const U32x4*>(qp + j * 64)
+                                 : U32x4{0, 0, 0, 0};
+    };
+
+    auto load = [&](const Cursor& c, Tile<D>& t) -> bool {
+      bool bad = c.bad;
+      if (c.length == 0) return bad;
+      const int t0 = c.tile * kTileTokens;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        // a half behind the last token loads the first one's rows again
+        const int at = t0 + 16 * s < c.length ? t0 + 16 * s : t0;
+        int page = scalar_at(a.table, (int64_t)c.b * a.table_stride + (at >> a.shift));
+        if ((uint32_t)page >= (uint32_t)a.pages) {
+          bad = true;
+          page = 0;
+        }
+        const uint32_t in_page = (uint32_t)at & ((1u << a.shift) - 1u);
+        const auto kr = view_at(a.keys + ((int64_t)page * a.k_ps + (int64_t)c.h * a.k_hs) * 2
+                                + (uint64_t)in_page * a.k_ts);
+        const auto vr = view_at(a.values + ((int64_t)page * a.v_ps + (int64_t)c.h * a.v_hs) * 2
+                                + (uint64_t)in_page * a.v_ts);
+        const uint32_t ko = (uint32_t)li * a.k_ts + (uint32_t)lg * 16u;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+          t.k[s][j] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(ko + 64u * j), 0, 0);
+        const uint32_t vo = (uint32_t)(4 * lg) * a.v_ts;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int so = (int)(e * a.v_ts);
+#pragma unroll
+          for (int c8 = 0; c8 < P::k8; ++c8)
+            t.v8[c8][4 * s + e] = __builtin_amdgcn_raw_buffer_load_b128(
+                vr, (int)(vo + li * 16u + 256u * c8), so, 0);
+          if constexpr (P::k4 > 0)
+            t.v4[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b64(
+                vr, (int)(vo + li * 8u + 256u * P::k8), so, 0);
+          if constexpr (P::k2 > 0)
+            t.v2[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b32(
+                vr, (int)(vo + li * 4u + 256u * P::k8 + 128u * P::k4), so, 0);
+        }
+      }
+      return bad;
+    };
+
+    auto begin_row = [&](const Cursor& c) {
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) q[j] = __builtin_bit_cast(V8, q_next[j]);
+#pragma unroll
+      for (int n = 0; n < P::kBlocks; ++n) acc[n] = F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      m = kNegInf;
+      l = 0.0f;
+      bad_row = false;
+      begun = c.tile == 0;
+    };
+
+    auto compute = [&](const Cursor& c, Tile<D>& t, bool bad, bool last_tile) {
+      bad_row |= bad;
+      if (c.length > 0) {
+        float x[8];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          F32x4 s4 = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j)
+            s4 = T::mma(__builtin_bit_cast(V8, t.k[s][j]), q[j], s4);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[4 * s + r] = s4[r] * a.scale;
+        }
+        const int behind = c.length - c.tile * kTileTokens;  // tokens from the tile's first on
+        if (behind < kTileTokens) {
+          // the last tile: what lies behind the end weighs nothing, whatever
+          // its bytes are
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool live = 16 * (e / 4) + 4 * lg + e % 4 < behind;
+            x[e] = live ? x[e] : kNegInf;
+#pragma unroll
+            for (int c8 = 0; c8 < P::k8; ++c8)
+              t.v8[c8][e] = live ? t.v8[c8][e] : U32x4{0, 0, 0, 0};
+            if constexpr (P::k4 > 0) t.v4[e] = live ? t.v4[e] : U32x2{0, 0};
+            if constexpr (P::k2 > 0) t.v2[e] = live ? t.v2[e] : 0u;
+          }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = __builtin_fmaxf(top, x[e]);
+        float u, w;
+        xor16_pair(top, u, w);
+        top = __builtin_fmaxf(u, w);
+        xor32_pair(top, u, w);
+        top = __builtin_fmaxf(u, w);
+        if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+          const float mn = __builtin_fmaxf(m, top);
+          const float by = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= by;
+#pragma unroll
+          for (int n = 0; n < P::kBlocks; ++n) acc[n] *= by;
+        }
+        const float base = m == kNegInf ? 0.0f : m;
+        V8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float p = __builtin_amdgcn_exp2f(x[e] - base);
+          l += p;
+          // the weight as the sum of two 16-bit parts: its rounding would
+          // otherwise be the largest error of the result
+          hi[e] = (E)p;
+          lo[e] = (E)(p - (float)hi[e]);
+        }
+        // dims' products: byte permutes gather one dim of two tokens a word
+        auto product = [&](int n, uint32_t (&words)[4]) {
+          const V8 v = __builtin_bit_cast(V8, U32x4{words[0], words[1], words[2], words[3]});
+          acc[n] = T::mma(v, hi, acc[n]);
+          acc[n] = T::mma(v, lo, acc[n]);
+        };
+        constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
+#pragma unroll
+        for (int n = 0; n < P::kBlocks; ++n) {
+          uint32_t words[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t even, odd;
+            int d;
+            if (n < 8 * P::k8) {
+              d = n % 8;
+              even = t.v8[n / 8][2 * e][d / 2];
+              odd = t.v8[n / 8][2 * e + 1][d / 2];
+            } else if (n < 8 * P::k8 + 4 * P::k4) {
+              d = n - 8 * P::k8;
+              even = t.v4[2 * e][d / 2];
+              odd = t.v4[2 * e + 1][d / 2];
+            } else {
+              d = n - 8 * P::k8 - 4 * P::k4;
+              even = t.v2[2 * e];
+              odd = t.v2[2 * e + 1];
+            }
+            words[e] = __builtin_amdgcn_perm(odd, even, d % 2 ? kHigh : kLow);
+          }
+          product(n, words);
+        }
+      }
+      const bool ends = c.tile + 1 == c.tiles;
+      if (!ends && !last_tile) return;
+      float u, w, sum_l = l;
+      xor16_pair(sum_l, u, w);
+      sum_l = u + w;
+      xor32_pair(sum_l, u, w);
+      sum_l = u + w;
+      if (bad_row) sum_l = __builtin_nanf("");
+      const int64_t row = (int64_t)c.b * a.heads + c.h;
+      if (begun && ends) {
+        if (li < a.group) {
+          // a sequence without tokens gives zeros
+          const float by = c.length == 0 && !bad_row ? 0.0f : 1.0f / sum_l;
+          char* out = a.out + (row * a.group + li) * (D * 2);
+#pragma unroll
+          for (int n = 0; n < P::kBlocks; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              *reinterpret_cast<E*>(out + P::dim(n, 4 * lg + r) * 2) = (E)(acc[n][r] * by);
+        }
+        return;
+      }
+      const int slot = begun ? 1 : 0;
+      Part<D>& part = parts[wave][slot];
+      if (lane == 0) heads_s[wave][slot] = PartHead{row, begun, ends};
+      if (li < a.group) {
+        if (lg == 0) part.ml[li] = make_float2(m, sum_l);
+#pragma unroll
+        for (int n = 0; n < P::kBlocks; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) part.acc[li][P::dim(n, 4 * lg + r)] = acc[n][r];
+      }
+    };
+
+    Tile<D> t0, t1;
+    Cursor ahead = cur;
+    load_query(cur);
+    bool bad0 = load(cur, t0), bad1 = false;
+    bool row_start = true;  // of the row, or of the wave's share of it
+    for (;;) {
+      if (row_start) begin_row(cur);
+      if (left > 1) {
+        next_tile(a, ahead);
+        if (ahead.tile == 0) load_query(ahead);
+        bad1 = load(ahead, t1);
+      }
+      compute(cur, t0, bad0, left == 1);
+      if (--left == 0) break;
+      cur = ahead;
+      if (cur.tile == 0) begin_row(cur);
+      if (left > 1) {
+        next_tile(a, ahead);
+        if (ahead.tile == 0) load_query(ahead);
+        bad0 = load(ahead, t0);
+      }
+      compute(cur, t1, bad1, left == 1);
+      if (--left == 0) break;
+      cur = ahead;
+      row_start = cur.tile == 0;
+    }
   }
-  const float y = length <= 0 ? 0.0f : o / L;
-  char* out = a.out + (((int64_t)b * a.heads * a.group + hq) * D + d) * 2;
-  if constexpr (kHalf) *reinterpret_cast<_Float16*>(out) = (_Float16)y;
-  else *reinterpret_cast<uint16_t*>(out) = bf16_rne(y);
+  __syncthreads();
+
+  // ---- the waves' parts of rows: neighbours of one row are joined, in order
+  if (tid == 0) {
+    a.part_row[(int64_t)blockIdx.x * 2] = -1;
+    a.part_row[(int64_t)blockIdx.x * 2 + 1] = -1;
+  }
+  for (int s = 0; s < 2 * kWaves;) {
+    const PartHead head = heads_s[s / 2][s % 2];
+    int e = s + 1;
+    if (head.row < 0) {
+      s = e;
+      continue;
+    }
+    bool ends = head.ends;
+    for (; e < 2 * kWaves; ++e) {
+      const PartHead next = heads_s[e / 2][e % 2];
+      if (next.row >= 0 && next.row != head.row) break;
+      if (next.row >= 0) ends = next.ends;
+    }
+    const int64_t to = (int64_t)blockIdx.x * 2 + (head.begins ? 1 : 0);
+    const bool whole = head.begins && ends;
+    for (int x = tid; x < a.group * D; x += kThreads) {
+      const int g = x / D, d = x % D;
+      float M = kNegInf;
+      for (int i = s; i < e; ++i)
+        if (heads_s[i / 2][i % 2].row >= 0) M = __builtin_fmaxf(M, parts[i / 2][i % 2].ml[g].x);
+      float L = 0.0f, o = 0.0f;
+      for (int i = s; i < e; ++i) {
+        if (heads_s[i / 2][i % 2].row < 0) continue;
+        const Part<D>& p = parts[i / 2][i % 2];
+        const float w = p.ml[g].x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(p.ml[g].x - M);
+        // (a NaN sum stays one, whatever its weight)
+        L += p.ml[g].y * w;
+        o += p.acc[g][d] * w;
+      }
+      if (whole) {
+        *reinterpret_cast<E*>(a.out + ((head.row * a.group + g) * D + d) * 2) = (E)(o / L);
+      } else {
+        a.part_acc[(to * a.group + g) * D + d] = o;
+        if (d == 0) a.part_ml[to * a.group + g] = make_float2(M, L);
+      }
+    }
+    if (!whole && tid == 0) a.part_row[to] = head.row;
+    s = e;
+  }
+}
+
+// Joins the parts of one row that several workgroups hold: workgroup (k, g)
+// query row g of the row that begins in the attention's workgroup k and goes
+// on in those after it.
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedArgs a, int grid) {
+  constexpr int kStripes = kThreads / (D / 4) < 1 ? 1 : kThreads / (D / 4);
+  __shared__ alignas(16) float acc_s[kStripes][D];
+  __shared__ float2 ml_s[kStripes];
+  const int k = blockIdx.x, g = blockIdx.y;
+  const int64_t row = a.part_row[2 * (int64_t)k + 1];
+  if (row < 0) return;
+  // the workgroups after it whose first part is of the same row
+  int n = 1;
+  for (int j = k + 1; j < grid; j += kWave) {
+    const int at = j + (int)(threadIdx.x % kWave);
+    const uint64_t same =
+        __builtin_amdgcn_ballot_w64(at < grid && a.part_row[2 * (int64_t)at] == row);
+    const int run = ~same ? __builtin_ctzll(~same) : kWave;
+    n += run;
+    if (run < kWave) break;
+  }
+  const int c = threadIdx.x % (D / 4), stripe = threadIdx.x / (D / 4);
+  float m = kNegInf, l = 0.0f;
+  F32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (stripe < kStripes) {
+    for (int j = stripe; j < n; j += kStripes) {
+      const int64_t at = (2 * (int64_t)(k + j) + (j == 0 ? 1 : 0)) * a.group + g;
+      const float2 ml = a.part_ml[at];
+      const F32x4 x = *reinterpret_cast<const F32x4*>(a.part_acc + at * D + 4 * c);
+      const float mn = __builtin_fmaxf(m, ml.x);
+      const float old = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+      const float w = ml.x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+      l = l * old + ml.y * w;
+      o = o * old + x * w;
+      m = mn;
+    }
+    *reinterpret_cast<F32x4*>(&acc_s[stripe][4 * c]) = o;
+    if (c == 0) ml_s[stripe] = make_float2(m, l);
+  }
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  const int d = threadIdx.x;
+  float M = kNegInf, L = 0.0f, y = 0.0f;
+  for (int j = 0; j < kStripes; ++j) M = __builtin_fmaxf(M, ml_s[j].x);
+  for (int j = 0; j < kStripes; ++j) {
+    const float w = ml_s[j].x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml_s[j].x - M);
+    L += ml_s[j].y * w;
+    y += acc_s[j][d] * w;
+  }
+  using E = typename Type16<kHalf>::E;
+  *reinterpret_cast<E*>(a.out + ((row * a.group + g) * D + d) * 2) = (E)(y / L);
+}
+
+// Workgroups that the current device holds at once, 0 if unknown.
+template <int D, bool kHalf>
+int paged_resident() {
+  static std::atomic<int> of_dev[64];  // per device; 0 = not asked yet
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 0;
+  int n = of_dev[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    int cus = 0, per_cu = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, paged_kernel<D, kHalf>, kThreads,
+                                                     0) != hipSuccess)
+      return 0;
+    n = cus * per_cu;
+    of_dev[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+struct PagedPlan {
+  int grid = 0;
+  size_t ml_off = 0, acc_off = 0, total = 0;
+};
+
+PagedPlan paged_plan(const rkv_paged_cache* c, int64_t group) {
+  PagedPlan P;
+  RKV_DISPATCH_DIM(c->dim, D, {
+    P.grid = c->dtype == RKV_F16 ? paged_resident<D, true>() : paged_resident<D, false>();
+  });
+  if (P.grid <= 0) P.grid = 512;
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  const size_t parts = (size_t)P.grid * 2;
+  P.ml_off = up(parts * sizeof(int64_t));
+  P.acc_off = P.ml_off + up(parts * group * sizeof(float2));
+  P.total = P.acc_off + up(parts * group * c->dim * sizeof(float));
+  return P;
 }
 
 int check_paged(const char* who, const rkv_paged_cache* c, int64_t group) {
@@ -109,6 +609,12 @@ int check_paged(const char* who, const rkv_paged_cache* c, int64_t group) {
                              c->value_page_stride, c->value_head_stride, c->value_token_stride};
   for (int64_t s : strides)
     if (s % 8) return set_error(kInvalidArgument, "%s: cache strides must be multiples of 8", who);
+  const int64_t tiles = c->max_blocks * c->page_size / kTileTokens + 1;
+  if (tiles > ((int64_t(1) << 31) - 1) / c->heads)
+    return set_error(kUnsupported, "%s: a sequence's table covers too many tokens", who);
+  // 16 rows of a page are addressed with 32-bit byte offsets
+  if (c->key_token_stride > (1 << 25) || c->value_token_stride > (1 << 25))
+    return set_error(kUnsupported, "%s: rows more than 64 MiB apart", who);
   if (!aligned(c->keys, 16) || !aligned(c->values, 16))
     return set_error(kInvalidArgument, "%s: the cache must be 16-byte aligned", who);
   return kOk;
@@ -125,7 +631,7 @@ extern "C" int rkv_paged_plan(const rkv_paged_cache* cache, int64_t group,
   if (!workspace_bytes) return set_error(kInvalidArgument, "rkv_paged_plan: null pointer");
   const int rc = check_paged("rkv_paged_plan", cache, group);
   if (rc) return rc;
-  *workspace_bytes = 0;
+  *workspace_bytes = paged_plan(cache, group).total;
   return kOk;
 }
 
@@ -142,6 +648,12 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
     return set_error(kInvalidArgument,
                      "%s: query and output must be 16-byte aligned with strides in multiples of 8",
                      who);
+  const PagedPlan P = paged_plan(cache, group);
+  if (!workspace || workspace_bytes < P.total)
+    return set_error(kWorkspaceTooSmall, "%s: workspace of %zu bytes, %zu needed", who,
+                     workspace_bytes, P.total);
+  if (!aligned(workspace, 16))
+    return set_error(kInvalidArgument, "%s: workspace must be 16-byte aligned", who);
   PagedArgs a{};
   a.query = static_cast<const char*>(query);
   a.q_bs = q_sequence_stride;
@@ -150,10 +662,10 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
   a.values = static_cast<const char*>(cache->values);
   a.k_ps = cache->key_page_stride;
   a.k_hs = cache->key_head_stride;
-  a.k_ts = cache->key_token_stride;
   a.v_ps = cache->value_page_stride;
   a.v_hs = cache->value_head_stride;
-  a.v_ts = cache->value_token_stride;
+  a.k_ts = (uint32_t)(cache->key_token_stride * 2);
+  a.v_ts = (uint32_t)(cache->value_token_stride * 2);
   a.table = cache->block_table;
   a.table_stride = cache->table_stride;
   a.lengths = cache->lengths;
@@ -163,13 +675,22 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
   a.max_blocks = (int)cache->max_blocks;
   a.pages = (int)cache->pages;
   a.shift = page_shift(cache->page_size);
-  a.scale = scale;
+  a.scale = scale * kLog2e;
   a.out = static_cast<char*>(output);
-  const dim3 grid((unsigned)(cache->heads * group), (unsigned)cache->sequences);
-  const bool half = cache->dtype == RKV_F16;
+  a.min_tiles = 1;
+  char* ws = static_cast<char*>(workspace);
+  a.part_row = reinterpret_cast<int64_t*>(ws);
+  a.part_ml = reinterpret_cast<float2*>(ws + P.ml_off);
+  a.part_acc = reinterpret_cast<float*>(ws + P.acc_off);
+  const dim3 join((unsigned)P.grid, (unsigned)group);
   RKV_DISPATCH_DIM(cache->dim, D, {
-    if (half) paged_kernel<D, true><<<grid, dim3(kThreads), 0, stream>>>(a);
-    else paged_kernel<D, false><<<grid, dim3(kThreads), 0, stream>>>(a);
+    if (cache->dtype == RKV_F16) {
+      paged_kernel<D, true><<<dim3(P.grid), dim3(kThreads), 0, stream>>>(a);
+      paged_join_kernel<D, true><<<join, dim3(kThreads), 0, stream>>>(a, P.grid);
+    } else {
+      paged_kernel<D, false><<<dim3(P.grid), dim3(kThreads), 0, stream>>>(a);
+      paged_join_kernel<D, false><<<join, dim3(kThreads), 0, stream>>>(a, P.grid);
+    }
   });
   return check_launch("paged_kernel");
 }

@@ -305,7 +305,8 @@ def _decode_case(lengths, page, heads, group, dim, dtype, seed, peak=0.0, **over
     ([255, 256, 257], 256, 1, 16, 256, BF16), ([900, 100], 128, 3, 5, 160, F16),
     ([333, 1], 16, 2, 2, 96, BF16), ([500], 32, 1, 9, 192, F16), ([77, 400], 16, 1, 3, 224, BF16),
     ([50 + 13 * b for b in range(40)], 16, 2, 8, 64, BF16), ([4000], 16, 1, 1, 128, BF16),
-    ([3, 0] * 90, 16, 3, 2, 32, BF16),
+    ([3, 0] * 90, 16, 3, 2, 32, BF16), ([3, 0, 40] * 200, 16, 1, 2, 32, F16),
+    ([20000, 7], 16, 2, 3, 64, BF16), ([9000, 9000], 64, 3, 1, 256, BF16),
 ])
 def test_decode(lengths, page, heads, group, dim, dtype):
     case = _decode_case(lengths, page, heads, group, dim, dtype, seed=sum(lengths) + dim,
