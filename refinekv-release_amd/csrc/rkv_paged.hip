@@ -10,8 +10,14 @@
 namespace rkv {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
+constexpr int kJoinThreads = 256;
+// Waves of a workgroup: more of them share a row's parts in LDS, and leave
+// fewer parts for the join.
+#ifndef KW
+#define KW 8
+#endif
+template <int D>
+constexpr int kWavesOf = D <= 128 ? KW : 4;
 constexpr int kTileTokens = 32;  // tokens a wave takes at a time: two halves of 16
 
 typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
@@ -54,7 +60,7 @@ struct PagedArgs {
   int min_tiles;                 // tiles a wave takes at the least
   // a row (sequence, KV head) whose tiles lie in several workgroups: their
   // partial results, [workgroup][0: began before, 1: begins here]
-  int64_t* part_row;             // row, or -1
+  int* part_row;                 // row, or -1
   float2* part_ml;               // [..][group]
   float* part_acc;               // [..][group][D]
 };
@@ -87,14 +93,15 @@ struct Tile {
   uint32_t v2[8];
 };
 
-// A buffer view from `base` on, without an upper bound (the caller's offsets
-// stay inside a page); base must be wave-uniform.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t view_at(const char* base) {
+// A buffer view of `bytes` bytes at `base`, both wave-uniform; loads past it
+// return zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t view_of(const char* base, uint32_t bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a);
   const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo),
-                                           (short)0, (int)0x7fffffff, 0x00020000);
+                                           (short)0, (int)__builtin_amdgcn_readfirstlane(bytes),
+                                           0x00020000);
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -113,6 +120,22 @@ __device__ __forceinline__ int length_of(const PagedArgs& a, int n, bool& bad) {
   return bad || n < 0 ? 0 : n;
 }
 
+// Inclusive sum over the wave's lanes: within rows of 16 by row shifts, then
+// the rows' totals.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  const int lane = threadIdx.x % kWave;
+#define SHR(n) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x110 + n, 0xF, 0xF, false)
+  SHR(1);
+  SHR(2);
+  SHR(4);
+  SHR(8);
+#undef SHR
+  const uint32_t r0 = (uint32_t)__builtin_amdgcn_readlane((int)x, 15);
+  const uint32_t r1 = r0 + (uint32_t)__builtin_amdgcn_readlane((int)x, 31);
+  const uint32_t r2 = r1 + (uint32_t)__builtin_amdgcn_readlane((int)x, 47);
+  return x + (lane < 16 ? 0u : lane < 32 ? r0 : lane < 48 ? r1 : r2);
+}
+
 // Tiles of a sequence's row: one at least, so that every row has an owner
 // that writes its output.
 __device__ __forceinline__ int tiles_of(int length) {
@@ -123,8 +146,18 @@ __device__ __forceinline__ int tiles_of(int length) {
 // by KV head, tile by tile.
 struct Cursor {
   int b, h, tile, tiles, length;
+  int page0, page1;  // of the tile's two halves, as the table has them
   bool bad;
 };
+
+// The table's entries for the tile (any in-bounds entry for a half with no
+// token, whose page is not used).
+__device__ __forceinline__ void fetch_pages(const PagedArgs& a, Cursor& c) {
+  const int t0 = c.tile * kTileTokens, t1 = t0 + kTileTokens / 2;
+  const int64_t row = (int64_t)c.b * a.table_stride;
+  c.page0 = scalar_at(a.table, row + (t0 < c.length ? t0 >> a.shift : 0));
+  c.page1 = scalar_at(a.table, row + (t1 < c.length ? t1 >> a.shift : 0));
+}
 
 __device__ __forceinline__ void next_tile(const PagedArgs& a, Cursor& c) {
   if (++c.tile < c.tiles) return;
@@ -146,7 +179,7 @@ struct Part {
 };
 
 struct PartHead {
-  int64_t row;        // -1: unused
+  int row;            // -1: unused
   int begins, ends;   // the row's first / last tile is in the wave
 };
 
@@ -165,79 +198,59 @@ struct PartHead {
 //     transposes them with byte permutes; the m-th of 8 products takes dim
 //     8 (l % 16) + m for its row l % 16.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kThreads)
+__global__ __launch_bounds__(kWavesOf<D> * kWave)
 __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedArgs a) {
+  constexpr int kWaves = kWavesOf<D>, kThreads = kWaves * kWave;
   using T = Type16<kHalf>;
   using V8 = typename T::V8;
   using E = typename T::E;
   using P = Pieces<D>;
   __shared__ alignas(16) Part<D> parts[kWaves][2];
   __shared__ PartHead heads_s[kWaves][2];
-  __shared__ int64_t wave_sum[kWaves];
-  __shared__ int64_t start_s[kWaves], count_s[kWaves];
-  __shared__ int seq_s[kWaves];
-  __shared__ int64_t rest_s[kWaves];
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = uniform(tid / kWave);
   const int li = lane & 15, lg = lane >> 4;
-
-  // ---- this workgroup's share of the tiles
-  const int per = (a.sequences + kThreads - 1) / kThreads;
-  const int b0 = tid * per, b1 = min(b0 + per, a.sequences);
-  int64_t sum = 0;
-  for (int b = b0; b < b1; ++b) {
-    bool bad;
-    sum += tiles_of(length_of(a, a.lengths[b], bad));
-  }
-  sum *= a.heads;
-  int64_t before = sum;  // inclusive scan over the workgroup's threads
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int64_t x = __shfl_up(before, o, kWave);
-    before += lane >= o ? x : 0;
-  }
-  if (lane == kWave - 1) wave_sum[wave] = before;
   if (tid < kWaves * 2) heads_s[tid / 2][tid % 2].row = -1;
   __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += wave_sum[w];
-    total += wave_sum[w];
-  }
-  before -= sum;
-  int64_t waves = (int64_t)gridDim.x * kWaves;
-  const int64_t useful = (total + a.min_tiles - 1) / a.min_tiles;
-  waves = useful < waves ? useful : waves;
-  const int64_t share = total / waves, extra = total % waves;
-  for (int w = 0; w < kWaves; ++w) {
-    const int64_t id = (int64_t)blockIdx.x * kWaves + w;
-    const int64_t first = id * share + (id < extra ? id : extra);
-    const int64_t n = id < waves ? share + (id < extra ? 1 : 0) : 0;
-    if (tid == 0) count_s[w] = n;
-    if (n > 0 && first >= before && first < before + sum) {
-      int64_t rest = first - before;
-      int b = b0;
-      for (;; ++b) {
-        bool bad;
-        const int64_t here = (int64_t)tiles_of(length_of(a, a.lengths[b], bad)) * a.heads;
-        if (rest < here) break;
-        rest -= here;
-      }
-      seq_s[w] = b;
-      rest_s[w] = rest;
-    }
-  }
-  __syncthreads();
 
-  int64_t left = count_s[wave];
-  left = ((int64_t)uniform((int)(left >> 32)) << 32) | (uint32_t)uniform((int)left);
+  // ---- this wave's share of the tiles: every wave sums the lengths itself,
+  // each lane those of `per` sequences (no exchange between waves)
+  const int per = (a.sequences + kWave - 1) / kWave;
+  const int b0 = lane * per;
+  uint32_t sum = 0;
+#pragma unroll 4
+  for (int i = 0; i < per; ++i) {
+    const int b = b0 + i;
+    bool bad;
+    const int n = tiles_of(length_of(a, a.lengths[b < a.sequences ? b : a.sequences - 1], bad));
+    sum += b < a.sequences ? (uint32_t)n : 0u;
+  }
+  sum *= (uint32_t)a.heads;
+  const uint32_t upto = wave_scan(sum);  // tiles up to the lane's last sequence
+  const uint32_t total = (uint32_t)uniform((int)__shfl((int)upto, kWave - 1, kWave));
+  uint32_t waves = gridDim.x * kWaves;
+  const uint32_t useful = (total + (uint32_t)a.min_tiles - 1u) / (uint32_t)a.min_tiles;
+  waves = useful < waves ? useful : waves;
+  const uint32_t id = blockIdx.x * kWaves + (uint32_t)wave;
+  const uint32_t share = total / waves, extra = total % waves;
+  uint32_t left = id < waves ? share + (id < extra ? 1u : 0u) : 0u;
   if (left > 0) {
+    const uint32_t start = id * share + (id < extra ? id : extra);
+    const uint64_t after = __builtin_amdgcn_ballot_w64(upto > start);
+    const int owner = (int)__builtin_ctzll(after);  // the lane whose sequences hold the start
+    uint32_t rest = start - (uint32_t)uniform(__shfl((int)(upto - sum), owner, kWave));
     Cursor cur;
-    cur.b = uniform(seq_s[wave]);
-    cur.length = length_of(a, scalar_at(a.lengths, cur.b), cur.bad);
-    cur.tiles = tiles_of(cur.length);
-    const uint32_t rest = (uint32_t)uniform((int)rest_s[wave]);
+    cur.b = owner * per;
+    for (;; ++cur.b) {
+      cur.length = length_of(a, scalar_at(a.lengths, cur.b), cur.bad);
+      cur.tiles = tiles_of(cur.length);
+      const uint32_t here = (uint32_t)cur.tiles * (uint32_t)a.heads;
+      if (rest < here) break;
+      rest -= here;
+    }
     cur.h = (int)(rest / (uint32_t)cur.tiles);
     cur.tile = (int)(rest % (uint32_t)cur.tiles);
+    fetch_pages(a, cur);
 
     F32x4 acc[P::kBlocks];
     V8 q[D / 32];
@@ -246,51 +259,57 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
     bool bad_row = false;
     bool begun = false;  // the row's first tile was this wave's
 
+    // (query rows past the group read outside the view: zeros)
+    const uint32_t qo = li < a.group ? (uint32_t)li * (uint32_t)a.q_hs * 2u + (uint32_t)lg * 16u
+                                     : 0x80000000u;
     auto load_query = [&](const Cursor& c) {
-      const char* qp = a.query + ((int64_t)c.b * a.q_bs + (int64_t)(c.h * a.group + li) * a.q_hs
-                                  + lg * 8) * 2;
+      const auto qr = view_of(
+          a.query + ((int64_t)c.b * a.q_bs + (int64_t)c.h * a.group * a.q_hs) * 2,
+          (uint32_t)(a.group - 1) * (uint32_t)a.q_hs * 2u + D * 2u);
 #pragma unroll
       for (int j = 0; j < D / 32; ++j)
-        q_next[j] = li < a.group ? *reinterpret_cast<const U32x4*>(qp + j * 64)
-                                 : U32x4{0, 0, 0, 0};
+        q_next[j] = __builtin_amdgcn_raw_buffer_load_b128(qr, (int)(qo + 64u * j), 0, 0);
     };
 
-    auto load = [&](const Cursor& c, Tile<D>& t) -> bool {
+    // The loads of a tile, always as many (a tile or half that is not there
+    // reads through an empty view): a later wait for one tile then never
+    // waits for the next one's.
+    const uint32_t ko = (uint32_t)li * a.k_ts + (uint32_t)lg * 16u;
+    auto load = [&](const Cursor& c, Tile<D>& t, bool there) -> bool {
       bool bad = c.bad;
-      if (c.length == 0) return bad;
-      const int t0 = c.tile * kTileTokens;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        // a half behind the last token loads the first one's rows again
-        const int at = t0 + 16 * s < c.length ? t0 + 16 * s : t0;
-        int page = scalar_at(a.table, (int64_t)c.b * a.table_stride + (at >> a.shift));
-        if ((uint32_t)page >= (uint32_t)a.pages) {
-          bad = true;
-          page = 0;
-        }
-        const uint32_t in_page = (uint32_t)at & ((1u << a.shift) - 1u);
-        const auto kr = view_at(a.keys + ((int64_t)page * a.k_ps + (int64_t)c.h * a.k_hs) * 2
-                                + (uint64_t)in_page * a.k_ts);
-        const auto vr = view_at(a.values + ((int64_t)page * a.v_ps + (int64_t)c.h * a.v_hs) * 2
-                                + (uint64_t)in_page * a.v_ts);
-        const uint32_t ko = (uint32_t)li * a.k_ts + (uint32_t)lg * 16u;
+        const int at = c.tile * kTileTokens + 16 * s;
+        // rows of the half, those past the sequence's end left out
+        const int rows = there ? min(c.length - at, 16) : 0;
+        int page = s ? c.page1 : c.page0;
+        const bool out = (uint32_t)page >= (uint32_t)a.pages;
+        bad |= out && rows > 0;
+        page = out ? 0 : page;
+        const uint32_t in_page = rows > 0 ? (uint32_t)at & ((1u << a.shift) - 1u) : 0u;
+        const bool any = rows > 0 && !out;
+        const auto kr = view_of(a.keys + ((int64_t)page * a.k_ps + (int64_t)c.h * a.k_hs) * 2
+                                    + (uint64_t)in_page * a.k_ts,
+                                any ? (uint32_t)(rows - 1) * a.k_ts + D * 2u : 0u);
+        const auto vr = view_of(a.values + ((int64_t)page * a.v_ps + (int64_t)c.h * a.v_hs) * 2
+                                    + (uint64_t)in_page * a.v_ts,
+                                any ? (uint32_t)(rows - 1) * a.v_ts + D * 2u : 0u);
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
           t.k[s][j] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(ko + 64u * j), 0, 0);
-        const uint32_t vo = (uint32_t)(4 * lg) * a.v_ts;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int so = (int)(e * a.v_ts);
+          const uint32_t vo = (uint32_t)(4 * lg + e) * a.v_ts;
 #pragma unroll
           for (int c8 = 0; c8 < P::k8; ++c8)
             t.v8[c8][4 * s + e] = __builtin_amdgcn_raw_buffer_load_b128(
-                vr, (int)(vo + li * 16u + 256u * c8), so, 0);
+                vr, (int)(vo + li * 16u + 256u * c8), 0, 0);
           if constexpr (P::k4 > 0)
             t.v4[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b64(
-                vr, (int)(vo + li * 8u + 256u * P::k8), so, 0);
+                vr, (int)(vo + li * 8u + 256u * P::k8), 0, 0);
           if constexpr (P::k2 > 0)
             t.v2[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b32(
-                vr, (int)(vo + li * 4u + 256u * P::k8 + 128u * P::k4), so, 0);
+                vr, (int)(vo + li * 4u + 256u * P::k8 + 128u * P::k4), 0, 0);
         }
       }
       return bad;
@@ -309,7 +328,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
 
     auto compute = [&](const Cursor& c, Tile<D>& t, bool bad, bool last_tile) {
       bad_row |= bad;
-      if (c.length > 0) {
+      {
         float x[8];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -320,20 +339,12 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[4 * s + r] = s4[r] * a.scale;
         }
-        const int behind = c.length - c.tile * kTileTokens;  // tokens from the tile's first on
+        // rows behind the sequence's end were loaded as zeros and weigh nothing
+        const int behind = c.length - c.tile * kTileTokens;
         if (behind < kTileTokens) {
-          // the last tile: what lies behind the end weighs nothing, whatever
-          // its bytes are
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const bool live = 16 * (e / 4) + 4 * lg + e % 4 < behind;
-            x[e] = live ? x[e] : kNegInf;
-#pragma unroll
-            for (int c8 = 0; c8 < P::k8; ++c8)
-              t.v8[c8][e] = live ? t.v8[c8][e] : U32x4{0, 0, 0, 0};
-            if constexpr (P::k4 > 0) t.v4[e] = live ? t.v4[e] : U32x2{0, 0};
-            if constexpr (P::k2 > 0) t.v2[e] = live ? t.v2[e] : 0u;
-          }
+          for (int e = 0; e < 8; ++e)
+            x[e] = 16 * (e / 4) + 4 * lg + e % 4 < behind ? x[e] : kNegInf;
         }
         float top = x[0];
 #pragma unroll
@@ -402,12 +413,12 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
       xor32_pair(sum_l, u, w);
       sum_l = u + w;
       if (bad_row) sum_l = __builtin_nanf("");
-      const int64_t row = (int64_t)c.b * a.heads + c.h;
+      const int row = c.b * a.heads + c.h;
       if (begun && ends) {
         if (li < a.group) {
           // a sequence without tokens gives zeros
           const float by = c.length == 0 && !bad_row ? 0.0f : 1.0f / sum_l;
-          char* out = a.out + (row * a.group + li) * (D * 2);
+          char* out = a.out + ((int64_t)row * a.group + li) * (D * 2);
 #pragma unroll
           for (int n = 0; n < P::kBlocks; ++n)
 #pragma unroll
@@ -429,30 +440,34 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
     };
 
     Tile<D> t0, t1;
-    Cursor ahead = cur;
+    Cursor ahead = cur, far;  // the tile that is loading, and the one after it
     load_query(cur);
-    bool bad0 = load(cur, t0), bad1 = false;
+    bool bad0 = load(cur, t0, true), bad1 = false;
+    if (left > 1) {
+      next_tile(a, ahead);
+      fetch_pages(a, ahead);
+    }
     bool row_start = true;  // of the row, or of the wave's share of it
-    for (;;) {
+    auto step = [&](Tile<D>& now, bool bad, Tile<D>& next) -> bool {
       if (row_start) begin_row(cur);
-      if (left > 1) {
-        next_tile(a, ahead);
-        if (ahead.tile == 0) load_query(ahead);
-        bad1 = load(ahead, t1);
+      if (left > 1 && ahead.tile == 0) load_query(ahead);
+      far = ahead;
+      if (left > 2) {
+        next_tile(a, far);
+        fetch_pages(a, far);
       }
-      compute(cur, t0, bad0, left == 1);
-      if (--left == 0) break;
+      const bool next_bad = load(ahead, next, left > 1);
+      compute(cur, now, bad, left == 1);
       cur = ahead;
-      if (cur.tile == 0) begin_row(cur);
-      if (left > 1) {
-        next_tile(a, ahead);
-        if (ahead.tile == 0) load_query(ahead);
-        bad0 = load(ahead, t0);
-      }
-      compute(cur, t1, bad1, left == 1);
-      if (--left == 0) break;
-      cur = ahead;
+      ahead = far;
       row_start = cur.tile == 0;
+      return next_bad;
+    };
+    for (;;) {
+      bad1 = step(t0, bad0, t1);
+      if (--left == 0) break;
+      bad0 = step(t1, bad1, t0);
+      if (--left == 0) break;
     }
   }
   __syncthreads();
@@ -492,7 +507,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
         o += p.acc[g][d] * w;
       }
       if (whole) {
-        *reinterpret_cast<E*>(a.out + ((head.row * a.group + g) * D + d) * 2) = (E)(o / L);
+        *reinterpret_cast<E*>(a.out + (((int64_t)head.row * a.group + g) * D + d) * 2) = (E)(o / L);
       } else {
         a.part_acc[(to * a.group + g) * D + d] = o;
         if (d == 0) a.part_ml[to * a.group + g] = make_float2(M, L);
@@ -507,19 +522,20 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
 // query row g of the row that begins in the attention's workgroup k and goes
 // on in those after it.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedArgs a, int grid) {
-  constexpr int kStripes = kThreads / (D / 4) < 1 ? 1 : kThreads / (D / 4);
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedArgs a, int grid) {
+  constexpr int kStripes = kJoinThreads / (D / 4);
+  constexpr int kBatch = 8;
   __shared__ alignas(16) float acc_s[kStripes][D];
   __shared__ float2 ml_s[kStripes];
   const int k = blockIdx.x, g = blockIdx.y;
-  const int64_t row = a.part_row[2 * (int64_t)k + 1];
+  const int row = a.part_row[2 * k + 1];
   if (row < 0) return;
   // the workgroups after it whose first part is of the same row
   int n = 1;
   for (int j = k + 1; j < grid; j += kWave) {
     const int at = j + (int)(threadIdx.x % kWave);
     const uint64_t same =
-        __builtin_amdgcn_ballot_w64(at < grid && a.part_row[2 * (int64_t)at] == row);
+        __builtin_amdgcn_ballot_w64(at < grid && a.part_row[2 * at] == row);
     const int run = ~same ? __builtin_ctzll(~same) : kWave;
     n += run;
     if (run < kWave) break;
@@ -528,16 +544,31 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedArgs a, int g
   float m = kNegInf, l = 0.0f;
   F32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   if (stripe < kStripes) {
-    for (int j = stripe; j < n; j += kStripes) {
-      const int64_t at = (2 * (int64_t)(k + j) + (j == 0 ? 1 : 0)) * a.group + g;
-      const float2 ml = a.part_ml[at];
-      const F32x4 x = *reinterpret_cast<const F32x4*>(a.part_acc + at * D + 4 * c);
-      const float mn = __builtin_fmaxf(m, ml.x);
+    // parts in batches whose loads are all in flight before the first use
+    for (int j0 = stripe; j0 < n; j0 += kStripes * kBatch) {
+      float2 ml[kBatch];
+      F32x4 x[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int j = min(j0 + i * kStripes, n - 1);
+        const int64_t at = (2 * (int64_t)(k + j) + (j == 0 ? 1 : 0)) * a.group + g;
+        ml[i] = a.part_ml[at];
+        x[i] = *reinterpret_cast<const F32x4*>(a.part_acc + at * D + 4 * c);
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) mn = __builtin_fmaxf(mn, ml[i].x);
       const float old = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-      const float w = ml.x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
-      l = l * old + ml.y * w;
-      o = o * old + x * w;
+      l *= old;
+      o *= old;
       m = mn;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const bool there = j0 + i * kStripes < n;
+        const float w = ml[i].x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - mn);
+        l += there ? ml[i].y * w : 0.0f;
+        o += there ? x[i] * w : F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
     }
     *reinterpret_cast<F32x4*>(&acc_s[stripe][4 * c]) = o;
     if (c == 0) ml_s[stripe] = make_float2(m, l);
@@ -553,7 +584,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedArgs a, int g
     y += acc_s[j][d] * w;
   }
   using E = typename Type16<kHalf>::E;
-  *reinterpret_cast<E*>(a.out + ((row * a.group + g) * D + d) * 2) = (E)(y / L);
+  *reinterpret_cast<E*>(a.out + (((int64_t)row * a.group + g) * D + d) * 2) = (E)(y / L);
 }
 
 // Workgroups that the current device holds at once, 0 if unknown.
@@ -566,8 +597,8 @@ int paged_resident() {
   if (n == 0) {
     int cus = 0, per_cu = 0;
     if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, paged_kernel<D, kHalf>, kThreads,
-                                                     0) != hipSuccess)
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, paged_kernel<D, kHalf>,
+                                                     kWavesOf<D> * kWave, 0) != hipSuccess)
       return 0;
     n = cus * per_cu;
     of_dev[dev].store(n, std::memory_order_relaxed);
@@ -585,10 +616,10 @@ PagedPlan paged_plan(const rkv_paged_cache* c, int64_t group) {
   RKV_DISPATCH_DIM(c->dim, D, {
     P.grid = c->dtype == RKV_F16 ? paged_resident<D, true>() : paged_resident<D, false>();
   });
-  if (P.grid <= 0) P.grid = 512;
+  if (P.grid <= 0) P.grid = 256;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t parts = (size_t)P.grid * 2;
-  P.ml_off = up(parts * sizeof(int64_t));
+  P.ml_off = up(parts * sizeof(int));
   P.acc_off = P.ml_off + up(parts * group * sizeof(float2));
   P.total = P.acc_off + up(parts * group * c->dim * sizeof(float));
   return P;
@@ -609,9 +640,12 @@ int check_paged(const char* who, const rkv_paged_cache* c, int64_t group) {
                              c->value_page_stride, c->value_head_stride, c->value_token_stride};
   for (int64_t s : strides)
     if (s % 8) return set_error(kInvalidArgument, "%s: cache strides must be multiples of 8", who);
+  if (c->key_token_stride < c->dim || c->value_token_stride < c->dim)
+    return set_error(kInvalidArgument, "%s: row strides must be >= head_dim", who);
+  // tiles and rows are counted in 32 bits
   const int64_t tiles = c->max_blocks * c->page_size / kTileTokens + 1;
-  if (tiles > ((int64_t(1) << 31) - 1) / c->heads)
-    return set_error(kUnsupported, "%s: a sequence's table covers too many tokens", who);
+  if (tiles > ((int64_t(1) << 31) - 1) / c->heads / c->sequences)
+    return set_error(kUnsupported, "%s: the block table covers too many tokens", who);
   // 16 rows of a page are addressed with 32-bit byte offsets
   if (c->key_token_stride > (1 << 25) || c->value_token_stride > (1 << 25))
     return set_error(kUnsupported, "%s: rows more than 64 MiB apart", who);
@@ -644,6 +678,8 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
   const int rc = check_paged(who, cache, group);
   if (rc) return rc;
   if (!query || !output) return set_error(kInvalidArgument, "%s: null pointer argument", who);
+  if (q_sequence_stride < 0 || q_head_stride < 0 || q_head_stride > (1 << 25))
+    return set_error(kUnsupported, "%s: query stride", who);
   if (!aligned(query, 16) || !aligned(output, 16) || q_sequence_stride % 8 || q_head_stride % 8)
     return set_error(kInvalidArgument,
                      "%s: query and output must be 16-byte aligned with strides in multiples of 8",
@@ -679,17 +715,17 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
   a.out = static_cast<char*>(output);
   a.min_tiles = 1;
   char* ws = static_cast<char*>(workspace);
-  a.part_row = reinterpret_cast<int64_t*>(ws);
+  a.part_row = reinterpret_cast<int*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + P.ml_off);
   a.part_acc = reinterpret_cast<float*>(ws + P.acc_off);
   const dim3 join((unsigned)P.grid, (unsigned)group);
   RKV_DISPATCH_DIM(cache->dim, D, {
     if (cache->dtype == RKV_F16) {
-      paged_kernel<D, true><<<dim3(P.grid), dim3(kThreads), 0, stream>>>(a);
-      paged_join_kernel<D, true><<<join, dim3(kThreads), 0, stream>>>(a, P.grid);
+      paged_kernel<D, true><<<dim3(P.grid), dim3(kWavesOf<D> * kWave), 0, stream>>>(a);
+      paged_join_kernel<D, true><<<join, dim3(kJoinThreads), 0, stream>>>(a, P.grid);
     } else {
-      paged_kernel<D, false><<<dim3(P.grid), dim3(kThreads), 0, stream>>>(a);
-      paged_join_kernel<D, false><<<join, dim3(kThreads), 0, stream>>>(a, P.grid);
+      paged_kernel<D, false><<<dim3(P.grid), dim3(kWavesOf<D> * kWave), 0, stream>>>(a);
+      paged_join_kernel<D, false><<<join, dim3(kJoinThreads), 0, stream>>>(a, P.grid);
     }
   });
   return check_launch("paged_kernel");
