@@ -11,13 +11,18 @@ namespace rkv {
 namespace {
 
 constexpr int kJoinThreads = 256;
-// Waves of a workgroup: more of them share a row's parts in LDS, and leave
-// fewer parts for the join.
-#ifndef KW
-#define KW 8
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+#ifndef PERCU
+#define PERCU 1
+#define PERCU64 2
 #endif
+#ifndef AUX
+#define AUX 2
+#endif
+// Workgroups per CU that share the tiles.
 template <int D>
-constexpr int kWavesOf = D <= 128 ? KW : 4;
+constexpr int kPerCu = D <= 64 ? PERCU64 : PERCU;
 constexpr int kTileTokens = 32;  // tokens a wave takes at a time: two halves of 16
 
 typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
@@ -60,7 +65,8 @@ struct PagedArgs {
   int min_tiles;                 // tiles a wave takes at the least
   // a row (sequence, KV head) whose tiles lie in several workgroups: their
   // partial results, [workgroup][0: began before, 1: begins here]
-  int* part_row;                 // row, or -1
+  int2* open;                    // [workgroup]: the row that begins there (-1: none goes on
+                                 // behind it), the workgroups that hold parts of it
   float2* part_ml;               // [..][group]
   float* part_acc;               // [..][group][D]
 };
@@ -179,9 +185,56 @@ struct Part {
 };
 
 struct PartHead {
-  int row;            // -1: unused
-  int begins, ends;   // the row's first / last tile is in the wave
+  int row;              // -1: unused
+  int begins, ends;     // the row's first / last tile is in the wave
+  uint32_t from, tiles;  // the row's tiles in the list of all
 };
+
+// The (begin, count) of a wave's tiles in the list of all: an equal share each,
+// the first `extra` waves one more.
+struct Shares {
+  uint32_t share, extra;
+  __device__ __forceinline__ uint32_t begin(uint32_t id) const {
+    return id * share + (id < extra ? id : extra);
+  }
+  __device__ __forceinline__ uint32_t workgroup_of(uint32_t tile) const {
+    const uint32_t longer = extra * (share + 1u);
+    return (tile < longer ? tile / (share + 1u) : extra + (tile - longer) / share) / kWaves;
+  }
+};
+
+// Folds parts j = first, first + step, .. of n into (m, l, o): in batches whose
+// loads are all in flight before the first use.
+template <typename Ml, typename Acc>
+__device__ __forceinline__ void fold_parts(uint32_t first, uint32_t step, uint32_t n, float& m,
+                                           float& l, F32x4& o, Ml load_ml, Acc load_acc) {
+  constexpr uint32_t kBatch = 8;
+  for (uint32_t j0 = first; j0 < n; j0 += step * kBatch) {
+    float2 ml[kBatch];
+    float4 x[kBatch];
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i) {
+      const uint32_t j = min(j0 + i * step, n - 1u);
+      ml[i] = load_ml(j);
+      x[i] = load_acc(j);
+    }
+    float mn = m;
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i) mn = __builtin_fmaxf(mn, ml[i].x);
+    const float old = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    l *= old;
+    o *= old;
+    m = mn;
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i) {
+      const bool there = j0 + i * step < n;
+      const float w = ml[i].x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - mn);
+      // (a NaN sum stays one, whatever its weight)
+      l += there ? ml[i].y * w : 0.0f;
+      o += there ? F32x4{x[i].x, x[i].y, x[i].z, x[i].w} * w : F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+}
 
 // Every wave takes an equal, contiguous share of all tiles and walks it alone:
 // the keys and values of the next tile are loading while one is computed,
@@ -198,15 +251,16 @@ struct PartHead {
 //     transposes them with byte permutes; the m-th of 8 products takes dim
 //     8 (l % 16) + m for its row l % 16.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kWavesOf<D> * kWave)
+__global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedArgs a) {
-  constexpr int kWaves = kWavesOf<D>, kThreads = kWaves * kWave;
   using T = Type16<kHalf>;
   using V8 = typename T::V8;
   using E = typename T::E;
   using P = Pieces<D>;
   __shared__ alignas(16) Part<D> parts[kWaves][2];
   __shared__ PartHead heads_s[kWaves][2];
+  __shared__ float weight_s[kMaxGroup][16];
+  __shared__ float2 total_s[kMaxGroup];
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = uniform(tid / kWave);
   const int li = lane & 15, lg = lane >> 4;
@@ -232,10 +286,11 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
   const uint32_t useful = (total + (uint32_t)a.min_tiles - 1u) / (uint32_t)a.min_tiles;
   waves = useful < waves ? useful : waves;
   const uint32_t id = blockIdx.x * kWaves + (uint32_t)wave;
-  const uint32_t share = total / waves, extra = total % waves;
-  uint32_t left = id < waves ? share + (id < extra ? 1u : 0u) : 0u;
+  const Shares shares{total / waves, total % waves};
+  uint32_t left = id < waves ? shares.share + (id < shares.extra ? 1u : 0u) : 0u;
   if (left > 0) {
-    const uint32_t start = id * share + (id < extra ? id : extra);
+    const uint32_t start = shares.begin(id);
+    uint32_t pos = start;  // the computed tile's place in the list
     const uint64_t after = __builtin_amdgcn_ballot_w64(upto > start);
     const int owner = (int)__builtin_ctzll(after);  // the lane whose sequences hold the start
     uint32_t rest = start - (uint32_t)uniform(__shfl((int)(upto - sum), owner, kWave));
@@ -296,17 +351,17 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
                                 any ? (uint32_t)(rows - 1) * a.v_ts + D * 2u : 0u);
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
-          t.k[s][j] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(ko + 64u * j), 0, 0);
+          t.k[s][j] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(ko + 64u * j), 0, AUX);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t vo = (uint32_t)(4 * lg + e) * a.v_ts;
 #pragma unroll
           for (int c8 = 0; c8 < P::k8; ++c8)
             t.v8[c8][4 * s + e] = __builtin_amdgcn_raw_buffer_load_b128(
-                vr, (int)(vo + li * 16u + 256u * c8), 0, 0);
+                vr, (int)(vo + li * 16u + 256u * c8), 0, AUX);
           if constexpr (P::k4 > 0)
             t.v4[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b64(
-                vr, (int)(vo + li * 8u + 256u * P::k8), 0, 0);
+                vr, (int)(vo + li * 8u + 256u * P::k8), 0, AUX);
           if constexpr (P::k2 > 0)
             t.v2[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b32(
                 vr, (int)(vo + li * 4u + 256u * P::k8 + 128u * P::k4), 0, 0);
@@ -429,7 +484,8 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
       }
       const int slot = begun ? 1 : 0;
       Part<D>& part = parts[wave][slot];
-      if (lane == 0) heads_s[wave][slot] = PartHead{row, begun, ends};
+      if (lane == 0) heads_s[wave][slot] = PartHead{row, begun, ends, pos - (uint32_t)c.tile,
+                                                (uint32_t)c.tiles};
       if (li < a.group) {
         if (lg == 0) part.ml[li] = make_float2(m, sum_l);
 #pragma unroll
@@ -461,6 +517,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
       cur = ahead;
       ahead = far;
       row_start = cur.tile == 0;
+      ++pos;
       return next_bad;
     };
     for (;;) {
@@ -473,48 +530,68 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
   __syncthreads();
 
   // ---- the waves' parts of rows: neighbours of one row are joined, in order
-  if (tid == 0) {
-    a.part_row[(int64_t)blockIdx.x * 2] = -1;
-    a.part_row[(int64_t)blockIdx.x * 2 + 1] = -1;
-  }
-  for (int s = 0; s < 2 * kWaves;) {
-    const PartHead head = heads_s[s / 2][s % 2];
-    int e = s + 1;
-    if (head.row < 0) {
-      s = e;
-      continue;
+  if (tid == 0) a.open[blockIdx.x] = make_int2(-1, 0);
+  constexpr int kParts = 2 * kWaves;
+  const PartHead mine = heads_s[lane % kParts / 2][lane % 2];  // lane i: part i
+  const int my_row = lane < kParts ? mine.row : -1;
+  uint64_t todo = __builtin_amdgcn_ballot_w64(my_row >= 0);
+  while (todo) {
+    const int first = (int)__builtin_ctzll(todo);
+    const int row = __builtin_amdgcn_readlane(my_row, first);
+    const uint64_t same = __builtin_amdgcn_ballot_w64(my_row == row);
+    const int last = 63 - (int)__builtin_clzll(same), end = last + 1;
+    const bool begins = __builtin_amdgcn_readlane(mine.begins, first);
+    const bool ends = __builtin_amdgcn_readlane(mine.ends, last);
+    todo &= ~same;
+    const bool whole = begins && ends;
+    const int to = blockIdx.x * 2 + (begins ? 1 : 0);
+    // weights: lane i of 16 the row's part i of query row tid / 16
+    for (int at = tid; at < kMaxGroup * 16; at += kThreads) {
+      const int g = at / 16, i = at % 16;
+      const bool in = same >> i & 1;
+      const float2 ml = in ? parts[i / 2][i % 2].ml[g] : make_float2(kNegInf, 0.0f);
+      float M = ml.x;
+      M = __builtin_fmaxf(M, row_ror<8>(M));
+      M = __builtin_fmaxf(M, row_ror<4>(M));
+      M = __builtin_fmaxf(M, row_ror<2>(M));
+      M = __builtin_fmaxf(M, row_ror<1>(M));
+      const float w = ml.x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+      // (a NaN sum stays one, whatever its weight)
+      const float L = row16_sum_all(ml.y * w);
+      weight_s[g][i] = w;
+      if (i == 0) total_s[g] = make_float2(M, L);
     }
-    bool ends = head.ends;
-    for (; e < 2 * kWaves; ++e) {
-      const PartHead next = heads_s[e / 2][e % 2];
-      if (next.row >= 0 && next.row != head.row) break;
-      if (next.row >= 0) ends = next.ends;
-    }
-    const int64_t to = (int64_t)blockIdx.x * 2 + (head.begins ? 1 : 0);
-    const bool whole = head.begins && ends;
-    for (int x = tid; x < a.group * D; x += kThreads) {
-      const int g = x / D, d = x % D;
-      float M = kNegInf;
-      for (int i = s; i < e; ++i)
-        if (heads_s[i / 2][i % 2].row >= 0) M = __builtin_fmaxf(M, parts[i / 2][i % 2].ml[g].x);
-      float L = 0.0f, o = 0.0f;
-      for (int i = s; i < e; ++i) {
-        if (heads_s[i / 2][i % 2].row < 0) continue;
-        const Part<D>& p = parts[i / 2][i % 2];
-        const float w = p.ml[g].x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(p.ml[g].x - M);
-        // (a NaN sum stays one, whatever its weight)
-        L += p.ml[g].y * w;
-        o += p.acc[g][d] * w;
+    __syncthreads();
+    for (int x = tid; x < a.group * (D / 4); x += kThreads) {
+      const int g = x / (D / 4), d = x % (D / 4) * 4;
+      F32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+      for (int i = first; i < end; ++i) {
+        const float w = weight_s[g][i];
+        const F32x4 p = *reinterpret_cast<const F32x4*>(&parts[i / 2][i % 2].acc[g][d]);
+        o += w != 0.0f ? p * w : F32x4{0.0f, 0.0f, 0.0f, 0.0f};  // (an unused part holds anything)
       }
+      const float2 ml = total_s[g];
       if (whole) {
-        *reinterpret_cast<E*>(a.out + (((int64_t)head.row * a.group + g) * D + d) * 2) = (E)(o / L);
+        typedef E E4 __attribute__((ext_vector_type(4)));
+        const float by = 1.0f / ml.y;
+        E4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = (E)(o[r] * by);
+        *reinterpret_cast<E4*>(a.out + (((int64_t)row * a.group + g) * D + d) * 2) = y;
       } else {
-        a.part_acc[(to * a.group + g) * D + d] = o;
-        if (d == 0) a.part_ml[to * a.group + g] = make_float2(M, L);
+        const int64_t at = (int64_t)to * a.group + g;
+        *reinterpret_cast<F32x4*>(a.part_acc + at * D + d) = o;
+        if (d == 0) a.part_ml[at] = ml;
       }
     }
-    if (!whole && tid == 0) a.part_row[to] = head.row;
-    s = e;
+    if (begins && !ends && tid == 0) {
+      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane((int)mine.from, first);
+      const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane((int)mine.tiles, first);
+      const uint32_t to_last = shares.workgroup_of(from + tiles - 1u);
+      a.open[blockIdx.x] = make_int2(row, (int)(to_last - blockIdx.x + 1u));
+    }
+    if (todo) __syncthreads();
   }
 }
 
@@ -522,54 +599,26 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
 // query row g of the row that begins in the attention's workgroup k and goes
 // on in those after it.
 template <int D, bool kHalf>
-__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedArgs a, int grid) {
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedArgs a) {
   constexpr int kStripes = kJoinThreads / (D / 4);
-  constexpr int kBatch = 8;
   __shared__ alignas(16) float acc_s[kStripes][D];
   __shared__ float2 ml_s[kStripes];
   const int k = blockIdx.x, g = blockIdx.y;
-  const int row = a.part_row[2 * k + 1];
+  const int2 held = a.open[k];
+  const int row = held.x, n = held.y;
   if (row < 0) return;
-  // the workgroups after it whose first part is of the same row
-  int n = 1;
-  for (int j = k + 1; j < grid; j += kWave) {
-    const int at = j + (int)(threadIdx.x % kWave);
-    const uint64_t same =
-        __builtin_amdgcn_ballot_w64(at < grid && a.part_row[2 * at] == row);
-    const int run = ~same ? __builtin_ctzll(~same) : kWave;
-    n += run;
-    if (run < kWave) break;
-  }
   const int c = threadIdx.x % (D / 4), stripe = threadIdx.x / (D / 4);
   float m = kNegInf, l = 0.0f;
   F32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   if (stripe < kStripes) {
-    // parts in batches whose loads are all in flight before the first use
-    for (int j0 = stripe; j0 < n; j0 += kStripes * kBatch) {
-      float2 ml[kBatch];
-      F32x4 x[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int j = min(j0 + i * kStripes, n - 1);
-        const int64_t at = (2 * (int64_t)(k + j) + (j == 0 ? 1 : 0)) * a.group + g;
-        ml[i] = a.part_ml[at];
-        x[i] = *reinterpret_cast<const F32x4*>(a.part_acc + at * D + 4 * c);
-      }
-      float mn = m;
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) mn = __builtin_fmaxf(mn, ml[i].x);
-      const float old = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-      l *= old;
-      o *= old;
-      m = mn;
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const bool there = j0 + i * kStripes < n;
-        const float w = ml[i].x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - mn);
-        l += there ? ml[i].y * w : 0.0f;
-        o += there ? x[i] * w : F32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      }
-    }
+    auto part_at = [&](uint32_t j) {
+      return (2 * ((int64_t)k + j) + (j == 0 ? 1 : 0)) * a.group + g;
+    };
+    fold_parts((uint32_t)stripe, (uint32_t)kStripes, (uint32_t)n, m, l, o,
+               [&](uint32_t j) { return a.part_ml[part_at(j)]; },
+               [&](uint32_t j) {
+                 return *reinterpret_cast<const float4*>(a.part_acc + part_at(j) * D + 4 * c);
+               });
     *reinterpret_cast<F32x4*>(&acc_s[stripe][4 * c]) = o;
     if (c == 0) ml_s[stripe] = make_float2(m, l);
   }
@@ -587,20 +636,16 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(PagedArgs a, i
   *reinterpret_cast<E*>(a.out + (((int64_t)row * a.group + g) * D + d) * 2) = (E)(y / L);
 }
 
-// Workgroups that the current device holds at once, 0 if unknown.
-template <int D, bool kHalf>
-int paged_resident() {
+// Compute units of the current device, 256 if unknown.
+int compute_units() {
   static std::atomic<int> of_dev[64];  // per device; 0 = not asked yet
   int dev = -1;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
   int n = of_dev[dev].load(std::memory_order_relaxed);
   if (n == 0) {
-    int cus = 0, per_cu = 0;
-    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, paged_kernel<D, kHalf>,
-                                                     kWavesOf<D> * kWave, 0) != hipSuccess)
-      return 0;
-    n = cus * per_cu;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        n <= 0)
+      return 256;
     of_dev[dev].store(n, std::memory_order_relaxed);
   }
   return n;
@@ -613,13 +658,10 @@ struct PagedPlan {
 
 PagedPlan paged_plan(const rkv_paged_cache* c, int64_t group) {
   PagedPlan P;
-  RKV_DISPATCH_DIM(c->dim, D, {
-    P.grid = c->dtype == RKV_F16 ? paged_resident<D, true>() : paged_resident<D, false>();
-  });
-  if (P.grid <= 0) P.grid = 256;
+  RKV_DISPATCH_DIM(c->dim, D, P.grid = compute_units() * kPerCu<D>);
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t parts = (size_t)P.grid * 2;
-  P.ml_off = up(parts * sizeof(int));
+  P.ml_off = up(P.grid * sizeof(int2));
   P.acc_off = P.ml_off + up(parts * group * sizeof(float2));
   P.total = P.acc_off + up(parts * group * c->dim * sizeof(float));
   return P;
@@ -715,17 +757,17 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
   a.out = static_cast<char*>(output);
   a.min_tiles = 1;
   char* ws = static_cast<char*>(workspace);
-  a.part_row = reinterpret_cast<int*>(ws);
+  a.open = reinterpret_cast<int2*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + P.ml_off);
   a.part_acc = reinterpret_cast<float*>(ws + P.acc_off);
   const dim3 join((unsigned)P.grid, (unsigned)group);
   RKV_DISPATCH_DIM(cache->dim, D, {
     if (cache->dtype == RKV_F16) {
-      paged_kernel<D, true><<<dim3(P.grid), dim3(kWavesOf<D> * kWave), 0, stream>>>(a);
-      paged_join_kernel<D, true><<<join, dim3(kJoinThreads), 0, stream>>>(a, P.grid);
+      paged_kernel<D, true><<<dim3(P.grid), dim3(kThreads), 0, stream>>>(a);
+      paged_join_kernel<D, true><<<join, dim3(kJoinThreads), 0, stream>>>(a);
     } else {
-      paged_kernel<D, false><<<dim3(P.grid), dim3(kWavesOf<D> * kWave), 0, stream>>>(a);
-      paged_join_kernel<D, false><<<join, dim3(kJoinThreads), 0, stream>>>(a, P.grid);
+      paged_kernel<D, false><<<dim3(P.grid), dim3(kThreads), 0, stream>>>(a);
+      paged_join_kernel<D, false><<<join, dim3(kJoinThreads), 0, stream>>>(a);
     }
   });
   return check_launch("paged_kernel");
