@@ -5,7 +5,11 @@
 //   y0 = x0 c - x1 s,  y1 = x1 c + x0 s,  c = a cos t, s = a sin t,
 // with a the table's attention factor.  The half layout pairs dims i and
 // i + r/2, the interleaved one 2i and 2i + 1; dims from r on pass.  Memory
-// bound: every value is read and written once.
+// bound: every value is read and written once, at 5.7-5.8 TB/s for long
+// prompts (131001 tokens of 32 + 8 + 8 heads, d 128, 3.2 GB: 555 us; a copy of
+// 2 GiB by the device reaches 5.0 TB/s).  A cos and sin costs some 45
+// instructions a pair, so a thread that turned one head alone was bound by
+// them (862 us).
 #include "rkv_common.h"
 #include "rkv_internal.h"
 #include "rkv_paged.h"
@@ -14,6 +18,18 @@ namespace rkv {
 namespace {
 
 constexpr int kThreads = 256;
+// Heads of a thread's loads in flight together (1, 3 and 4 instead of 2: 64 K
+// tokens of 28 + 4 heads 194, 198 and 186 us against 187, 131001 tokens of 48
+// heads 611, 551 and 592 against 555, eight tokens of 40 heads 4.2, - and 5.1
+// against 4.2).
+constexpr int kBatch = 2;
+// A call that moves more than the caches hold stores past them (64 K tokens of
+// 28 + 4 heads, 537 MB written: 210 -> 198 us); what a smaller one writes is
+// left there for whoever reads it next.
+constexpr int64_t kStreamBytes = int64_t(64) << 20;
+// From so many threads on the device is full (4 waves per SIMD), and fewer
+// threads turn more heads each with the same cos and sin.
+constexpr int64_t kManyThreads = 4 * 1024 * 64;
 
 // A set of rows (token, head, dim): strides in elements, dim dense.
 struct Rows {
@@ -118,8 +134,10 @@ __device__ __forceinline__ Place place_of(const RotaryArgs& a, int64_t t) {
 // half layout: gap r/2; the interleaved one's pairs where no vector holds
 // whole ones: W 1, gap 1), one vector of W / 2 adjacent pairs (kAdjacent), or
 // one of W dims that pass.  It works out the item's cos and sin once and
-// applies them to every slots-th head of its token.
-template <typename T, int W, bool kAdjacent>
+// applies them to every slots-th head of its token, kBatch heads at a time
+// whose loads are all in flight before the first use; those of the first
+// batch are on their way before the position is known.
+template <typename T, int W, bool kAdjacent, bool kStream>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   constexpr int kPairs = kAdjacent ? W / 2 : W;
   constexpr int kSize = sizeof(T);
@@ -130,13 +148,34 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   const int slot = (int)(rest / (uint32_t)wide);
   const int64_t t = (int64_t)blockIdx.x * a.per_block + in_block;
   if (in_block >= a.per_block || t >= a.tokens) return;
-  const Place place = place_of(a, t);
+  Place place;
+  bool placed = false;
   for (int item = (int)(rest % (uint32_t)wide); item < a.items; item += kThreads) {
     const bool turns = item < a.turning;
     const int d0 = turns ? item * a.step : a.rotary_dim + (item - a.turning) * W;
     const bool two = turns && !kAdjacent;
+    V x[kBatch], z[kBatch];
+    // queries, then keys, then values
+    const int q_end = a.rows[0].heads, k_end = q_end + a.rows[1].heads;
+#define PICK(field) (q ? a.rows[0].field : v ? a.rows[2].field : a.rows[1].field)
+    auto load = [&](int n0) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int n = min(n0 + i * a.slots, a.heads - 1);
+        const bool q = n < q_end, v = n >= k_end;
+        const int h = n - (q ? 0 : v ? k_end : q_end);
+        const char* src = PICK(src) + (t * PICK(src_ts) + h * PICK(src_hs) + d0) * kSize;
+        x[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src));
+        if (two)
+          z[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + a.gap * kSize));
+      }
+    };
+    load(slot);
+    if (!placed) place = place_of(a, t);
+    placed = true;
+    const bool live = turns && place.live;
     float c[kPairs], s[kPairs];
-    if (turns && place.live) {
+    if (live) {
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         cos_sin((double)place.position * a.rates[item * kPairs + i], c[i], s[i]);
@@ -144,38 +183,47 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         s[i] *= a.scale * a.sign;
       }
     }
-    for (int n = slot; n < a.heads; n += a.slots) {
-      // queries, then keys, then values
-      const bool q = n < a.rows[0].heads, v = n >= a.rows[0].heads + a.rows[1].heads;
-      const int h = n - (q ? 0 : a.rows[0].heads) - (v ? a.rows[1].heads : 0);
-#define PICK(field) (q ? a.rows[0].field : v ? a.rows[2].field : a.rows[1].field)
-      if (PICK(paged) && place.page < 0) continue;
-      const char* src = PICK(src) + (t * PICK(src_ts) + h * PICK(src_hs) + d0) * kSize;
-      char* dst = PICK(dst) + ((PICK(paged) ? place.page * PICK(dst_ps) + place.row * PICK(dst_ts)
-                                            : t * PICK(dst_ts)) + h * PICK(dst_hs) + d0) * kSize;
-#undef PICK
-      V x = *reinterpret_cast<const V*>(src), z = x;
-      if (two) z = *reinterpret_cast<const V*>(src + a.gap * kSize);
-      if (turns && !v && place.live) {
+    for (int n0 = slot;;) {
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) {
-          float x0, x1;
-          if constexpr (kAdjacent) x0 = (float)x[2 * i], x1 = (float)x[2 * i + 1];
-          else x0 = (float)x[i], x1 = (float)z[i];
-          const float y0 = __builtin_fmaf(x0, c[i], -(x1 * s[i]));
-          const float y1 = __builtin_fmaf(x1, c[i], x0 * s[i]);
-          if constexpr (kAdjacent) {
-            x[2 * i] = (T)y0;
-            x[2 * i + 1] = (T)y1;
-          } else {
-            x[i] = (T)y0;
-            z[i] = (T)y1;
+      for (int i = 0; i < kBatch; ++i) {
+        const int n = n0 + i * a.slots;
+        const bool q = n < q_end, v = n >= k_end;
+        const int h = n - (q ? 0 : v ? k_end : q_end);
+        if (n >= a.heads || (PICK(paged) && place.page < 0)) continue;
+        if (live && !v) {
+#pragma unroll
+          for (int p = 0; p < kPairs; ++p) {
+            float x0, x1;
+            if constexpr (kAdjacent) x0 = (float)x[i][2 * p], x1 = (float)x[i][2 * p + 1];
+            else x0 = (float)x[i][p], x1 = (float)z[i][p];
+            const float y0 = __builtin_fmaf(x0, c[p], -(x1 * s[p]));
+            const float y1 = __builtin_fmaf(x1, c[p], x0 * s[p]);
+            if constexpr (kAdjacent) {
+              x[i][2 * p] = (T)y0;
+              x[i][2 * p + 1] = (T)y1;
+            } else {
+              x[i][p] = (T)y0;
+              z[i][p] = (T)y1;
+            }
           }
         }
+        char* dst = PICK(dst) + ((PICK(paged) ? place.page * PICK(dst_ps) + place.row * PICK(dst_ts)
+                                              : t * PICK(dst_ts)) + h * PICK(dst_hs) + d0) * kSize;
+        V* const to = reinterpret_cast<V*>(dst);
+        V* const to_z = reinterpret_cast<V*>(dst + a.gap * kSize);
+        if constexpr (kStream) {
+          __builtin_nontemporal_store(x[i], to);
+          if (two) __builtin_nontemporal_store(z[i], to_z);
+        } else {
+          *to = x[i];
+          if (two) *to_z = z[i];
+        }
       }
-      *reinterpret_cast<V*>(dst) = x;
-      if (two) *reinterpret_cast<V*>(dst + a.gap * kSize) = z;
+      n0 += kBatch * a.slots;
+      if (n0 >= a.heads) break;
+      load(n0);
     }
+#undef PICK
   }
 }
 
@@ -204,11 +252,22 @@ int launch_w(RotaryArgs& a, hipStream_t stream) {
   a.turning = half / (kAdjacent ? W / 2 : W);
   a.items = a.turning + (a.dim - a.rotary_dim) / W;
   const int wide = a.items < kThreads ? a.items : kThreads;
-  a.slots = kThreads / wide < a.heads ? kThreads / wide : a.heads;
+  // Few tokens: every thread kBatch heads, for latency.  Many: a wave holds
+  // one token's consecutive heads (d 128: 8 heads, 2 KB), each thread every
+  // 8th of them (against every 4th and 16th, 64 K tokens of 28 + 4 heads: 187
+  // against 197 and 200 us, 131001 of 48 heads 555 against 576 and 620).
+  a.slots = (a.heads + kBatch - 1) / kBatch;
+  if (a.tokens * wide * a.slots >= kManyThreads) a.slots = wide < kWave ? kWave / wide : 1;
+  a.slots = a.slots < a.heads ? a.slots : a.heads;
+  a.slots = a.slots < kThreads / wide ? a.slots : kThreads / wide;
   a.per_block = kThreads / (wide * a.slots);
   const int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
   if (blocks > 0x7fffffff) return set_error(kInvalidArgument, "rotary: too many tokens");
-  rotary_kernel<T, W, kAdjacent><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
+  const int64_t bytes = a.tokens * a.heads * a.dim * (int64_t)sizeof(T);
+  if (bytes >= kStreamBytes)
+    rotary_kernel<T, W, kAdjacent, true><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
+  else
+    rotary_kernel<T, W, kAdjacent, false><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
   return check_launch("rotary_kernel");
 }
 

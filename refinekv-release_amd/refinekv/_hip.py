@@ -14,7 +14,6 @@ variable ``REFINEKV_HIP_CHECK=1`` every ``decode`` call checks it (a host
 synchronization per call, so not under graph capture).
 """
 
-import contextlib
 import ctypes
 import os
 
@@ -543,100 +542,123 @@ def dense_decode(query, keys, values, length=None, workspace=None, output=None):
 # ---------------------------------------------------------------------------
 # Rotary positions and the paged cache
 # ---------------------------------------------------------------------------
+# (These calls are short: pointers and streams are passed as plain integers,
+# and what does not change between calls is read once.)
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
 
 def _dense_rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _rows_args(t):
-    """(pointer, token stride, head stride) of (tokens, heads, dim) rows."""
-    if t is None:
-        return None, 0, 0
-    return _ptr(t), t.stride(0), t.stride(1)
-
-
-def _on(device):
-    """The device's guard, for a call on another device than the current one."""
-    return (contextlib.nullcontext() if device.index == torch.cuda.current_device()
-            else torch.cuda.device(device))
+def _elsewhere(device):
+    """Whether the device is another than the current one."""
+    return device.index != torch.cuda.current_device()
 
 
 def rotary(query, key, positions, table, query_out=None, key_out=None, inverse=False):
     """rkv_rotary on checked (tokens, heads, dim) rows; returns (query, key)."""
-    device, config = query.device, table.config
-    query = _dense_rows(query)
+    device = query.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return rotary(query, key, positions, table, query_out, key_out, inverse)
+    query, config = _dense_rows(query), table.config
+    tokens, heads, dim = query.shape
     if query_out is None:
-        query_out = torch.empty(query.shape, device=device, dtype=query.dtype)
-    if key is not None:
-        key = _dense_rows(key)
+        query_out = torch.empty((tokens, heads, dim), device=device, dtype=query.dtype)
+    if key is None:
+        source, kv_heads, target = (0, 0, 0), 0, (0, 0, 0)
+    else:
+        key, kv_heads = _dense_rows(key), key.shape[1]
         if key_out is None:
-            key_out = torch.empty(key.shape, device=device, dtype=key.dtype)
+            key_out = torch.empty((tokens, kv_heads, dim), device=device, dtype=query.dtype)
+        source = (key.data_ptr(), key.stride(0), key.stride(1))
+        target = (key_out.data_ptr(), key_out.stride(0), key_out.stride(1))
     positions = positions.contiguous()
-    with _on(device):
-        rc = lib().rkv_rotary(
-            *_rows_args(query), query.shape[1], *_rows_args(key),
-            0 if key is None else key.shape[1], DTYPE_CODES[query.dtype], query.shape[0],
-            query.shape[2], _ptr(positions), positions.dtype == torch.int64, _ptr(table.turns),
-            config.rotary_dim, config.interleaved, table.scale, inverse, *_rows_args(query_out),
-            *_rows_args(key_out), _stream(device))
-    _check(rc, "rkv_rotary")
+    rc = lib().rkv_rotary(
+        query.data_ptr(), query.stride(0), query.stride(1), heads, *source, kv_heads,
+        DTYPE_CODES[query.dtype], tokens, dim, positions.data_ptr(),
+        positions.dtype == torch.int64, table.turns.data_ptr(), config.rotary_dim,
+        config.interleaved, table.scale, inverse, query_out.data_ptr(), query_out.stride(0),
+        query_out.stride(1), *target, _raw_stream(device))
+    if rc:
+        _check(rc, "rkv_rotary")
     return query_out, key_out
 
 
 def _cache_struct(cache):
-    """The C view of a PagedCache, made on its first call; its pointers are
-    taken from the tensors on every call."""
-    view = cache.__dict__.get("_hip_view")
-    if view is None:
+    """The C view of a PagedCache (made on its first call; the pointers are
+    taken from the tensors on every call) and a reference to it."""
+    made = cache.__dict__.get("_hip_view")
+    if made is None:
         view = _PagedCache(
             key_strides=(_i64 * 3)(*cache.keys.stride()[:3]),
             value_strides=(_i64 * 3)(*cache.values.stride()[:3]),
             table_stride=cache.block_table.stride(0), pages=cache.pages, heads=cache.heads,
             page_size=cache.page_size, dim=cache.head_dim, sequences=cache.sequences,
-            max_blocks=cache.max_blocks, dtype=DTYPE_CODES[cache.keys.dtype])
-        cache.__dict__["_hip_view"] = view
+            max_blocks=cache.max_blocks, dtype=DTYPE_CODES[cache.dtype])
+        made = cache.__dict__["_hip_view"] = (view, ctypes.byref(view))
+    view = made[0]
     view.keys, view.values = cache.keys.data_ptr(), cache.values.data_ptr()
     view.block_table, view.lengths = cache.block_table.data_ptr(), cache.lengths.data_ptr()
-    return view
+    return made[1]
 
 
 def paged_append(key, value, cache, query=None, table=None, token_starts=None, query_out=None):
     """rkv_paged_append on checked rows; returns the turned query or None."""
-    device = cache.keys.device
+    device = cache.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return paged_append(key, value, cache, query, table, token_starts, query_out)
     key, value = _dense_rows(key), _dense_rows(value)
+    rows = (0, 0, 0, 0, 0, 0, 0)
     if query is not None:
         query = _dense_rows(query)
         if query_out is None:
             query_out = torch.empty(query.shape, device=device, dtype=query.dtype)
-    if table is None:
-        turns = (None, 0, 0, 1.0)
-    else:
-        turns = (_ptr(table.turns), table.config.rotary_dim, table.config.interleaved, table.scale)
-    view = _cache_struct(cache)
-    with _on(device):
-        rc = lib().rkv_paged_append(
-            ctypes.byref(view), *_rows_args(query), 0 if query is None else query.shape[1],
-            *_rows_args(query_out), *_rows_args(key), *_rows_args(value), key.shape[0],
-            _ptr(token_starts), *turns, _stream(device))
-    _check(rc, "rkv_paged_append")
+        rows = (query.data_ptr(), query.stride(0), query.stride(1), query.shape[1],
+                query_out.data_ptr(), query_out.stride(0), query_out.stride(1))
+    turns = (0, 0, 0, 1.0) if table is None else (
+        table.turns.data_ptr(), table.config.rotary_dim, table.config.interleaved, table.scale)
+    rc = lib().rkv_paged_append(
+        _cache_struct(cache), *rows, key.data_ptr(), key.stride(0), key.stride(1),
+        value.data_ptr(), value.stride(0), value.stride(1), key.shape[0],
+        0 if token_starts is None else token_starts.data_ptr(), *turns, _raw_stream(device))
+    if rc:
+        _check(rc, "rkv_paged_append")
     return query_out
+
+
+def _paged_bytes(cache, group):
+    """Workspace bytes of paged_decode on the current device."""
+    sizes = cache.__dict__.setdefault("_hip_sizes", {})
+    if group not in sizes:
+        nbytes = _size()
+        _check(lib().rkv_paged_plan(_cache_struct(cache), group, ctypes.byref(nbytes)),
+               "rkv_paged_plan")
+        sizes[group] = nbytes.value
+    return sizes[group]
 
 
 def paged_decode(query, cache, scaling, workspace=None, output=None):
     """rkv_paged_decode on a checked (sequences, q_heads, dim) query."""
-    device, group = query.device, query.shape[1] // cache.heads
+    device = cache.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return paged_decode(query, cache, scaling, workspace, output)
+    group = query.shape[1] // cache.heads
     query = _row_aligned(query, 16)
     if output is None:
         output = torch.empty(query.shape, device=device, dtype=query.dtype)
-    view, nbytes = _cache_struct(cache), _size()
-    with _on(device):
-        _check(lib().rkv_paged_plan(ctypes.byref(view), group, ctypes.byref(nbytes)),
-               "rkv_paged_plan")
-        scratch = _buffer(workspace, "hip_paged_scratch", (nbytes.value,), device, torch.uint8)
-        rc = lib().rkv_paged_decode(ctypes.byref(view), _ptr(query), query.stride(0),
-                                    query.stride(1), group, scaling, _ptr(output), _ptr(scratch),
-                                    scratch.numel(), _stream(device))
-    _check(rc, "rkv_paged_decode")
+    scratch = _buffer(workspace, "hip_paged_scratch", (_paged_bytes(cache, group),), device,
+                      torch.uint8)
+    rc = lib().rkv_paged_decode(_cache_struct(cache), query.data_ptr(), query.stride(0),
+                                query.stride(1), group, scaling, output.data_ptr(),
+                                scratch.data_ptr(), scratch.numel(), _raw_stream(device))
+    if rc:
+        _check(rc, "rkv_paged_decode")
     return output
 
 

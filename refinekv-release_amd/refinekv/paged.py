@@ -16,13 +16,15 @@ serves every step of a batch.  ROCm tensors use the gfx950 kernels, others
 (and the types and shapes the kernels do not take) torch operations.
 """
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
+from . import _hip
 from .rotary import DTYPES, check_out, pick_backend, rows_overlap
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
+MAX_ROW_STRIDE = 1 << 25  # elements between a page's rows, at most
 
 
 @dataclass(frozen=True, eq=False)
@@ -41,6 +43,14 @@ class PagedCache:
     values: torch.Tensor
     block_table: torch.Tensor
     lengths: torch.Tensor
+    pages: int = field(init=False)
+    heads: int = field(init=False)
+    page_size: int = field(init=False)
+    head_dim: int = field(init=False)
+    sequences: int = field(init=False)
+    max_blocks: int = field(init=False)
+    dtype: torch.dtype = field(init=False)
+    device: torch.device = field(init=False)
 
     def __post_init__(self):
         keys, values, table, lengths = self.keys, self.values, self.block_table, self.lengths
@@ -66,6 +76,11 @@ class PagedCache:
             raise ValueError("lengths must be contiguous")
         if table.device != keys.device or lengths.device != keys.device:
             raise ValueError("block_table and lengths must be on the cache's device")
+        sizes = dict(zip(("pages", "heads", "page_size", "head_dim"), keys.shape),
+                     sequences=table.shape[0], max_blocks=table.shape[1], dtype=keys.dtype,
+                     device=keys.device)
+        for name, value in sizes.items():
+            object.__setattr__(self, name, value)
 
     @classmethod
     def empty(cls, pages, kv_heads, page_size, head_dim, sequences, max_blocks, *,
@@ -78,45 +93,21 @@ class PagedCache:
                    torch.zeros(sequences, dtype=torch.int32, device=device))
 
     @property
-    def pages(self):
-        return self.keys.shape[0]
-
-    @property
-    def heads(self):
-        return self.keys.shape[1]
-
-    @property
-    def page_size(self):
-        return self.keys.shape[2]
-
-    @property
-    def head_dim(self):
-        return self.keys.shape[3]
-
-    @property
-    def sequences(self):
-        return self.block_table.shape[0]
-
-    @property
-    def max_blocks(self):
-        return self.block_table.shape[1]
-
-    @property
     def capacity(self):
         """Tokens a sequence's row of the table can address."""
         return self.max_blocks * self.page_size
 
 
-def _check_rows(name, rows, cache, tokens=None):
-    if (rows.ndim != 3 or rows.shape[1] <= 0 or rows.shape[2] != cache.head_dim
-            or (tokens is not None and rows.shape[0] != tokens)):
-        raise ValueError(f"{name} must have shape (tokens, heads, head_dim) with the cache's "
-                         "head_dim and the key's tokens")
-    if rows.dtype != cache.keys.dtype or rows.device != cache.keys.device:
+def _check_rows(name, rows, cache, tokens, heads=None):
+    shape = rows.shape
+    if (len(shape) != 3 or shape[0] != tokens or shape[2] != cache.head_dim
+            or (shape[1] <= 0 if heads is None else shape[1] != heads)):
+        raise ValueError(f"{name} must have shape (tokens, heads, head_dim) with the key's "
+                         "tokens and the cache's head_dim and, keys and values, heads")
+    if rows.dtype != cache.dtype or rows.device != cache.device:
         raise ValueError(f"{name} must have the cache's dtype and device")
 
 
-@torch.no_grad()
 def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=None,
                  query_out=None, backend="auto"):
     """Write new (tokens, kv_heads, head_dim) keys and values to their
@@ -134,17 +125,15 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     stored.  No two rows of a call may fall on the same place: a page written
     here belongs to one sequence.
     """
-    _check_rows("key", key, cache)
-    _check_rows("value", value, cache, key.shape[0])
-    if key.shape[1] != cache.heads or value.shape[1] != cache.heads:
-        raise ValueError("key and value must have the cache's heads")
-    device = cache.keys.device
+    tokens, device = key.shape[0] if key.ndim else 0, cache.device
+    _check_rows("key", key, cache, tokens, cache.heads)
+    _check_rows("value", value, cache, tokens, cache.heads)
     if token_starts is not None:
         if (token_starts.shape != (cache.sequences + 1,) or token_starts.dtype != torch.int32
                 or token_starts.device != device or not token_starts.is_contiguous()):
             raise ValueError("token_starts must be contiguous int32 with shape (sequences + 1,) "
                              "on the cache's device")
-    elif key.shape[0] != cache.sequences:
+    elif tokens != cache.sequences:
         raise ValueError("without token_starts there is one token per sequence")
     if rotary is not None and (rotary.config.head_dim != cache.head_dim
                                or rotary.device != device):
@@ -152,38 +141,46 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     if query is not None:
         if rotary is None:
             raise ValueError("a query is only taken to be turned: pass rotary")
-        _check_rows("query", query, cache, key.shape[0])
+        _check_rows("query", query, cache, tokens)
         if query_out is not None:
             check_out("query_out", query_out, query, (key, value))
     elif query_out is not None:
         raise ValueError("query_out without a query")
     if pick_backend(key, backend, key.dtype in DTYPES,
                     "the HIP append needs a bf16, fp16 or fp32 cache") == "hip":
-        from . import _hip
-
         return _hip.paged_append(key, value, cache, query, rotary, token_starts, query_out)
     from .reference_paged import append
 
-    turned = append(cache, key, value, query, rotary, token_starts)
-    return turned if query_out is None else query_out.copy_(turned)
+    with torch.no_grad():
+        turned = append(cache, key, value, query, rotary, token_starts)
+        return turned if query_out is None else query_out.copy_(turned)
 
 
-def _decode_support(query, cache):
-    """None, or why the HIP kernel does not take the call."""
-    from . import _hip
+def _decode_support(cache, group):
+    """None, or why the HIP kernel does not take the cache with this group;
+    looked up once (a frozen cache's tensors keep their layout)."""
+    known = cache.__dict__.setdefault("_hip_support", {})
+    if group not in known:
+        known[group] = _why_not(cache, group)
+    return known[group]
 
-    group = query.shape[1] // cache.heads
-    if cache.keys.dtype not in (torch.bfloat16, torch.float16):
+
+def _why_not(cache, group):
+    dim = cache.head_dim
+    if cache.dtype not in (torch.bfloat16, torch.float16):
         return "the HIP paged decode needs a bf16 or fp16 cache"
-    if cache.head_dim not in _hip.SUPPORTED_DIMS or group > _hip.MAX_GROUP:
+    if dim not in _hip.SUPPORTED_DIMS or group > _hip.MAX_GROUP:
         return "the HIP paged decode needs head_dim in 32..256 (multiple of 32) and group <= 16"
     for t in (cache.keys, cache.values):
         if t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]):
             return "the HIP paged decode needs a cache of 16-byte aligned rows"
+        if not dim <= t.stride(2) <= MAX_ROW_STRIDE:
+            return "the HIP paged decode needs rows apart from each other, and not too far"
+    if cache.sequences * cache.heads * (cache.capacity // 32 + 1) >= 2 ** 31:
+        return "the HIP paged decode needs a block table of fewer tokens"
     return None
 
 
-@torch.no_grad()
 def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, backend="auto"):
     """Attention of one new token per sequence over its visible tokens.
 
@@ -197,7 +194,8 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
     among its visible ones, or a length past its table, gives NaN.
     """
     _check_rows("query", query, cache, cache.sequences)
-    if query.shape[1] % cache.heads:
+    group = query.shape[1] // cache.heads
+    if query.shape[1] != group * cache.heads:
         raise ValueError("query heads must be a multiple of the cache's heads")
     if output is not None:
         if (output.shape != query.shape or output.dtype != query.dtype
@@ -206,12 +204,11 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
         if rows_overlap(output, query):
             raise ValueError("output must not overlap the query")
     scaling = cache.head_dim ** -0.5 if scaling is None else float(scaling)
-    why = _decode_support(query, cache) if query.is_cuda else None
+    why = _decode_support(cache, group) if query.is_cuda else None
     if pick_backend(query, backend, why is None, why) == "hip":
-        from . import _hip
-
         return _hip.paged_decode(query, cache, scaling, workspace, output)
     from .reference_paged import decode
 
-    out = decode(query, cache, scaling)
-    return out if output is None else output.copy_(out)
+    with torch.no_grad():
+        out = decode(query, cache, scaling)
+        return out if output is None else output.copy_(out)

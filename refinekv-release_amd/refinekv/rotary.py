@@ -16,6 +16,7 @@ import math
 
 import torch
 
+from . import _hip
 from .config import BACKENDS, KERNEL_BACKENDS
 
 SCALINGS = ("none", "linear", "ntk", "llama3", "yarn")
@@ -142,8 +143,6 @@ def pick_backend(tensor, backend, supported, why):
     """"hip" or "torch" for a call on ``tensor``: the kernels where they run
     (``supported``; an explicit request otherwise raises ``why``), never a
     silent fallback for a missing library on a GPU."""
-    from . import _hip
-
     if backend not in BACKENDS:
         raise ValueError("backend must be 'auto', 'torch', 'hip', or 'triton'")
     if backend == "torch":
@@ -203,7 +202,6 @@ def check_out(name, out, like, others=()):
             raise ValueError(f"{name} overlaps an input or output of the call")
 
 
-@torch.no_grad()
 def rotate_heads(query, key, positions, rotary, *, query_out=None, key_out=None, inverse=False,
                  backend="auto"):
     """Turn (tokens, heads, head_dim) query and key rows to their positions.
@@ -238,15 +236,14 @@ def rotate_heads(query, key, positions, rotary, *, query_out=None, key_out=None,
         check_out("key_out", key_out, key, [query])
     if pick_backend(query, backend, query.dtype in DTYPES,
                     "the HIP rotation needs bf16, fp16 or fp32 rows") == "hip":
-        from . import _hip
-
         return _hip.rotary(query, key, positions, rotary, query_out, key_out, inverse)
     from .reference_paged import rotate
 
     rows = []
-    for x, out in ((query, query_out), (key, key_out)):
-        if x is not None:
-            y = rotate(x, positions, rotary, inverse)
-            x = y if out is None else out.copy_(y)
-        rows.append(x)
+    with torch.no_grad():
+        for x, out in ((query, query_out), (key, key_out)):
+            if x is not None:
+                y = rotate(x, positions, rotary, inverse)
+                x = y if out is None else out.copy_(y)
+            rows.append(x)
     return tuple(rows)
