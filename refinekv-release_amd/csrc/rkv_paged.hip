@@ -2,6 +2,7 @@
 //   out[b, h, g] = softmax_t(scale q[b, h, g] . K[t]) V,  t < lengths[b],
 // token t of KV head h at row t % P of page table[b][t / P].
 #include <atomic>
+#include <type_traits>
 
 #include "rkv_common.h"
 #include "rkv_internal.h"
@@ -62,7 +63,6 @@ struct PagedArgs {
   int sequences, heads, group, max_blocks, pages, shift;
   float scale;                   // times log2 e: the softmax runs on 2^x
   char* out;                     // (B, H G, D) dense
-  int min_tiles;                 // tiles a wave takes at the least
   // a row (sequence, KV head) whose tiles lie in several workgroups: their
   // partial results, [workgroup][0: began before, 1: begins here]
   int2* open;                    // [workgroup]: the row that begins there (-1: none goes on
@@ -79,13 +79,15 @@ struct Pieces {
   static constexpr int k4 = D % 128 >= 64 ? 1 : 0;
   static constexpr int k2 = D % 64 >= 32 ? 1 : 0;
   static constexpr int kBlocks = D / 16;  // 16-dim matrix products: 8 k8 + 4 k4 + 2 k2
-  // first dim of lane column i's piece of product m, and the dim in it
-  static __device__ __forceinline__ int dim(int m, int i) {
-    if (m < 8 * k8) return (m / 8) * 128 + i * 8 + m % 8;
-    m -= 8 * k8;
-    if (m < 4 * k4) return 128 * k8 + i * 4 + m;
-    m -= 4 * k4;
-    return 128 * k8 + 64 * k4 + i * 2 + m;
+  // Calls put(first product, first dim, size as an integral constant) for each
+  // piece of lane column i: the products' dims are consecutive there.
+  template <typename Put>
+  static __device__ __forceinline__ void each(int i, Put put) {
+#pragma unroll
+    for (int c = 0; c < k8; ++c) put(8 * c, 128 * c + i * 8, std::integral_constant<int, 8>());
+    if constexpr (k4 > 0) put(8 * k8, 128 * k8 + i * 4, std::integral_constant<int, 4>());
+    if constexpr (k2 > 0)
+      put(8 * k8 + 4 * k4, 128 * k8 + 64 * k4 + i * 2, std::integral_constant<int, 2>());
   }
 };
 
@@ -283,8 +285,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
   const uint32_t upto = wave_scan(sum);  // tiles up to the lane's last sequence
   const uint32_t total = (uint32_t)uniform((int)__shfl((int)upto, kWave - 1, kWave));
   uint32_t waves = gridDim.x * kWaves;
-  const uint32_t useful = (total + (uint32_t)a.min_tiles - 1u) / (uint32_t)a.min_tiles;
-  waves = useful < waves ? useful : waves;
+  waves = total < waves ? total : waves;
   const uint32_t id = blockIdx.x * kWaves + (uint32_t)wave;
   const Shares shares{total / waves, total % waves};
   uint32_t left = id < waves ? shares.share + (id < shares.extra ? 1u : 0u) : 0u;
@@ -475,10 +476,14 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
           const float by = c.length == 0 && !bad_row ? 0.0f : 1.0f / sum_l;
           char* out = a.out + ((int64_t)row * a.group + li) * (D * 2);
 #pragma unroll
-          for (int n = 0; n < P::kBlocks; ++n)
+          for (int r = 0; r < 4; ++r)
+            P::each(4 * lg + r, [&](int n0, int d, auto size) {
+              typedef E EN __attribute__((ext_vector_type(size())));
+              EN y;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              *reinterpret_cast<E*>(out + P::dim(n, 4 * lg + r) * 2) = (E)(acc[n][r] * by);
+              for (int i = 0; i < size(); ++i) y[i] = (E)(acc[n0 + i][r] * by);
+              *reinterpret_cast<EN*>(out + d * 2) = y;
+            });
         }
         return;
       }
@@ -489,9 +494,18 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
       if (li < a.group) {
         if (lg == 0) part.ml[li] = make_float2(m, sum_l);
 #pragma unroll
-        for (int n = 0; n < P::kBlocks; ++n)
+        for (int r = 0; r < 4; ++r)
+          P::each(4 * lg + r, [&](int n0, int d, auto size) {
+            constexpr int kN = size() < 4 ? size() : 4;
+            typedef float FN __attribute__((ext_vector_type(kN)));
 #pragma unroll
-          for (int r = 0; r < 4; ++r) part.acc[li][P::dim(n, 4 * lg + r)] = acc[n][r];
+            for (int i = 0; i < size(); i += kN) {
+              FN y;
+#pragma unroll
+              for (int j = 0; j < kN; ++j) y[j] = acc[n0 + i + j][r];
+              *reinterpret_cast<FN*>(&part.acc[li][d + i]) = y;
+            }
+          });
       }
     };
 
@@ -755,7 +769,6 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
   a.shift = page_shift(cache->page_size);
   a.scale = scale * kLog2e;
   a.out = static_cast<char*>(output);
-  a.min_tiles = 1;
   char* ws = static_cast<char*>(workspace);
   a.open = reinterpret_cast<int2*>(ws);
   a.part_ml = reinterpret_cast<float2*>(ws + P.ml_off);

@@ -130,16 +130,18 @@ __device__ __forceinline__ Place place_of(const RotaryArgs& a, int64_t t) {
   return p;
 }
 
-// A thread holds one item of a row: two vectors of W dims `gap` apart (the
-// half layout: gap r/2; the interleaved one's pairs where no vector holds
-// whole ones: W 1, gap 1), one vector of W / 2 adjacent pairs (kAdjacent), or
-// one of W dims that pass.  It works out the item's cos and sin once and
+// A thread holds one item of a row, two vectors of W dims: in the half layout
+// r/2 apart (W pairs), in the interleaved one side by side (kAdjacent: W / 2
+// pairs each; W 1: one pair), and side by side too where dims pass.  A part
+// that is an odd number of vectors has one in its last item.  (One vector an
+// item where dims pass: 50266 tokens of 28 + 4 heads, 64 of 128 dims turning,
+// 207 us.)  The thread works out the item's cos and sin once and
 // applies them to every slots-th head of its token, kBatch heads at a time
 // whose loads are all in flight before the first use; those of the first
 // batch are on their way before the position is known.
 template <typename T, int W, bool kAdjacent, bool kStream>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
-  constexpr int kPairs = kAdjacent ? W / 2 : W;
+  constexpr int kPairs = W;
   constexpr int kSize = sizeof(T);
   typedef T V __attribute__((ext_vector_type(W)));
   const int wide = a.items < kThreads ? a.items : kThreads;
@@ -152,8 +154,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   bool placed = false;
   for (int item = (int)(rest % (uint32_t)wide); item < a.items; item += kThreads) {
     const bool turns = item < a.turning;
-    const int d0 = turns ? item * a.step : a.rotary_dim + (item - a.turning) * W;
-    const bool two = turns && !kAdjacent;
+    const int d0 = turns ? item * a.step : a.rotary_dim + (item - a.turning) * (2 * W);
+    const int gap = turns ? a.gap : W;
+    const bool two = turns ? !kAdjacent || d0 + W < a.rotary_dim : d0 + W < a.dim;
     V x[kBatch], z[kBatch];
     // queries, then keys, then values
     const int q_end = a.rows[0].heads, k_end = q_end + a.rows[1].heads;
@@ -167,7 +170,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         const char* src = PICK(src) + (t * PICK(src_ts) + h * PICK(src_hs) + d0) * kSize;
         x[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src));
         if (two)
-          z[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + a.gap * kSize));
+          z[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + gap * kSize));
       }
     };
     load(slot);
@@ -178,7 +181,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     if (live) {
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
-        cos_sin((double)place.position * a.rates[item * kPairs + i], c[i], s[i]);
+        // (the pairs of a second vector that is not there are not read)
+        const int pair = item * kPairs + (kAdjacent && i >= W / 2 && !two ? 0 : i);
+        cos_sin((double)place.position * a.rates[pair], c[i], s[i]);
         c[i] *= a.scale;
         s[i] *= a.scale * a.sign;
       }
@@ -194,13 +199,15 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
 #pragma unroll
           for (int p = 0; p < kPairs; ++p) {
             float x0, x1;
-            if constexpr (kAdjacent) x0 = (float)x[i][2 * p], x1 = (float)x[i][2 * p + 1];
+            V& pairs = p < W / 2 ? x[i] : z[i];
+            const int at = p % (W / 2 > 0 ? W / 2 : 1) * 2;
+            if constexpr (kAdjacent) x0 = (float)pairs[at], x1 = (float)pairs[at + 1];
             else x0 = (float)x[i][p], x1 = (float)z[i][p];
             const float y0 = __builtin_fmaf(x0, c[p], -(x1 * s[p]));
             const float y1 = __builtin_fmaf(x1, c[p], x0 * s[p]);
             if constexpr (kAdjacent) {
-              x[i][2 * p] = (T)y0;
-              x[i][2 * p + 1] = (T)y1;
+              pairs[at] = (T)y0;
+              pairs[at + 1] = (T)y1;
             } else {
               x[i][p] = (T)y0;
               z[i][p] = (T)y1;
@@ -210,7 +217,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
         char* dst = PICK(dst) + ((PICK(paged) ? place.page * PICK(dst_ps) + place.row * PICK(dst_ts)
                                               : t * PICK(dst_ts)) + h * PICK(dst_hs) + d0) * kSize;
         V* const to = reinterpret_cast<V*>(dst);
-        V* const to_z = reinterpret_cast<V*>(dst + a.gap * kSize);
+        V* const to_z = reinterpret_cast<V*>(dst + gap * kSize);
         if constexpr (kStream) {
           __builtin_nontemporal_store(x[i], to);
           if (two) __builtin_nontemporal_store(z[i], to_z);
@@ -249,8 +256,8 @@ int vector_bytes(const RotaryArgs& a, int size, bool interleaved) {
 template <typename T, int W, bool kAdjacent>
 int launch_w(RotaryArgs& a, hipStream_t stream) {
   const int half = a.rotary_dim / 2;
-  a.turning = half / (kAdjacent ? W / 2 : W);
-  a.items = a.turning + (a.dim - a.rotary_dim) / W;
+  a.turning = kAdjacent ? (half + W - 1) / W : half / W;
+  a.items = a.turning + (a.dim - a.rotary_dim + 2 * W - 1) / (2 * W);
   const int wide = a.items < kThreads ? a.items : kThreads;
   // Few tokens: every thread kBatch heads, for latency.  Many: a wave holds
   // one token's consecutive heads (d 128: 8 heads, 2 KB), each thread every
@@ -276,8 +283,8 @@ int launch_t(RotaryArgs& a, bool interleaved, hipStream_t stream) {
   constexpr int kSize = sizeof(T);
   const int bytes = vector_bytes(a, kSize, interleaved);
   if (interleaved && bytes > kSize) {
-    a.gap = 0;
-    a.step = bytes / kSize;
+    a.gap = bytes / kSize;
+    a.step = 2 * a.gap;
     return bytes == 16 ? launch_w<T, 16 / kSize, true>(a, stream)
                        : launch_w<T, 8 / kSize, true>(a, stream);
   }
