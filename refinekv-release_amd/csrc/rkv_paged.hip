@@ -1,6 +1,14 @@
 // Attention of one new token per sequence over a paged KV cache:
 //   out[b, h, g] = softmax_t(scale q[b, h, g] . K[t]) V,  t < lengths[b],
 // token t of KV head h at row t % P of page table[b][t / P].
+//
+// Two launches: paged_kernel attends, paged_join_kernel joins the rows that
+// several workgroups hold parts of.  (One launch whose last workgroup of a row
+// joined it, through counters and stores past the caches, was as fast at best:
+// one sequence of 2003 tokens 13.0 us against 12.5, of 131072 91.4 against
+// 91.8, 128 short ones at head_dim 64 75 against 72.)  Sums, maxima and
+// accumulators are fp32; the partition into shares depends on the batch's
+// lengths and the device alone, so a call repeats bit for bit.
 #include <atomic>
 #include <type_traits>
 
@@ -11,20 +19,25 @@
 namespace rkv {
 namespace {
 
-constexpr int kJoinThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-#ifndef PERCU
-#define PERCU 1
-#define PERCU64 2
-#endif
-#ifndef AUX
-#define AUX 2
-#endif
-// Workgroups per CU that share the tiles.
-template <int D>
-constexpr int kPerCu = D <= 64 ? PERCU64 : PERCU;
+constexpr int kJoinThreads = 256;
 constexpr int kTileTokens = 32;  // tokens a wave takes at a time: two halves of 16
+
+// Workgroups per CU that share the tiles.  One keeps the CU's loads full (each
+// of its waves has two tiles on their way) and leaves the fewest parts to
+// join; at head_dim 32 a tile is 4 KB and two are needed (64 sequences of up
+// to 20000 tokens 77.5 -> 67.5 us; head_dim 64, 8 x 60000 tokens 165 -> 167,
+// 96, 100000 tokens 35.9 -> 37.9, 128, 131072 tokens 92.2 -> 93.4).
+template <int D>
+constexpr int kPerCu = D < 64 ? 2 : 1;
+
+// Cache policy of the key and value loads: non-temporal.  A token is read once
+// a step, and kept lines only push out others: 16 x 131072 tokens 1470 -> 1327
+// us, one 103.5 -> 92, 64 ragged ones 112 -> 100.  (Sequences that share most
+// of their pages lose what the caches would have held: 16 on the same 32768
+// tokens 172 -> 276 us, 64 on the same 4096 95 -> 99; the call cannot know.)
+constexpr int kStreamLoad = 2;
 
 typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
@@ -172,8 +185,8 @@ __device__ __forceinline__ void next_tile(const PagedArgs& a, Cursor& c) {
   c.tile = 0;
   if (++c.h < a.heads) return;
   c.h = 0;
-  ++c.b;
-  if (c.b < a.sequences) {
+  if (c.b + 1 < a.sequences) {
+    ++c.b;
     c.length = length_of(a, scalar_at(a.lengths, c.b), c.bad);
     c.tiles = tiles_of(c.length);
   }
@@ -240,9 +253,10 @@ __device__ __forceinline__ void fold_parts(uint32_t first, uint32_t step, uint32
 
 // Every wave takes an equal, contiguous share of all tiles and walks it alone:
 // the keys and values of the next tile are loading while one is computed,
-// across rows' ends too.  A tile is 32 tokens, all of S^T = K Q^T and
-// O^T = V^T P^T on the matrix cores with the query rows in the columns, so
-// that a lane's maximum, sum and accumulators all belong to query row l % 16:
+// across rows' ends too, so that ragged batches stream like long ones.  A
+// tile's S^T = K Q^T and O^T = V^T P^T run on the matrix cores with the query
+// rows in the columns, so that a lane's maximum, sum and accumulators all
+// belong to query row l % 16:
 //   S^T: A = 16 key rows straight from memory (lane l: row l % 16, dims
 //     8 (l / 16) + 32 j ..), B = the query rows; the result in lane l is
 //     S[t = 4 (l / 16) + r][l % 16], r = 0..3.
@@ -251,7 +265,12 @@ __device__ __forceinline__ void fold_parts(uint32_t first, uint32_t step, uint32
 //     that lane l already holds.  A = V^T over the same slots: lane l loads
 //     the same 8 dims of those 8 tokens (16 lanes: a whole row) and
 //     transposes them with byte permutes; the m-th of 8 products takes dim
-//     8 (l % 16) + m for its row l % 16.
+//     8 (l % 16) + m for its row l % 16.  (Rows of 64 and 32 dims: 4 and 2.)
+// HBM bounds it: 8.6 GB of 16 x 131072 tokens (8 KV heads, group 4, d 128) in
+// 1256-1327 us, 6.5-6.8 TB/s, by the box; the matrix cores are at 6 % and the
+// vector ALUs at a fifth.  Small calls are a chain of latencies: 504 tiles of
+// 2003 tokens take 7 us, of which 2 to know the share and its pages, 2 for
+// the loads, 1.3 to join the waves; then 4 for the join kernel.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedArgs a) {
@@ -301,7 +320,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
       cur.length = length_of(a, scalar_at(a.lengths, cur.b), cur.bad);
       cur.tiles = tiles_of(cur.length);
       const uint32_t here = (uint32_t)cur.tiles * (uint32_t)a.heads;
-      if (rest < here) break;
+      if (rest < here || cur.b + 1 >= a.sequences) break;
       rest -= here;
     }
     cur.h = (int)(rest / (uint32_t)cur.tiles);
@@ -352,17 +371,17 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
                                 any ? (uint32_t)(rows - 1) * a.v_ts + D * 2u : 0u);
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
-          t.k[s][j] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(ko + 64u * j), 0, AUX);
+          t.k[s][j] = __builtin_amdgcn_raw_buffer_load_b128(kr, (int)(ko + 64u * j), 0, kStreamLoad);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t vo = (uint32_t)(4 * lg + e) * a.v_ts;
 #pragma unroll
           for (int c8 = 0; c8 < P::k8; ++c8)
             t.v8[c8][4 * s + e] = __builtin_amdgcn_raw_buffer_load_b128(
-                vr, (int)(vo + li * 16u + 256u * c8), 0, AUX);
+                vr, (int)(vo + li * 16u + 256u * c8), 0, kStreamLoad);
           if constexpr (P::k4 > 0)
             t.v4[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b64(
-                vr, (int)(vo + li * 8u + 256u * P::k8), 0, AUX);
+                vr, (int)(vo + li * 8u + 256u * P::k8), 0, kStreamLoad);
           if constexpr (P::k2 > 0)
             t.v2[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b32(
                 vr, (int)(vo + li * 4u + 256u * P::k8 + 128u * P::k4), 0, 0);
@@ -418,7 +437,10 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
 #pragma unroll
           for (int n = 0; n < P::kBlocks; ++n) acc[n] *= by;
         }
-        const float base = m == kNegInf ? 0.0f : m;
+        // fp16 weights go up to 2^15 instead of 1, so that those of 2^-24 to
+        // 2^-39 of the largest, many in a long context, do not round to zero
+        // (the sum has the same factor)
+        const float base = m == kNegInf ? 0.0f : kHalf ? m - 15.0f : m;
         V8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {

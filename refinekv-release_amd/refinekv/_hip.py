@@ -652,7 +652,10 @@ def paged_decode(query, cache, scaling, workspace=None, output=None):
     query = _row_aligned(query, 16)
     if output is None:
         output = torch.empty(query.shape, device=device, dtype=query.dtype)
-    scratch = _buffer(workspace, "hip_paged_scratch", (_paged_bytes(cache, group),), device,
+    nbytes = _paged_bytes(cache, group)
+    # (a buffer for each size, none ever replaced: a captured graph keeps using
+    # the one it was captured with)
+    scratch = _buffer(workspace, ("hip_paged_scratch", nbytes, device.index), (nbytes,), device,
                       torch.uint8)
     rc = lib().rkv_paged_decode(_cache_struct(cache), query.data_ptr(), query.stride(0),
                                 query.stride(1), group, scaling, output.data_ptr(),

@@ -14,6 +14,7 @@ token per sequence over its visible tokens.  A decode step::
 Lengths and block table are read on the device, so one captured HIP graph
 serves every step of a batch.  ROCm tensors use the gfx950 kernels, others
 (and the types and shapes the kernels do not take) torch operations.
+Inference only, as the whole package: the results carry no gradient.
 """
 
 from dataclasses import dataclass, field
@@ -21,7 +22,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _hip
-from .rotary import DTYPES, check_out, pick_backend, rows_overlap
+from .rotary import DTYPES, check_out, overlaps_itself, pick_backend, rows_overlap
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_ROW_STRIDE = 1 << 25  # elements between a page's rows, at most
@@ -65,6 +66,8 @@ class PagedCache:
             raise ValueError(f"page_size must be one of {PAGE_SIZES}")
         if keys.shape[3] > 1 and (keys.stride(3) != 1 or values.stride(3) != 1):
             raise ValueError("keys and values must have a dense head_dim")
+        if overlaps_itself(keys) or overlaps_itself(values):
+            raise ValueError("keys and values must not overlap themselves")
         if table.ndim != 2 or min(table.shape) <= 0 or table.dtype != torch.int32:
             raise ValueError("block_table must be int32 with a nonempty (sequences, max_blocks) "
                              "shape")

@@ -182,18 +182,23 @@ def rows_overlap(a, b):
     return not (gap >= ra and gap + rb <= pitch)
 
 
+def overlaps_itself(t):
+    """Whether two elements of a strided view may share memory."""
+    inner = 1
+    for stride, count in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride < inner:
+            return True
+        inner += stride * (count - 1)
+    return False
+
+
 def check_out(name, out, like, others=()):
     """``out`` can take rows like ``like``'s, in place of them or apart from
     every tensor in ``others``."""
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have its input's shape, dtype and device")
-    # rows and heads apart from each other, largest stride first
-    dims = sorted(((s, n) for s, n in zip(out.stride(), out.shape) if n > 1), reverse=True)
-    inner = 1
-    for stride, count in reversed(dims):
-        if stride < inner:
-            raise ValueError(f"{name} must not overlap itself")
-        inner += stride * (count - 1)
+    if overlaps_itself(out):
+        raise ValueError(f"{name} must not overlap itself")
     if out.shape[-1] > 1 and out.stride(-1) != 1:
         raise ValueError(f"{name} must have a dense head_dim")
     same = out.data_ptr() == like.data_ptr() and out.stride() == like.stride()

@@ -240,6 +240,14 @@ def test_append_torch_places_every_row():
         assert torch.equal(new_t[rest].view(torch.int32), old[rest].view(torch.int32))
 
 
+def test_append_torch_no_tokens():
+    cache = PagedCache.empty(4, 2, 16, 8, 3, 2, dtype=F32)
+    rows = torch.empty(0, 2, 8)
+    out = paged_append(rows, rows, cache, query=rows, rotary=Rotary(RotaryConfig(head_dim=8)),
+                       token_starts=torch.zeros(4, dtype=torch.int32))
+    assert out.shape == (0, 2, 8)
+
+
 def test_cache_refusals():
     _, keys, values, table, lengths = _case([20, 20])
     PagedCache(keys, values, table, lengths)
@@ -251,6 +259,7 @@ def test_cache_refusals():
         (keys, values, table[:, :0], lengths),
         (keys.transpose(2, 3).contiguous().transpose(2, 3), values, table, lengths),
         (keys, values, table.t().contiguous().t(), lengths),
+        (keys[:, :1].expand(-1, 2, -1, -1), values, table, lengths),
         (keys, values, table, lengths.repeat_interleave(2)[::2]),
     ]
     for args in bad:

@@ -46,6 +46,10 @@ def bits(t):
     (9, 2, 1, 34, 6, True, F32), (5, 3, 2, 7, 6, False, BF16), (5, 3, 2, 7, 6, True, F16),
     (3, 2, 1, 700, 700, False, F32), (2, 1, 1, 2, 2, True, BF16), (300, 1, 1, 300, 2, False, F16),
     (21, 300, 9, 32, 32, False, BF16),  # more heads than a workgroup holds
+    # parts of an odd number of vectors
+    (40, 3, 1, 64, 40, True, BF16), (40, 3, 1, 72, 32, False, F16), (17, 6, 2, 88, 48, True, BF16),
+    (25, 2, 1, 20, 12, True, F32), (25, 2, 2, 24, 16, False, F32),
+    (2000, 17, 3, 128, 128, False, BF16),  # enough threads that each turns several heads
 ])
 def test_rotate_heads(tokens, heads, kv, dim, rotary_dim, interleaved, dtype):
     gen = torch.Generator().manual_seed(tokens * 1000 + dim)
@@ -399,6 +403,46 @@ def test_decode_repeats_bit_for_bit_and_workspaces_are_reusable():
             assert torch.equal(bits(got), bits(first.setdefault(i, got.clone()))), (again, i)
 
 
+def test_decode_fp16_keeps_many_small_weights():
+    """One key that outweighs each of 60000 others by 2^24 or more: together
+    the others still weigh, though each is below fp16's subnormals against 1."""
+    length, dim = 60001, 32
+    query = torch.zeros(1, 1, dim, dtype=F16)
+    query[0, 0, 0] = 1.0
+    blocks = -(-length // 256)
+    keys = torch.zeros(blocks, 1, 256, dim, dtype=F16)
+    values = torch.full((blocks, 1, 256, dim), -1.0, dtype=F16)
+    values[7, 0, 100] = 1.0
+    lengths = torch.tensor([length], dtype=torch.int32)
+    table = torch.arange(blocks, dtype=torch.int32)[None]
+    for above in (17.0, 19.0, 23.0):
+        keys[7, 0, 100, 0] = above
+        case = (query, keys, values, table, lengths)
+        want, room = decode64(*case, 1.0)
+        others = 60000 * math.exp(-above)
+        assert abs(float(want[0, 0, 0]) - (1 - others) / (1 + others)) < 1e-9
+        assert_within(_decode(case, 1, scaling=1.0), want, room, str(above))
+
+
+def test_decode_nan_query_stays_in_its_row():
+    case = _decode_case([300, 40], 16, 2, 4, 64, BF16, seed=14)
+    clean = _decode(case, 4).cpu()
+    case[0][0, 5, 3] = math.nan
+    got = _decode(case, 4).cpu()
+    assert got[0, 5].isnan().all()
+    got[0, 5] = clean[0, 5]
+    assert torch.equal(bits(got), bits(clean))
+
+
+def test_decode_many_sequences():
+    """More sequences than a wave has lanes, many of them idle."""
+    gen = torch.Generator().manual_seed(5)
+    lengths = torch.randint(-2, 60, (3000,), generator=gen).clamp_min(0).tolist()
+    case = _decode_case(lengths, 16, 1, 1, 32, BF16, seed=15)
+    want, room = decode64(*case, 32 ** -0.5)
+    assert_within(_decode(case, 1), want, room)
+
+
 # -- together ----------------------------------------------------------------
 
 def _serving_batch(seed, page=16, heads=2, group=4, dim=64, dtype=BF16):
@@ -493,6 +537,59 @@ def test_graph_replays_of_append_and_decode_match_eager_steps():
         assert torch.equal(bits(a), bits(b))
     for a, b in zip(results[0][1:], results[1][1:]):
         assert torch.equal(bits(a), bits(b))
+
+
+def test_graphs_of_two_shapes_share_a_workspace():
+    """Two captured calls whose scratch differs in size keep theirs: replays
+    in turn, with eager work between, give the eager results."""
+    workspace, runs = {}, []
+    for seed, (lengths, heads, group, dim) in enumerate((([900, 30], 2, 4, 64),
+                                                         ([70, 0, 2000], 1, 16, 128))):
+        case = _decode_case(lengths, 16, heads, group, dim, BF16, seed=60 + seed)
+        query, *parts = on_gpu(*case)
+        cache, out = PagedCache(*parts), torch.empty_like(query)
+        want = paged_decode(query, cache, workspace=workspace, backend="hip")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            paged_decode(query, cache, workspace=workspace, output=out, backend="hip")
+        runs.append((graph, out, want, query, cache))
+    for _ in range(4):
+        for graph, out, want, query, cache in runs:
+            out.zero_()
+            junk = torch.randn(1 << 20, device=DEV)  # takes memory that was let go
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(bits(out), bits(want)) and bool(junk.isfinite().all())
+
+
+def test_append_no_tokens():
+    cache = PagedCache.empty(4, 2, 16, 64, 3, 2, device=DEV)
+    rows = torch.empty(0, 2, 64, device=DEV, dtype=BF16)
+    starts = torch.zeros(4, device=DEV, dtype=torch.int32)
+    out = paged_append(rows, rows, cache, query=rows, rotary=Rotary(RotaryConfig(head_dim=64), DEV),
+                       token_starts=starts, backend="hip")
+    assert out.shape == (0, 2, 64) and not cache.keys.any()
+
+
+def test_unsupported_shapes_take_torch_or_are_refused():
+    """auto answers what the kernels do not take; an explicit request says why."""
+    for heads, group, dim, dtype in ((1, 17, 64, BF16), (2, 2, 48, BF16), (2, 2, 64, F32)):
+        query, *parts = on_gpu(*_decode_case([40, 0, 17], 16, heads, group, dim, dtype, seed=dim))
+        cache = PagedCache(*parts)
+        with pytest.raises(TypeError):
+            paged_decode(query, cache, backend="hip")
+        got = paged_decode(query, cache)
+        want, room = decode64(query.cpu(), *(t.cpu() for t in parts), dim ** -0.5)
+        assert_within(got, want, room + 2.0 ** -12 * want.abs())
+    x = torch.randn(5, 2, 64, device=DEV, dtype=torch.float64)
+    positions = torch.arange(5, device=DEV)
+    config = RotaryConfig(head_dim=64)
+    with pytest.raises(TypeError):
+        rotate_heads(x, None, positions, Rotary(config, DEV), backend="hip")
+    got, _ = rotate_heads(x, None, positions, Rotary(config, DEV))
+    want, _ = rotate64(x.cpu(), positions.cpu(), config.rates())
+    assert float((got.cpu() - want).abs().max()) < 1e-12
 
 
 def test_calls_on_another_stream():
