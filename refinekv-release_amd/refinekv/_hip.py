@@ -553,6 +553,16 @@ def _dense_rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _rows(t):
+    """(pointer, token stride, head stride) of (tokens, heads, dim) rows."""
+    strides = t.stride()
+    return t.data_ptr(), strides[0], strides[1]
+
+
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _elsewhere(device):
     """Whether the device is another than the current one."""
     return device.index != torch.cuda.current_device()
@@ -567,22 +577,20 @@ def rotary(query, key, positions, table, query_out=None, key_out=None, inverse=F
     query, config = _dense_rows(query), table.config
     tokens, heads, dim = query.shape
     if query_out is None:
-        query_out = torch.empty((tokens, heads, dim), device=device, dtype=query.dtype)
+        query_out = _like(query)
     if key is None:
         source, kv_heads, target = (0, 0, 0), 0, (0, 0, 0)
     else:
         key, kv_heads = _dense_rows(key), key.shape[1]
         if key_out is None:
-            key_out = torch.empty((tokens, kv_heads, dim), device=device, dtype=query.dtype)
-        source = (key.data_ptr(), key.stride(0), key.stride(1))
-        target = (key_out.data_ptr(), key_out.stride(0), key_out.stride(1))
+            key_out = _like(key)
+        source, target = _rows(key), _rows(key_out)
     positions = positions.contiguous()
     rc = lib().rkv_rotary(
-        query.data_ptr(), query.stride(0), query.stride(1), heads, *source, kv_heads,
-        DTYPE_CODES[query.dtype], tokens, dim, positions.data_ptr(),
-        positions.dtype == torch.int64, table.turns.data_ptr(), config.rotary_dim,
-        config.interleaved, table.scale, inverse, query_out.data_ptr(), query_out.stride(0),
-        query_out.stride(1), *target, _raw_stream(device))
+        *_rows(query), heads, *source, kv_heads, DTYPE_CODES[query.dtype], tokens, dim,
+        positions.data_ptr(), positions.dtype == torch.int64, table.turns.data_ptr(),
+        config.rotary_dim, config.interleaved, table.scale, inverse, *_rows(query_out), *target,
+        _raw_stream(device))
     if rc:
         _check(rc, "rkv_rotary")
     return query_out, key_out
@@ -617,14 +625,12 @@ def paged_append(key, value, cache, query=None, table=None, token_starts=None, q
     if query is not None:
         query = _dense_rows(query)
         if query_out is None:
-            query_out = torch.empty(query.shape, device=device, dtype=query.dtype)
-        rows = (query.data_ptr(), query.stride(0), query.stride(1), query.shape[1],
-                query_out.data_ptr(), query_out.stride(0), query_out.stride(1))
+            query_out = _like(query)
+        rows = (*_rows(query), query.shape[1], *_rows(query_out))
     turns = (0, 0, 0, 1.0) if table is None else (
         table.turns.data_ptr(), table.config.rotary_dim, table.config.interleaved, table.scale)
     rc = lib().rkv_paged_append(
-        _cache_struct(cache), *rows, key.data_ptr(), key.stride(0), key.stride(1),
-        value.data_ptr(), value.stride(0), value.stride(1), key.shape[0],
+        _cache_struct(cache), *rows, *_rows(key), *_rows(value), key.shape[0],
         0 if token_starts is None else token_starts.data_ptr(), *turns, _raw_stream(device))
     if rc:
         _check(rc, "rkv_paged_append")
@@ -651,15 +657,15 @@ def paged_decode(query, cache, scaling, workspace=None, output=None):
     group = query.shape[1] // cache.heads
     query = _row_aligned(query, 16)
     if output is None:
-        output = torch.empty(query.shape, device=device, dtype=query.dtype)
+        output = _like(query)
     nbytes = _paged_bytes(cache, group)
     # (a buffer for each size, none ever replaced: a captured graph keeps using
     # the one it was captured with)
     scratch = _buffer(workspace, ("hip_paged_scratch", nbytes, device.index), (nbytes,), device,
                       torch.uint8)
-    rc = lib().rkv_paged_decode(_cache_struct(cache), query.data_ptr(), query.stride(0),
-                                query.stride(1), group, scaling, output.data_ptr(),
-                                scratch.data_ptr(), scratch.numel(), _raw_stream(device))
+    rc = lib().rkv_paged_decode(_cache_struct(cache), *_rows(query), group, scaling,
+                                output.data_ptr(), scratch.data_ptr(), nbytes,
+                                _raw_stream(device))
     if rc:
         _check(rc, "rkv_paged_decode")
     return output

@@ -443,6 +443,32 @@ def test_decode_many_sequences():
     assert_within(_decode(case, 1), want, room)
 
 
+def test_offsets_past_32_bits():
+    """A cache of 2^32 elements and more a tensor: the first and last pages,
+    written and read."""
+    heads, page, dim = 8, 16, 128
+    pages = (1 << 32) // (heads * page * dim) + 5
+    keys, values = (torch.empty(pages, heads, page, dim, device=DEV, dtype=BF16) for _ in range(2))
+    places = [pages - 1, 0, pages - 3, 131073, pages - 2]
+    table = torch.tensor([places], dtype=torch.int32, device=DEV)
+    length = 5 * page - 3
+    cache = PagedCache(keys, values, table,
+                       torch.tensor([length], dtype=torch.int32, device=DEV))
+    gen = torch.Generator().manual_seed(21)
+    key, value = (torch.randn(length, heads, dim, generator=gen).to(BF16) for _ in range(2))
+    query = torch.randn(1, heads * 4, dim, generator=gen).to(BF16)
+    starts = torch.tensor([0, length], dtype=torch.int32, device=DEV)
+    paged_append(*on_gpu(key, value), cache, token_starts=starts, backend="hip")
+    got = paged_decode(query.to(DEV), cache, backend="hip")
+    small = [t[places].cpu() for t in (keys, values)]
+    for t, rows in zip(small, (key, value)):
+        held = t.transpose(1, 2).reshape(-1, heads, dim)[:length]
+        assert torch.equal(bits(held), bits(rows))
+    want, room = decode64(query, *small, torch.arange(5, dtype=torch.int32)[None], [length],
+                          dim ** -0.5)
+    assert_within(got, want, room)
+
+
 # -- together ----------------------------------------------------------------
 
 def _serving_batch(seed, page=16, heads=2, group=4, dim=64, dtype=BF16):
