@@ -5,11 +5,11 @@
 //   y0 = x0 c - x1 s,  y1 = x1 c + x0 s,  c = a cos t, s = a sin t,
 // with a the table's attention factor.  The half layout pairs dims i and
 // i + r/2, the interleaved one 2i and 2i + 1; dims from r on pass.  Memory
-// bound: every value is read and written once, at 5.7-5.8 TB/s for long
-// prompts (131001 tokens of 32 + 8 + 8 heads, d 128, 3.2 GB: 555 us; a copy of
-// 2 GiB by the device reaches 5.0 TB/s).  A cos and sin costs some 45
-// instructions a pair, so a thread that turned one head alone was bound by
-// them (862 us).
+// bound: every value is read and written once, at 5.9 TB/s for long prompts
+// (131001 tokens of 32 + 8 + 8 heads, d 128, 3.2 GB: 542 us; torch's copy of
+// 2 GiB reaches 5.0 TB/s).  A cos and sin costs some 30 instructions a pair
+// (45 before the quarters were taken off by one addition), so a thread that
+// turned one head alone was bound by them (862 us).
 #include "rkv_common.h"
 #include "rkv_internal.h"
 #include "rkv_paged.h"
@@ -39,7 +39,7 @@ struct Rows {
   int64_t dst_ts, dst_hs;    // of dst (a page's row and head strides in a cache)
   int64_t dst_ps;            // page stride of dst, elements (cache only)
   int heads;
-  int paged;                 // dst is the cache's pages
+  int paged;                 // dst is the cache's pages (keys and values alike)
 };
 
 struct RotaryArgs {
@@ -63,14 +63,17 @@ struct RotaryArgs {
   int slots, per_block;      // heads that a token's threads hold at a time, a workgroup's tokens
 };
 
-// cos and sin of `turns` whole turns, to an ulp or two of fp32.  The angle of
-// a far position needs more than fp32's 24 bits (131071 * 1 rad has an ulp of
-// 0.008 rad there), so the whole quarter turns are taken off in fp64; what
-// is left, at most pi/4, goes through the Taylor series of sin (to a^9,
+// cos and sin of `quarters` quarter turns, to an ulp or two of fp32.  The
+// angle of a far position needs more than fp32's 24 bits (131071 * 1 rad has
+// an ulp of 0.008 rad there), so the whole quarters are taken off in fp64:
+// adding 1.5 * 2^52 leaves them in the sum's low bits, rounded to nearest.
+// What is left, at most pi/4, goes through the Taylor series of sin (to a^9,
 // truncation 2e-9) and cos (to a^10, 2e-10).
-__device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
-  const double quarter = __builtin_rint(turns * 4.0);
-  const float a = (float)((turns - quarter * 0.25) * 6.283185307179586477);
+__device__ __forceinline__ void cos_sin(double quarters, float& c, float& s) {
+  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
+  const double sum = quarters + kWhole;
+  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, sum);
+  const float a = (float)(quarters - (sum - kWhole)) * 1.57079632679489662f;
   const float a2 = a * a;
   float p = 2.75573192239858907e-06f;                    // 1/9!
   p = __builtin_fmaf(p, a2, -1.98412698412698413e-04f);  // 1/7!
@@ -83,12 +86,17 @@ __device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
   q = __builtin_fmaf(q, a2, 4.16666666666666667e-02f);   // 1/4!
   q = __builtin_fmaf(q, a2, -0.5f);
   const float cn = __builtin_fmaf(q, a2, 1.0f);
-  // the low two bits of the whole quarters (their count may pass 32 bits)
-  const int k = (int)(quarter - 4.0 * __builtin_floor(quarter * 0.25));
-  c = k & 1 ? sn : cn;
-  s = k & 1 ? cn : sn;
-  c = k == 1 || k == 2 ? -c : c;
-  s = k >= 2 ? -s : s;
+  // quarter 0 (c, s), 1 (-s, c), 2 (-c, -s), 3 (s, -c)
+  const bool swap = (k & 1u) != 0u;
+  c = bits_f32(f32_bits(swap ? sn : cn) ^ ((k + 1u) << 30 & 0x80000000u));
+  s = bits_f32(f32_bits(swap ? cn : sn) ^ (k << 30 & 0x80000000u));
+}
+
+// One of three values, chosen as values: a choice between variables would be
+// one of addresses, and put them in scratch.
+template <typename T>
+__device__ __forceinline__ T pick(bool q, bool v, T of_query, T of_key, T of_value) {
+  return q ? of_query : v ? of_value : of_key;
 }
 
 // Where a token's rows go: its position, and its page and row in a cache
@@ -158,16 +166,21 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     const int gap = turns ? a.gap : W;
     const bool two = turns ? !kAdjacent || d0 + W < a.rotary_dim : d0 + W < a.dim;
     V x[kBatch], z[kBatch];
-    // queries, then keys, then values
+    // queries, then keys, then values: each kind's first head, and the others
+    // by its head stride
     const int q_end = a.rows[0].heads, k_end = q_end + a.rows[1].heads;
-#define PICK(field) (q ? a.rows[0].field : v ? a.rows[2].field : a.rows[1].field)
+    const char* const from_q = a.rows[0].src + (t * a.rows[0].src_ts + d0) * kSize;
+    const char* const from_k = a.rows[1].src + (t * a.rows[1].src_ts + d0) * kSize;
+    const char* const from_v = a.rows[2].src + (t * a.rows[2].src_ts + d0) * kSize;
+    const int64_t q_hs = a.rows[0].src_hs * kSize, k_hs = a.rows[1].src_hs * kSize,
+                  v_hs = a.rows[2].src_hs * kSize;
     auto load = [&](int n0) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int n = min(n0 + i * a.slots, a.heads - 1);
         const bool q = n < q_end, v = n >= k_end;
         const int h = n - (q ? 0 : v ? k_end : q_end);
-        const char* src = PICK(src) + (t * PICK(src_ts) + h * PICK(src_hs) + d0) * kSize;
+        const char* src = pick(q, v, from_q, from_k, from_v) + h * pick(q, v, q_hs, k_hs, v_hs);
         x[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src));
         if (two)
           z[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + gap * kSize));
@@ -177,24 +190,36 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
     if (!placed) place = place_of(a, t);
     placed = true;
     const bool live = turns && place.live;
+    const double position4 = 4.0 * (double)place.position;  // rates are whole turns
     float c[kPairs], s[kPairs];
     if (live) {
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) {
         // (the pairs of a second vector that is not there are not read)
         const int pair = item * kPairs + (kAdjacent && i >= W / 2 && !two ? 0 : i);
-        cos_sin((double)place.position * a.rates[pair], c[i], s[i]);
+        cos_sin(position4 * a.rates[pair], c[i], s[i]);
         c[i] *= a.scale;
         s[i] *= a.scale * a.sign;
       }
     }
+    // (a cache's keys and values, or rows of this token)
+    const int64_t k_row = a.rows[1].paged ? place.page * a.rows[1].dst_ps +
+                                                place.row * a.rows[1].dst_ts
+                                          : t * a.rows[1].dst_ts;
+    const int64_t v_row = place.page * a.rows[2].dst_ps + place.row * a.rows[2].dst_ts;
+    char* const to_q = a.rows[0].dst + (t * a.rows[0].dst_ts + d0) * kSize;
+    char* const to_k = a.rows[1].dst + (k_row + d0) * kSize;
+    char* const to_v = a.rows[2].dst + (v_row + d0) * kSize;
+    const int64_t qo_hs = a.rows[0].dst_hs * kSize, ko_hs = a.rows[1].dst_hs * kSize,
+                  vo_hs = a.rows[2].dst_hs * kSize;
+    const bool stored = place.page >= 0;  // keys and values of a cache
     for (int n0 = slot;;) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int n = n0 + i * a.slots;
         const bool q = n < q_end, v = n >= k_end;
         const int h = n - (q ? 0 : v ? k_end : q_end);
-        if (n >= a.heads || (PICK(paged) && place.page < 0)) continue;
+        if (n >= a.heads || (!q && a.rows[1].paged && !stored)) continue;
         if (live && !v) {
 #pragma unroll
           for (int p = 0; p < kPairs; ++p) {
@@ -214,15 +239,14 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
             }
           }
         }
-        char* dst = PICK(dst) + ((PICK(paged) ? place.page * PICK(dst_ps) + place.row * PICK(dst_ts)
-                                              : t * PICK(dst_ts)) + h * PICK(dst_hs) + d0) * kSize;
-        V* const to = reinterpret_cast<V*>(dst);
+        char* dst = pick(q, v, to_q, to_k, to_v) + h * pick(q, v, qo_hs, ko_hs, vo_hs);
+        V* const to_x = reinterpret_cast<V*>(dst);
         V* const to_z = reinterpret_cast<V*>(dst + gap * kSize);
         if constexpr (kStream) {
-          __builtin_nontemporal_store(x[i], to);
+          __builtin_nontemporal_store(x[i], to_x);
           if (two) __builtin_nontemporal_store(z[i], to_z);
         } else {
-          *to = x[i];
+          *to_x = x[i];
           if (two) *to_z = z[i];
         }
       }
@@ -230,7 +254,6 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
       if (n0 >= a.heads) break;
       load(n0);
     }
-#undef PICK
   }
 }
 
