@@ -308,7 +308,10 @@ int rkv_paged_append(const rkv_paged_cache* cache, const void* query, int64_t q_
  *   <= 16; query, output and cache 16-byte aligned, strides multiples of 8.
  *   workspace: rkv_paged_plan's bytes.
  * lengths[b] <= 0 gives zeros.  A page outside the cache among the visible
- * ones, or a length past the table, gives NaN in that sequence's rows.
+ * ones, or a length past the table, gives NaN in that sequence's rows.  What
+ * lies behind a sequence's end is not read.  Scores of +inf or NaN make a row
+ * NaN, as a softmax does, and so do scores of -inf alone; an infinite visible
+ * value makes its dim infinite or NaN.
  */
 int rkv_paged_decode(const rkv_paged_cache* cache, const void* query, int64_t q_sequence_stride,
                      int64_t q_head_stride, int64_t group, float scale, void* output,

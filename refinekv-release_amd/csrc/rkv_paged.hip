@@ -437,14 +437,14 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
 #pragma unroll
           for (int n = 0; n < P::kBlocks; ++n) acc[n] *= by;
         }
-        // fp16 weights go up to 2^15 instead of 1, so that those of 2^-24 to
-        // 2^-39 of the largest, many in a long context, do not round to zero
-        // (the sum has the same factor)
-        const float base = m == kNegInf ? 0.0f : kHalf ? m - 15.0f : m;
+        const float base = m == kNegInf ? 0.0f : m;
         V8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float p = __builtin_amdgcn_exp2f(x[e] - base);
+          // (fp16 weights go up to 2^15 instead of 1, and the sum with them, so
+          // that those of 2^-24 to 2^-39 of the largest, many in a long
+          // context, do not round to zero)
+          const float p = __builtin_amdgcn_exp2f(x[e] - base) * (kHalf ? 32768.0f : 1.0f);
           l += p;
           // the weight as the sum of two 16-bit parts: its rounding would
           // otherwise be the largest error of the result
@@ -605,7 +605,8 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
       for (int i = first; i < end; ++i) {
         const float w = weight_s[g][i];
         const F32x4 p = *reinterpret_cast<const F32x4*>(&parts[i / 2][i % 2].acc[g][d]);
-        o += w != 0.0f ? p * w : F32x4{0.0f, 0.0f, 0.0f, 0.0f};  // (an unused part holds anything)
+        // (a part that is not the row's holds anything)
+        o += same >> i & 1 ? p * w : F32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
       const float2 ml = total_s[g];
       if (whole) {
