@@ -85,6 +85,10 @@ class PagedCache:
         for name, value in sizes.items():
             object.__setattr__(self, name, value)
 
+    def __getstate__(self):
+        # (copies look up anew what the calls have noted about these tensors)
+        return {k: v for k, v in self.__dict__.items() if not k.startswith("_hip")}
+
     @classmethod
     def empty(cls, pages, kv_heads, page_size, head_dim, sequences, max_blocks, *,
               dtype=torch.bfloat16, device=None):

@@ -618,6 +618,66 @@ def test_unsupported_shapes_take_torch_or_are_refused():
     assert float((got.cpu() - want).abs().max()) < 1e-12
 
 
+def test_two_streams_at_once():
+    """Calls of two streams with a workspace each, interleaved."""
+    runs = []
+    for seed, shape in enumerate((([3000, 10], 16, 8, 4, 128, BF16), ([700] * 9, 32, 2, 7, 64, F16))):
+        lengths, page, heads, group, dim, dtype = shape
+        query, *parts = on_gpu(*_decode_case(lengths, page, heads, group, dim, dtype, seed=70 + seed))
+        cache = PagedCache(*parts)
+        runs.append((query, cache, paged_decode(query, cache, backend="hip"), {},
+                     torch.cuda.Stream(), []))
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for query, cache, _, workspace, stream, outs in runs:
+            with torch.cuda.stream(stream):
+                outs.append(paged_decode(query, cache, workspace=workspace, backend="hip"))
+    torch.cuda.synchronize()
+    for _, _, want, _, _, outs in runs:
+        assert all(torch.equal(bits(out), bits(want)) for out in outs)
+
+
+def test_unaligned_cache():
+    """A cache that starts two bytes past any vector boundary: the append
+    writes it element by element, the decode leaves it to torch or says why."""
+    case = _append_case([20, 5], [20, 5], 16, 2, 2, 64, BF16, seed=50)
+    shape = case["keys"].shape
+    keys, values = (torch.empty(case["keys"].numel() + 1, device=DEV, dtype=BF16)[1:].view(shape)
+                    .copy_(case[n]) for n in ("keys", "values"))
+    table, lengths, starts = on_gpu(case["table"], case["lengths"], case["starts"])
+    cache = PagedCache(keys, values, table, lengths)
+    config = RotaryConfig(head_dim=64)
+    query = paged_append(*on_gpu(case["key"], case["value"]), cache, query=case["query"].to(DEV),
+                         rotary=Rotary(config, DEV), token_starts=starts, backend="hip")
+    _check_append(case, config, cache, query)
+    last = torch.stack([query[19], query[24]])
+    with pytest.raises(TypeError):
+        paged_decode(last, cache, backend="hip")
+    got = paged_decode(last, cache)
+    want, room = decode64(last.cpu(), keys.cpu(), values.cpu(), case["table"], case["lengths"],
+                          64 ** -0.5)
+    assert_within(got, want, room + 2.0 ** -12 * want.abs())
+    # an unaligned query is copied
+    aligned = [t.clone() for t in (keys, values)]
+    odd = torch.empty(last.numel() + 1, device=DEV, dtype=BF16)[1:].view(last.shape).copy_(last)
+    cache = PagedCache(*aligned, table, lengths)
+    assert torch.equal(bits(paged_decode(odd, cache, backend="hip")),
+                       bits(paged_decode(last, cache, backend="hip")))
+
+
+def test_copies_of_a_cache_are_their_own():
+    import copy
+
+    case = _decode_case([40, 3], 16, 2, 2, 64, BF16, seed=51)
+    query, *parts = on_gpu(*case)
+    cache = PagedCache(*parts)
+    want = paged_decode(query, cache, backend="hip")
+    other = copy.deepcopy(cache)
+    cache.keys.zero_()
+    assert torch.equal(bits(paged_decode(query, other, backend="hip")), bits(want))
+    assert not torch.equal(bits(paged_decode(query, copy.copy(cache), backend="hip")), bits(want))
+
+
 def test_calls_on_another_stream():
     case = _decode_case([500, 30], 16, 2, 4, 64, BF16, seed=31)
     want = _decode(case, 4)
