@@ -565,7 +565,7 @@ def _like(t):
 
 def _elsewhere(device):
     """Whether the device is another than the current one."""
-    return device.index != torch.cuda.current_device()
+    return device.index != torch._C._cuda_getDevice()
 
 
 def rotary(query, key, positions, table, query_out=None, key_out=None, inverse=False):
@@ -585,7 +585,8 @@ def rotary(query, key, positions, table, query_out=None, key_out=None, inverse=F
         if key_out is None:
             key_out = _like(key)
         source, target = _rows(key), _rows(key_out)
-    positions = positions.contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
     rc = lib().rkv_rotary(
         *_rows(query), heads, *source, kv_heads, DTYPE_CODES[query.dtype], tokens, dim,
         positions.data_ptr(), positions.dtype == torch.int64, table.turns.data_ptr(),

@@ -21,6 +21,7 @@ from .config import BACKENDS, KERNEL_BACKENDS
 
 SCALINGS = ("none", "linear", "ntk", "llama3", "yarn")
 DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+POSITION_DTYPES = (torch.int64, torch.int32)
 
 
 @dataclass(frozen=True)
@@ -216,30 +217,29 @@ def rotate_heads(query, key, positions, rotary, *, query_out=None, key_out=None,
     which may be the inputs themselves.  ``inverse`` turns by the opposite
     angles (the factor of a yarn rotation multiplies either way).
     """
-    config = rotary.config
-    if query.ndim != 3 or query.shape[1] <= 0 or query.shape[2] != config.head_dim:
+    config, shape, dtype, device = rotary.config, query.shape, query.dtype, query.device
+    if len(shape) != 3 or shape[1] <= 0 or shape[2] != config.head_dim:
         raise ValueError("query must have shape (tokens, heads, head_dim) of the rotary's head_dim")
-    if not query.is_floating_point():
+    if not dtype.is_floating_point:
         raise TypeError("query must be floating point")
     if key is not None:
-        if (key.ndim != 3 or key.shape[0] != query.shape[0] or key.shape[1] <= 0
-                or key.shape[2] != config.head_dim):
+        kv = key.shape
+        if len(kv) != 3 or kv[0] != shape[0] or kv[1] <= 0 or kv[2] != shape[2]:
             raise ValueError("key must have shape (tokens, heads, head_dim) with the query's "
                              "tokens and head_dim")
-        if key.dtype != query.dtype or key.device != query.device:
+        if key.dtype != dtype or key.device != device:
             raise ValueError("query and key must have the same device and dtype")
     elif key_out is not None:
         raise ValueError("key_out without a key")
-    if positions.shape != (query.shape[0],) or positions.dtype not in (torch.int32, torch.int64):
+    if positions.shape != shape[:1] or positions.dtype not in POSITION_DTYPES:
         raise ValueError("positions must be int32 or int64 with shape (tokens,)")
-    if positions.device != query.device or rotary.device != query.device:
+    if positions.device != device or rotary.turns.device != device:
         raise ValueError("positions and rotary must be on the query device")
-    apart = [t for t in (key, key_out) if t is not None]
     if query_out is not None:
-        check_out("query_out", query_out, query, apart)
+        check_out("query_out", query_out, query, [t for t in (key, key_out) if t is not None])
     if key_out is not None:
         check_out("key_out", key_out, key, [query])
-    if pick_backend(query, backend, query.dtype in DTYPES,
+    if pick_backend(query, backend, dtype in DTYPES,
                     "the HIP rotation needs bf16, fp16 or fp32 rows") == "hip":
         return _hip.rotary(query, key, positions, rotary, query_out, key_out, inverse)
     from .reference_paged import rotate
