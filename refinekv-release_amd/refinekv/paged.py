@@ -131,6 +131,9 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     A row whose page is outside the cache, or past the block table, is not
     stored.  No two rows of a call may fall on the same place: a page written
     here belongs to one sequence.
+
+    (A prompt's own attention needs its turned keys as well: turn both with
+    rotate_heads, then append without ``rotary``.)
     """
     tokens, device = key.shape[0] if key.ndim else 0, cache.device
     _check_rows("key", key, cache, tokens, cache.heads)
