@@ -262,7 +262,8 @@ int rkv_rotary(const void* query, int64_t q_token_stride, int64_t q_head_stride,
  * token_stride elements into keys / values, head_dim dense.  lengths[b]:
  * the sequence's visible tokens, those of the call at hand included.
  * block_table and lengths are read on the device: a page outside [0, pages)
- * is never read or written.
+ * is never read or written.  The stride of an axis of length one is not read
+ * (here, and of queries, keys and values in the entries below).
  */
 typedef struct rkv_paged_cache {
   void* keys;

@@ -41,4 +41,7 @@ inline int check_cache(const char* who, const rkv_paged_cache* c) {
   return kOk;
 }
 
+// The stride of an axis of `count` places; that of a single place is not read.
+inline int64_t read_stride(int64_t stride, int64_t count) { return count > 1 ? stride : 0; }
+
 }  // namespace rkv

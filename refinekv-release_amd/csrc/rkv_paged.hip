@@ -272,8 +272,8 @@ __device__ __forceinline__ void fold_parts(uint32_t first, uint32_t step, uint32
 //     transposes them with byte permutes; the m-th of 8 products takes dim
 //     8 (l % 16) + m for its row l % 16.  (Rows of 64 and 32 dims: 4 and 2.)
 // HBM bounds it: 8.6 GB of 16 x 131072 tokens (8 KV heads, group 4, d 128) in
-// 1256-1327 us, 6.5-6.8 TB/s, by the box; the matrix cores are at 6 % and the
-// vector ALUs at a fifth.  Small calls are a chain of latencies: 504 tiles of
+// 1253-1327 us, 6.5-6.9 TB/s, by the box; the matrix cores are at 6 % and the
+// vector ALUs at 11 %.  Small calls are a chain of latencies: 504 tiles of
 // 2003 tokens take 7 us, of which 2 to know the share and its pages, 2 for
 // the loads, 1.3 to join the waves; then 4 for the join kernel.
 template <int D, bool kHalf>
@@ -720,8 +720,10 @@ int check_paged(const char* who, const rkv_paged_cache* c, int64_t group) {
   if (group <= 0) return set_error(kInvalidArgument, "%s: empty group", who);
   if (group > kMaxGroup)
     return set_error(kUnsupported, "%s: GQA group %lld exceeds 16", who, (long long)group);
-  const int64_t strides[] = {c->key_page_stride, c->key_head_stride, c->key_token_stride,
-                             c->value_page_stride, c->value_head_stride, c->value_token_stride};
+  const int64_t strides[] = {
+      read_stride(c->key_page_stride, c->pages),   read_stride(c->key_head_stride, c->heads),
+      read_stride(c->value_page_stride, c->pages), read_stride(c->value_head_stride, c->heads),
+      c->key_token_stride,                         c->value_token_stride};
   for (int64_t s : strides)
     if (s % 8) return set_error(kInvalidArgument, "%s: cache strides must be multiples of 8", who);
   if (c->key_token_stride < c->dim || c->value_token_stride < c->dim)
@@ -762,6 +764,8 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
   const int rc = check_paged(who, cache, group);
   if (rc) return rc;
   if (!query || !output) return set_error(kInvalidArgument, "%s: null pointer argument", who);
+  q_sequence_stride = read_stride(q_sequence_stride, cache->sequences);
+  q_head_stride = read_stride(q_head_stride, cache->heads * group);
   if (q_sequence_stride < 0 || q_head_stride < 0 || q_head_stride > (1 << 25))
     return set_error(kUnsupported, "%s: query stride", who);
   if (!aligned(query, 16) || !aligned(output, 16) || q_sequence_stride % 8 || q_head_stride % 8)
@@ -780,10 +784,10 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
   a.q_hs = q_head_stride;
   a.keys = static_cast<const char*>(cache->keys);
   a.values = static_cast<const char*>(cache->values);
-  a.k_ps = cache->key_page_stride;
-  a.k_hs = cache->key_head_stride;
-  a.v_ps = cache->value_page_stride;
-  a.v_hs = cache->value_head_stride;
+  a.k_ps = read_stride(cache->key_page_stride, cache->pages);
+  a.k_hs = read_stride(cache->key_head_stride, cache->heads);
+  a.v_ps = read_stride(cache->value_page_stride, cache->pages);
+  a.v_hs = read_stride(cache->value_head_stride, cache->heads);
   a.k_ts = (uint32_t)(cache->key_token_stride * 2);
   a.v_ts = (uint32_t)(cache->value_token_stride * 2);
   a.table = cache->block_table;

@@ -342,15 +342,15 @@ int check_rows(const char* who, const void* src, const void* dst, int64_t heads,
   return kOk;
 }
 
-Rows plain_rows(const void* src, int64_t ts, int64_t hs, int64_t heads, void* dst, int64_t dst_ts,
-                int64_t dst_hs) {
+Rows plain_rows(int64_t tokens, const void* src, int64_t ts, int64_t hs, int64_t heads, void* dst,
+                int64_t dst_ts, int64_t dst_hs) {
   Rows r{};
   r.src = static_cast<const char*>(src);
   r.dst = static_cast<char*>(dst);
-  r.src_ts = ts;
-  r.src_hs = hs;
-  r.dst_ts = dst_ts;
-  r.dst_hs = dst_hs;
+  r.src_ts = read_stride(ts, tokens);
+  r.src_hs = read_stride(hs, heads);
+  r.dst_ts = read_stride(dst_ts, tokens);
+  r.dst_hs = read_stride(dst_hs, heads);
   r.heads = (int)heads;
   return r;
 }
@@ -380,9 +380,9 @@ extern "C" int rkv_rotary(const void* query, int64_t q_token_stride, int64_t q_h
   if (!rc) rc = check_rows(who, key, key_out, tokens ? k_heads : 0, size);
   if (rc) return rc;
   RotaryArgs a{};
-  a.rows[0] = plain_rows(query, q_token_stride, q_head_stride, q_heads, query_out,
+  a.rows[0] = plain_rows(tokens, query, q_token_stride, q_head_stride, q_heads, query_out,
                          qo_token_stride, qo_head_stride);
-  a.rows[1] = plain_rows(key, k_token_stride, k_head_stride, k_heads, key_out, ko_token_stride,
+  a.rows[1] = plain_rows(tokens, key, k_token_stride, k_head_stride, k_heads, key_out, ko_token_stride,
                          ko_head_stride);
   a.tokens = tokens;
   a.dim = (int)dim;
@@ -416,14 +416,16 @@ extern "C" int rkv_paged_append(const rkv_paged_cache* cache, const void* query,
   if (!rc) rc = check_rows(who, value, cache->values, tokens ? cache->heads : 0, size);
   if (rc) return rc;
   RotaryArgs a{};
-  a.rows[0] = plain_rows(query, q_token_stride, q_head_stride, q_heads, query_out,
+  a.rows[0] = plain_rows(tokens, query, q_token_stride, q_head_stride, q_heads, query_out,
                          qo_token_stride, qo_head_stride);
-  a.rows[1] = plain_rows(key, k_token_stride, k_head_stride, cache->heads, cache->keys,
+  a.rows[1] = plain_rows(tokens, key, k_token_stride, k_head_stride, cache->heads, cache->keys,
                          cache->key_token_stride, cache->key_head_stride);
-  a.rows[2] = plain_rows(value, v_token_stride, v_head_stride, cache->heads, cache->values,
+  a.rows[2] = plain_rows(tokens, value, v_token_stride, v_head_stride, cache->heads, cache->values,
                          cache->value_token_stride, cache->value_head_stride);
-  a.rows[1].dst_ps = cache->key_page_stride;
-  a.rows[2].dst_ps = cache->value_page_stride;
+  a.rows[1].dst_ts = cache->key_token_stride;  // of a page's rows, however few tokens come
+  a.rows[2].dst_ts = cache->value_token_stride;
+  a.rows[1].dst_ps = read_stride(cache->key_page_stride, cache->pages);
+  a.rows[2].dst_ps = read_stride(cache->value_page_stride, cache->pages);
   a.rows[1].paged = a.rows[2].paged = 1;
   a.tokens = tokens;
   a.dim = (int)cache->dim;

@@ -182,7 +182,7 @@ def _why_not(cache, group):
     if dim not in _hip.SUPPORTED_DIMS or group > _hip.MAX_GROUP:
         return "the HIP paged decode needs head_dim in 32..256 (multiple of 32) and group <= 16"
     for t in (cache.keys, cache.values):
-        if t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:3]):
+        if t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:3], t.shape) if n > 1):
             return "the HIP paged decode needs a cache of 16-byte aligned rows"
         if not dim <= t.stride(2) <= MAX_ROW_STRIDE:
             return "the HIP paged decode needs rows apart from each other, and not too far"

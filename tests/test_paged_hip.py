@@ -665,6 +665,28 @@ def test_unaligned_cache():
                        bits(paged_decode(last, cache, backend="hip")))
 
 
+def test_strides_of_single_places_are_not_read():
+    """Views keep any stride on an axis of length one; with odd ones there the
+    calls answer as without."""
+    case = _decode_case([13], 16, 1, 1, 64, BF16, seed=52, spare=0)
+    query, keys, values, table, lengths = on_gpu(*case)
+    assert keys.shape == (1, 1, 16, 64)
+    want = paged_decode(query, PagedCache(keys, values, table, lengths), backend="hip")
+    odd = lambda t: t.as_strided(t.shape, (3, 5, 64, 1))  # noqa: E731
+    cache = PagedCache(odd(keys), odd(values), table, lengths)
+    got = paged_decode(query.as_strided((1, 1, 64), (7, 9, 1)), cache, backend="hip")
+    assert torch.equal(bits(got), bits(want))
+    rotary = Rotary(RotaryConfig(head_dim=64), DEV)
+    row = torch.randn(1, 1, 64, device=DEV).to(BF16)
+    turned = paged_append(row.as_strided((1, 1, 64), (3, 1, 1)), row, cache, query=row,
+                          rotary=rotary, backend="hip")
+    position = torch.tensor([12], device=DEV)
+    alone, _ = rotate_heads(row.as_strided((1, 1, 64), (1, 3, 1)), None, position, rotary,
+                            backend="hip")
+    place = keys[int(table[0, 0]), 0, 12]
+    assert torch.equal(bits(turned), bits(alone)) and torch.equal(bits(place), bits(alone[0, 0]))
+
+
 def test_copies_of_a_cache_are_their_own():
     import copy
 
