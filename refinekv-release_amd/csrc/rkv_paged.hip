@@ -443,7 +443,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
           for (int n = 0; n < P::kBlocks; ++n) acc[n] *= by;
         }
         const float base = m == kNegInf ? 0.0f : m;
-        V8 hi, lo;
+        V8 hi, lo, last;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           // (fp16 weights go up to 2^15 instead of 1, and the sum with them, so
@@ -451,16 +451,22 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
           // context, do not round to zero)
           const float p = __builtin_amdgcn_exp2f(x[e] - base) * (kHalf ? 32768.0f : 1.0f);
           l += p;
-          // the weight as the sum of two 16-bit parts: its rounding would
-          // otherwise be the largest error of the result
+          // the weight as a sum of 16-bit parts that holds all of it: two of
+          // fp16 (to 2^-23), three of bf16 (exact).  (Two of bf16 hold it to
+          // 2^-17: 1.4 times as many outputs rounded the other way at 131072
+          // tokens, and the same 92 us; 128 short sequences at head_dim 64 70.9
+          // us against 73.3.)
           hi[e] = (E)p;
-          lo[e] = (E)(p - (float)hi[e]);
+          const float rest = p - (float)hi[e];
+          lo[e] = (E)rest;
+          if constexpr (!kHalf) last[e] = (E)(rest - (float)lo[e]);
         }
         // dims' products: byte permutes gather one dim of two tokens a word
         auto product = [&](int n, uint32_t (&words)[4]) {
           const V8 v = __builtin_bit_cast(V8, U32x4{words[0], words[1], words[2], words[3]});
           acc[n] = T::mma(v, hi, acc[n]);
           acc[n] = T::mma(v, lo, acc[n]);
+          if constexpr (!kHalf) acc[n] = T::mma(v, last, acc[n]);
         };
         constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
 #pragma unroll
