@@ -290,7 +290,8 @@ typedef struct rkv_paged_cache {
  * A row of no sequence or at a negative position (an idle place of a padded
  * batch) is not stored and its query is copied unturned; a row whose page is
  * outside the cache or the table is not stored.  Sequences must not append
- * to the same page row in one call.
+ * to the same page row in one call.  A cache whose keys and values share
+ * memory is refused here (rkv_paged_decode reads it).
  */
 int rkv_paged_append(const rkv_paged_cache* cache, const void* query, int64_t q_token_stride,
                      int64_t q_head_stride, int64_t q_heads, void* query_out,

@@ -41,6 +41,58 @@ inline int check_cache(const char* who, const rkv_paged_cache* c) {
   return kOk;
 }
 
+// An axis of a cache: strides in bytes, and its places.
+struct CacheAxis {
+  int64_t key, value, count;
+};
+
+// Whether keys and values from axis `level` on share a cell, the values' first
+// one `apart` behind the keys'.  Axes go from the widest stride to the
+// narrowest; where both have the same, at most a few places of one lie opposite
+// a place of the other (more, or other strides: taken to meet if their spans
+// do).
+inline bool cells_meet(const CacheAxis* axes, int level, int count, int64_t size, int64_t apart) {
+  int64_t keys = size, values = size, key_rest = size, value_rest = size;
+  for (int i = count - 1; i >= level; --i) {
+    key_rest = keys;
+    value_rest = values;
+    keys += (axes[i].count - 1) * axes[i].key;
+    values += (axes[i].count - 1) * axes[i].value;
+  }
+  if (apart >= keys || -apart >= values) return false;
+  if (level == count) return true;
+  const CacheAxis& a = axes[level];
+  if (a.key != a.value || a.key <= 0) return true;
+  auto down = [](int64_t x, int64_t y) { return x / y - (x % y < 0 ? 1 : 0); };
+  int64_t from = -down(value_rest - 1 + apart, a.key), to = down(key_rest - 1 - apart, a.key);
+  from = from > 1 - a.count ? from : 1 - a.count;
+  to = to < a.count - 1 ? to : a.count - 1;
+  if (to - from > 2) return true;
+  for (int64_t d = from; d <= to; ++d)
+    if (cells_meet(axes, level + 1, count, size, apart + d * a.key)) return true;
+  return false;
+}
+
+// Whether a cache's keys and values may share memory (which a call that writes
+// both does not allow; interleaved ones do not share any).
+inline bool keys_meet_values(const rkv_paged_cache* c) {
+  const int64_t size = dtype_bytes(c->dtype);
+  CacheAxis axes[4] = {{c->key_page_stride * size, c->value_page_stride * size, c->pages},
+                       {c->key_head_stride * size, c->value_head_stride * size, c->heads},
+                       {c->key_token_stride * size, c->value_token_stride * size, c->page_size},
+                       {size, size, c->dim}};
+  int count = 0;
+  for (const CacheAxis& a : axes)
+    if (a.count > 1) {
+      int i = count++;
+      const CacheAxis here = a;
+      for (; i > 0 && axes[i - 1].key < here.key; --i) axes[i] = axes[i - 1];
+      axes[i] = here;
+    }
+  return cells_meet(axes, 0, count, size,
+                    static_cast<const char*>(c->values) - static_cast<const char*>(c->keys));
+}
+
 // The stride of an axis of `count` places; that of a single place is not read.
 inline int64_t read_stride(int64_t stride, int64_t count) { return count > 1 ? stride : 0; }
 

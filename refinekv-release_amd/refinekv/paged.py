@@ -115,6 +115,31 @@ def _check_rows(name, rows, cache, tokens, heads=None):
         raise ValueError(f"{name} must have the cache's dtype and device")
 
 
+def _keys_meet_values(cache):
+    """Whether the cache's keys and values may share memory: the C entry's own
+    rule, for the torch operations."""
+    size = cache.keys.element_size()
+    axes = sorted(((s * size, t * size, n) for s, t, n in
+                   zip(cache.keys.stride(), cache.values.stride(), cache.keys.shape) if n > 1),
+                  reverse=True)
+
+    def meet(level, apart):
+        keys, values = (size + sum((a[2] - 1) * a[i] for a in axes[level:]) for i in (0, 1))
+        if apart >= keys or -apart >= values:
+            return False
+        if level == len(axes):
+            return True
+        stride, other, count = axes[level]
+        if stride != other:
+            return True
+        keys, values = keys - (count - 1) * stride, values - (count - 1) * stride
+        steps = range(max(-((values - 1 + apart) // stride), 1 - count),
+                      min((keys - 1 - apart) // stride, count - 1) + 1)
+        return len(steps) > 3 or any(meet(level + 1, apart + d * stride) for d in steps)
+
+    return meet(0, cache.values.data_ptr() - cache.keys.data_ptr())
+
+
 def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=None,
                  query_out=None, backend="auto"):
     """Write new (tokens, kv_heads, head_dim) keys and values to their
@@ -130,7 +155,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     place: length 0) are not stored, and their queries are returned unturned.
     A row whose page is outside the cache, or past the block table, is not
     stored.  No two rows of a call may fall on the same place: a page written
-    here belongs to one sequence.
+    here belongs to one sequence, and a cache whose keys and values share
+    memory is refused.
 
     (A prompt's own attention needs its turned keys as well: turn both with
     rotate_heads, then append without ``rotary``.)
@@ -161,6 +187,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
         return _hip.paged_append(key, value, cache, query, rotary, token_starts, query_out)
     from .reference_paged import append
 
+    if _keys_meet_values(cache):
+        raise ValueError("the cache's keys and values share memory")
     with torch.no_grad():
         turned = append(cache, key, value, query, rotary, token_starts)
         return turned if query_out is None else query_out.copy_(turned)

@@ -1,0 +1,112 @@
+"""Paged-cache calls whose tensors share memory: what would read or write a
+place twice in one launch is refused, what lies apart is not."""
+
+import ctypes
+
+import pytest
+import torch
+
+from refinekv import PagedCache, paged_append, paged_decode
+
+F32 = torch.float32
+
+
+def _tables(sequences=2, blocks=2):
+    return (torch.arange(sequences * blocks, dtype=torch.int32).view(sequences, blocks),
+            torch.tensor([3, 20], dtype=torch.int32)[:sequences].contiguous())
+
+
+def _rows(cache):
+    return torch.ones(cache.sequences, cache.heads, cache.head_dim)
+
+
+def _c_append(cache, **over):
+    """rkv_paged_append's code for tensors of these addresses (refused before
+    any launch: nothing is followed here)."""
+    from refinekv import _hip
+
+    def strides(t):
+        return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+    view = _hip._PagedCache(
+        keys=cache.keys.data_ptr(), key_strides=strides(cache.keys),
+        values=cache.values.data_ptr(), value_strides=strides(cache.values),
+        block_table=cache.block_table.data_ptr(), table_stride=cache.block_table.stride(0),
+        lengths=cache.lengths.data_ptr(), pages=cache.pages, heads=cache.heads,
+        page_size=cache.page_size, dim=cache.head_dim, sequences=cache.sequences,
+        max_blocks=cache.max_blocks, dtype=_hip.DTYPE_CODES[cache.dtype])
+    rows = _rows(cache)
+    args = dict(query=0, q_heads=0, query_out=0)
+    args.update(over)
+    dim = cache.head_dim
+    code = _hip.lib().rkv_paged_append(
+        ctypes.byref(view), args["query"], args["q_heads"] * dim, dim, args["q_heads"],
+        args["query_out"], args["q_heads"] * dim, dim, rows.data_ptr(), rows.stride(0),
+        rows.stride(1), rows.data_ptr(), rows.stride(0), rows.stride(1), cache.sequences, 0, 0, 0,
+        0, 1.0, None)
+    return code, _hip.lib().rkv_last_error().decode()
+
+
+def _shared_caches():
+    """(name, keys, values) whose cells overlap."""
+    k = torch.zeros(4, 2, 16, 8)
+    yield "one tensor", k, k
+    pool = torch.zeros(9, 2, 16, 8)
+    yield "a page on", pool[:8], pool[1:]
+    flat = torch.zeros(5000)
+    whole = torch.as_strided(flat, (4, 2, 16, 8), (256, 128, 8, 1))
+    yield "half a row on", whole, torch.as_strided(flat, (4, 2, 16, 8), (256, 128, 8, 1), 4)
+    yield "a row on", whole, torch.as_strided(flat, (4, 2, 16, 8), (256, 128, 8, 1), 8)
+    yield "the other order", whole, torch.as_strided(flat, (4, 2, 16, 8), (256, 8, 16, 1))
+    wide = torch.zeros(4, 2, 16, 12)
+    yield "columns that meet", wide[..., :8], wide[..., 4:]
+
+
+@pytest.mark.parametrize("name", [name for name, *_ in _shared_caches()])
+def test_append_refuses_keys_and_values_that_share_memory(name):
+    keys, values = {n: (k, v) for n, k, v in _shared_caches()}[name]
+    cache = PagedCache(keys, values, *_tables())
+    before = keys.clone()
+    with pytest.raises(ValueError, match="share memory"):
+        paged_append(_rows(cache), 2 * _rows(cache), cache)
+    assert torch.equal(keys, before)
+    code, why = _c_append(cache)
+    assert code == 1 and "share memory" in why, (code, why)
+
+
+def test_decode_over_shared_keys_and_values_still_answers():
+    keys = torch.randn(4, 1, 16, 8, generator=torch.Generator().manual_seed(1))
+    cache = PagedCache(keys, keys, *_tables())
+    query = torch.zeros(2, 1, 8)
+    want = torch.stack([keys[0, 0, :3].mean(0), torch.cat([keys[2, 0], keys[3, 0, :4]]).mean(0)])
+    assert torch.allclose(paged_decode(query, cache)[:, 0], want, atol=1e-6)
+
+
+def test_append_takes_interleaved_keys_and_values():
+    """Keys and values in one tensor, by page, row, head or column, and caches
+    one behind the other: every row is stored in its place."""
+    both = torch.zeros(4, 2, 2, 16, 8)
+    rows = torch.zeros(4, 16, 2, 2, 8)
+    wide = torch.zeros(4, 2, 16, 16)
+    flat = torch.zeros(4 * 512)
+    layouts = {
+        "pages": (both[:, 0], both[:, 1]), "heads": (both[:, :, 0], both[:, :, 1]),
+        "rows": (rows[:, :, 0].transpose(1, 2), rows[:, :, 1].transpose(1, 2)),
+        "columns": (wide[..., :8], wide[..., 8:]), "turned": (wide[..., 8:], wide[..., :8]),
+        # a page's keys head by head, its values row by row behind them
+        "orders": (torch.as_strided(flat, (4, 2, 16, 8), (512, 128, 8, 1)),
+                   torch.as_strided(flat, (4, 2, 16, 8), (512, 8, 16, 1), 256)),
+        "halves": (both.view(8, 2, 16, 8)[:4], both.view(8, 2, 16, 8)[4:]),
+        "one page": (both[:1, 0], both[:1, 1]),
+    }
+    for name, (keys, values) in layouts.items():
+        keys.zero_(), values.zero_()
+        table, lengths = _tables()
+        cache = PagedCache(keys, values, table, lengths)
+        paged_append(_rows(cache), 2 * _rows(cache), cache)
+        for t, fill in ((keys, 1.0), (values, 2.0)):
+            want = torch.zeros(t.shape)
+            want[0, :, 2] = fill
+            if cache.pages > 3:
+                want[3, :, 3] = fill
+            assert torch.equal(t, want), name
