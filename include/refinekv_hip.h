@@ -282,6 +282,8 @@ typedef struct rkv_paged_cache {
  * same tokens' queries) turned on the way as by rkv_rotary.
  *   key/value: (tokens, heads, dim) rows with token and head strides, the
  *     cache's dtype; query: (tokens, q_heads, dim) or q_heads 0.
+ *   query_out may be query itself (in place), else must not overlap any
+ *     input; one that overlaps the cache is refused.
  *   token_starts: device int32 (sequences + 1,): sequence b's new tokens are
  *     rows token_starts[b] .. token_starts[b + 1] - 1 and become its last
  *     ones, ending at position lengths[b] - 1; NULL: tokens = sequences, one
@@ -306,7 +308,8 @@ int rkv_paged_append(const rkv_paged_cache* cache, const void* query, int64_t q_
  *   out[b, h * group + g] = softmax_t(scale query[b, h * group + g] . K[b, h, t]) V[b, h, t]
  * over t < lengths[b] (rkv_dense_decode for many sequences in pages).
  *   query: (sequences, heads * group, dim) with sequence and head strides;
- *   output: the same shape, dense.  bf16 or fp16, dim 32..256 step 32, group
+ *   output: the same shape, dense, apart from the query and (else refused)
+ *   from the cache.  bf16 or fp16, dim 32..256 step 32, group
  *   <= 16; query, output and cache 16-byte aligned, strides multiples of 8.
  *   workspace: rkv_paged_plan's bytes.
  * lengths[b] <= 0 gives zeros.  A page outside the cache among the visible

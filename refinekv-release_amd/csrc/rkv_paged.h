@@ -96,4 +96,22 @@ inline bool keys_meet_values(const rkv_paged_cache* c) {
 // The stride of an axis of `count` places; that of a single place is not read.
 inline int64_t read_stride(int64_t stride, int64_t count) { return count > 1 ? stride : 0; }
 
+// Whether (tokens, heads, dim) rows may lie among a cache's pages: the spans of
+// both meet.
+inline bool rows_meet_pages(const rkv_paged_cache* c, const void* rows, int64_t token_stride,
+                            int64_t head_stride, int64_t tokens, int64_t heads) {
+  const int64_t size = dtype_bytes(c->dtype);
+  if (tokens <= 0 || heads <= 0) return false;
+  const uint64_t from = reinterpret_cast<uint64_t>(rows);
+  const uint64_t to = from + ((tokens - 1) * token_stride + (heads - 1) * head_stride + c->dim) * size;
+  auto meets = [&](const void* pages, int64_t page, int64_t head, int64_t token) {
+    const uint64_t first = reinterpret_cast<uint64_t>(pages);
+    const uint64_t end = first + ((c->pages - 1) * page + (c->heads - 1) * head +
+                                  (c->page_size - 1) * token + c->dim) * size;
+    return from < end && first < to;
+  };
+  return meets(c->keys, c->key_page_stride, c->key_head_stride, c->key_token_stride) ||
+         meets(c->values, c->value_page_stride, c->value_head_stride, c->value_token_stride);
+}
+
 }  // namespace rkv

@@ -778,6 +778,9 @@ extern "C" int rkv_paged_decode(const rkv_paged_cache* cache, const void* query,
     return set_error(kInvalidArgument,
                      "%s: query and output must be 16-byte aligned with strides in multiples of 8",
                      who);
+  if (rows_meet_pages(cache, output, cache->heads * group * cache->dim, cache->dim,
+                      cache->sequences, cache->heads * group))
+    return set_error(kInvalidArgument, "%s: output overlaps the cache", who);
   const PagedPlan P = paged_plan(cache, group);
   if (!workspace || workspace_bytes < P.total)
     return set_error(kWorkspaceTooSmall, "%s: workspace of %zu bytes, %zu needed", who,

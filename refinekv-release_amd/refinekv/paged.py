@@ -140,6 +140,19 @@ def _keys_meet_values(cache):
     return meet(0, cache.values.data_ptr() - cache.keys.data_ptr())
 
 
+def _meet_pages(rows, cache):
+    """Whether (tokens, heads, head_dim) rows may lie among the cache's pages,
+    by the C entries' rule: their spans meet."""
+    def span(t):
+        first, size = t.data_ptr(), t.element_size()
+        return first, first + size * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+    if rows.numel() == 0:
+        return False
+    first, end = span(rows)
+    return any(first < e and f < end for f, e in map(span, (cache.keys, cache.values)))
+
+
 def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=None,
                  query_out=None, backend="auto"):
     """Write new (tokens, kv_heads, head_dim) keys and values to their
@@ -149,7 +162,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     token_starts[b + 1] are sequence b's last tokens, ending at position
     lengths[b] - 1; without it every sequence has one.  With ``rotary`` keys
     and ``query`` (tokens, q_heads, head_dim) are turned to those positions;
-    ``query_out`` takes the turned queries (it may be the query itself).
+    ``query_out`` takes the turned queries (it may be the query itself, but not
+    lie in the cache).
 
     Rows of no sequence (behind the last one) or without a position (an idle
     place: length 0) are not stored, and their queries are returned unturned.
@@ -189,6 +203,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
 
     if _keys_meet_values(cache):
         raise ValueError("the cache's keys and values share memory")
+    if query_out is not None and _meet_pages(query_out, cache):
+        raise ValueError("query_out overlaps the cache")
     with torch.no_grad():
         turned = append(cache, key, value, query, rotary, token_starts)
         return turned if query_out is None else query_out.copy_(turned)
@@ -224,7 +240,8 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
 
     ``query`` (sequences, q_heads, head_dim), q_heads a multiple of the
     cache's heads (head h's rows are its group h); ``scaling`` defaults to
-    head_dim^-0.5.  Returns a new tensor of the query's shape, or ``output``.
+    head_dim^-0.5.  Returns a new tensor of the query's shape, or ``output``
+    (apart from the query and the cache).
     ``workspace`` (a dict) keeps the partial results' buffer from call to
     call; calls that share one must be ordered on one stream.
 
@@ -247,6 +264,8 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
         return _hip.paged_decode(query, cache, scaling, workspace, output)
     from .reference_paged import decode
 
+    if output is not None and _meet_pages(output, cache):
+        raise ValueError("output overlaps the cache")
     with torch.no_grad():
         out = decode(query, cache, scaling)
         return out if output is None else output.copy_(out)

@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from refinekv import PagedCache, paged_append, paged_decode
+from refinekv import PagedCache, Rotary, RotaryConfig, paged_append, paged_decode
 
 F32 = torch.float32
 
@@ -36,12 +36,12 @@ def _c_append(cache, **over):
         page_size=cache.page_size, dim=cache.head_dim, sequences=cache.sequences,
         max_blocks=cache.max_blocks, dtype=_hip.DTYPE_CODES[cache.dtype])
     rows = _rows(cache)
-    args = dict(query=0, q_heads=0, query_out=0)
+    args = dict(query=0, q_heads=0, query_out=0, out_strides=(0, 0))
     args.update(over)
     dim = cache.head_dim
     code = _hip.lib().rkv_paged_append(
         ctypes.byref(view), args["query"], args["q_heads"] * dim, dim, args["q_heads"],
-        args["query_out"], args["q_heads"] * dim, dim, rows.data_ptr(), rows.stride(0),
+        args["query_out"], *args["out_strides"], rows.data_ptr(), rows.stride(0),
         rows.stride(1), rows.data_ptr(), rows.stride(0), rows.stride(1), cache.sequences, 0, 0, 0,
         0, 1.0, None)
     return code, _hip.lib().rkv_last_error().decode()
@@ -110,3 +110,72 @@ def test_append_takes_interleaved_keys_and_values():
             if cache.pages > 3:
                 want[3, :, 3] = fill
             assert torch.equal(t, want), name
+
+
+def _cache(sequences=2):
+    return PagedCache(torch.zeros(6, 2, 16, 8), torch.zeros(6, 2, 16, 8), *_tables(sequences))
+
+
+def _places():
+    """(cache, (2, 2, 8) rows in or beside it, whether in it)."""
+    for name in ("keys", "values"):
+        cache = _cache()
+        pages = getattr(cache, name)
+        yield cache, pages[5].transpose(0, 1)[:2], True
+        yield cache, pages.view(-1)[-32:].view(2, 2, 8), True
+        yield cache, pages.view(-1)[:32].view(2, 2, 8), True
+    for place, inside in ((slice(0, 32), False), (slice(1, 33), True), (slice(-32, None), False),
+                          (slice(-33, -1), True)):
+        pool = torch.zeros(6 * 256 + 64)
+        cache = _cache()
+        cache = PagedCache(pool[32:-32].view(6, 2, 16, 8), cache.values, cache.block_table,
+                           cache.lengths)
+        yield cache, pool[place].view(2, 2, 8), inside
+
+
+def test_append_refuses_queries_turned_into_the_cache():
+    for cache, rows, inside in _places():
+        args = dict(query=torch.ones(2, 2, 8), rotary=Rotary(RotaryConfig(head_dim=8)),
+                    query_out=rows)
+        if not inside:
+            assert paged_append(_rows(cache), _rows(cache), cache, **args) is rows
+            assert cache.keys.any()
+            continue
+        with pytest.raises(ValueError, match="overlaps the cache"):
+            paged_append(_rows(cache), _rows(cache), cache, **args)
+        assert not cache.keys.any() and not cache.values.any()
+        code, why = _c_append(cache, query=4096, q_heads=2, query_out=rows.data_ptr(),
+                              out_strides=rows.stride()[:2])
+        assert code == 1 and "overlaps the cache" in why, (code, why)
+
+
+def test_decode_refuses_an_output_in_the_cache():
+    for cache, rows, inside in _places():
+        if not rows.is_contiguous():
+            continue
+        query = torch.ones(2, 2, 8)
+        if inside:
+            with pytest.raises(ValueError, match="overlaps the cache"):
+                paged_decode(query, cache, output=rows)
+        else:
+            assert paged_decode(query, cache, output=rows) is rows
+
+
+def test_c_decode_refuses_an_output_in_the_cache():
+    from refinekv import _hip
+
+    page = 16 * 2 * 64 * 2  # bytes of a page's keys
+    view = _hip._PagedCache(
+        keys=1 << 20, values=1 << 21, block_table=4096, lengths=4096, pages=4, heads=2,
+        page_size=16, dim=64, sequences=2, max_blocks=3, dtype=0, table_stride=3,
+        key_strides=(ctypes.c_int64 * 3)(2048, 1024, 64),
+        value_strides=(ctypes.c_int64 * 3)(2048, 1024, 64))
+    out_bytes = 2 * 8 * 64 * 2
+    for first in (1 << 20, 1 << 21):
+        for out in (first, first + 4 * page - 16, first - out_bytes + 16):
+            code = _hip.lib().rkv_paged_decode(ctypes.byref(view), 4096, 512, 64, 4, 0.125, out,
+                                               4096, 0, None)
+            assert code == 1 and b"overlaps the cache" in _hip.lib().rkv_last_error()
+        for out in (first - out_bytes, first + 4 * page):  # (the workspace is too small)
+            assert _hip.lib().rkv_paged_decode(ctypes.byref(view), 4096, 512, 64, 4, 0.125, out,
+                                               4096, 0, None) == 4
