@@ -29,7 +29,8 @@ enum {
   RKV_INVALID_ARGUMENT = 1, /* raised as ValueError by the Python binding */
   RKV_UNSUPPORTED = 2,      /* TypeError */
   RKV_LAUNCH_FAILED = 3,    /* RuntimeError */
-  RKV_WORKSPACE_TOO_SMALL = 4
+  RKV_WORKSPACE_TOO_SMALL = 4,
+  RKV_ROWS_IN_CACHE = 5 /* rkv_paged_append only */
 };
 
 /* GQA reduction codes (src/refinekv/kernels/runtime.py:23). */
@@ -284,6 +285,9 @@ typedef struct rkv_paged_cache {
  *     cache's dtype; query: (tokens, q_heads, dim) or q_heads 0.
  *   query_out may be query itself (in place), else must not overlap any
  *     input; one that overlaps the cache is refused.
+ *   key, value or query rows that overlap the cache would be read while their
+ *     pages are written: refused with RKV_ROWS_IN_CACHE (pass copies; the
+ *     Python binding makes them).
  *   token_starts: device int32 (sequences + 1,): sequence b's new tokens are
  *     rows token_starts[b] .. token_starts[b + 1] - 1 and become its last
  *     ones, ending at position lengths[b] - 1; NULL: tokens = sequences, one

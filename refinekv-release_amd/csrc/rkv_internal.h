@@ -16,6 +16,7 @@ enum Status : int {
   kUnsupported = 2,
   kLaunchFailed = 3,
   kWorkspaceTooSmall = 4,
+  kRowsInCache = 5,
 };
 
 int set_error(int code, const char* fmt, ...);

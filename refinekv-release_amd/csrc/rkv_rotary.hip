@@ -419,6 +419,10 @@ extern "C" int rkv_paged_append(const rkv_paged_cache* cache, const void* query,
     return set_error(kInvalidArgument, "%s: the cache's keys and values share memory", who);
   if (q_heads && rows_meet_pages(cache, query_out, qo_token_stride, qo_head_stride, tokens, q_heads))
     return set_error(kInvalidArgument, "%s: query_out overlaps the cache", who);
+  if (rows_meet_pages(cache, key, k_token_stride, k_head_stride, tokens, cache->heads) ||
+      rows_meet_pages(cache, value, v_token_stride, v_head_stride, tokens, cache->heads) ||
+      (q_heads && rows_meet_pages(cache, query, q_token_stride, q_head_stride, tokens, q_heads)))
+    return set_error(kRowsInCache, "%s: rows overlap the cache", who);
   RotaryArgs a{};
   a.rows[0] = plain_rows(tokens, query, q_token_stride, q_head_stride, q_heads, query_out,
                          qo_token_stride, qo_head_stride);

@@ -597,6 +597,9 @@ def rotary(query, key, positions, table, query_out=None, key_out=None, inverse=F
     return query_out, key_out
 
 
+ROWS_IN_CACHE = 5  # RKV_ROWS_IN_CACHE
+
+
 def _cache_struct(cache):
     """The C view of a PagedCache (made on its first call; the pointers are
     taken from the tensors on every call) and a reference to it."""
@@ -633,6 +636,11 @@ def paged_append(key, value, cache, query=None, table=None, token_starts=None, q
     rc = lib().rkv_paged_append(
         _cache_struct(cache), *rows, *_rows(key), *_rows(value), key.shape[0],
         0 if token_starts is None else token_starts.data_ptr(), *turns, _raw_stream(device))
+    if rc == ROWS_IN_CACHE:
+        key, value = (t.clone(memory_format=torch.contiguous_format) for t in (key, value))
+        if query is not None:
+            query = query.clone(memory_format=torch.contiguous_format)
+        return paged_append(key, value, cache, query, table, token_starts, query_out)
     if rc:
         _check(rc, "rkv_paged_append")
     return query_out

@@ -170,7 +170,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     A row whose page is outside the cache, or past the block table, is not
     stored.  No two rows of a call may fall on the same place: a page written
     here belongs to one sequence, and a cache whose keys and values share
-    memory is refused.
+    memory is refused.  Rows that are views of the cache's pages are copied
+    first: the call stores what they hold before it.
 
     (A prompt's own attention needs its turned keys as well: turn both with
     rotate_heads, then append without ``rotary``.)

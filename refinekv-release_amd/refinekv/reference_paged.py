@@ -54,9 +54,12 @@ def append(cache, key, value, query, rotary, token_starts):
     stored = live & (block < cache.max_blocks) & (page >= 0) & (page < cache.pages)
     turned = key if rotary is None else rotate(key, position, rotary)
     at, row = page[stored], (position % cache.page_size)[stored]
-    cache.keys[at, :, row] = turned[stored]
-    cache.values[at, :, row] = value[stored]
-    return None if query is None else rotate(query, position, rotary, live=live)
+    # (all rows are read before any is stored: they may be views of the pages)
+    out = None if query is None else rotate(query, position, rotary, live=live)
+    turned, value = turned[stored], value[stored]
+    cache.keys[at, :, row] = turned
+    cache.values[at, :, row] = value
+    return out
 
 
 def decode(query, cache, scaling):

@@ -35,10 +35,9 @@ def _c_append(cache, **over):
         lengths=cache.lengths.data_ptr(), pages=cache.pages, heads=cache.heads,
         page_size=cache.page_size, dim=cache.head_dim, sequences=cache.sequences,
         max_blocks=cache.max_blocks, dtype=_hip.DTYPE_CODES[cache.dtype])
-    rows = _rows(cache)
-    args = dict(query=0, q_heads=0, query_out=0, out_strides=(0, 0))
+    args = dict(rows=_rows(cache), query=0, q_heads=0, query_out=0, out_strides=(0, 0))
     args.update(over)
-    dim = cache.head_dim
+    dim, rows = cache.head_dim, args["rows"]
     code = _hip.lib().rkv_paged_append(
         ctypes.byref(view), args["query"], args["q_heads"] * dim, dim, args["q_heads"],
         args["query_out"], *args["out_strides"], rows.data_ptr(), rows.stride(0),
@@ -179,3 +178,44 @@ def test_c_decode_refuses_an_output_in_the_cache():
         for out in (first - out_bytes, first + 4 * page):  # (the workspace is too small)
             assert _hip.lib().rkv_paged_decode(ctypes.byref(view), 4096, 512, 64, 4, 0.125, out,
                                                4096, 0, None) == 4
+
+
+def rows_of_pages(append):
+    """append(cache, key, value, query, rotary) with rows that are views of
+    pages the same call writes, against the same call with copies."""
+    gen = torch.Generator().manual_seed(7)
+    start = [torch.randn(6, 2, 16, 8, generator=gen) for _ in range(2)]
+    rotary = Rotary(RotaryConfig(head_dim=8))
+    results = []
+    for copied in (False, True):
+        cache = PagedCache(start[0].clone(), start[1].clone(), *_tables())
+        # sequence 0's token goes to row 2 of page 0, sequence 1's to row 3 of page 3
+        key = cache.keys[0].transpose(0, 1)[2:4]
+        value = cache.keys[3].transpose(0, 1)[3:5]
+        query = cache.values[0].transpose(0, 1)[1:3]
+        if copied:
+            key, value, query = key.clone(), value.clone(), query.clone()
+        out = append(cache, key, value, query, rotary)
+        results.append((out, cache.keys, cache.values))
+    for got, want in zip(*results):
+        assert torch.equal(got, want)
+    assert not torch.equal(results[1][1], start[0])
+
+
+def test_append_stores_what_its_rows_held_before():
+    rows_of_pages(lambda cache, key, value, query, rotary: paged_append(
+        key, value, cache, query=query, rotary=rotary))
+
+
+def test_c_append_names_rows_in_the_cache():
+    from refinekv import _hip
+
+    for which in ("rows", "query"):
+        cache = _cache()
+        for name in ("keys", "values"):
+            pages = getattr(cache, name)
+            rows = pages[5].transpose(0, 1)[:2]
+            over = (dict(rows=rows) if which == "rows" else
+                    dict(query=rows.data_ptr(), q_heads=2, query_out=4096, out_strides=(16, 8)))
+            code, why = _c_append(cache, **over)
+            assert code == _hip.ROWS_IN_CACHE and "rows overlap the cache" in why, (code, why)
