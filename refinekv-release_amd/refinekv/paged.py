@@ -261,12 +261,15 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
             raise ValueError("output must not overlap the query")
     scaling = cache.head_dim ** -0.5 if scaling is None else float(scaling)
     why = _decode_support(cache, group) if query.is_cuda else None
-    if pick_backend(query, backend, why is None, why) == "hip":
+    hip = pick_backend(query, backend, why is None, why) == "hip"
+    if hip and (output is None or output.data_ptr() % 16 == 0):
         return _hip.paged_decode(query, cache, scaling, workspace, output)
     from .reference_paged import decode
 
     if output is not None and _meet_pages(output, cache):
         raise ValueError("output overlaps the cache")
+    if hip:  # (the kernel stores whole vectors)
+        return output.copy_(_hip.paged_decode(query, cache, scaling, workspace))
     with torch.no_grad():
         out = decode(query, cache, scaling)
         return out if output is None else output.copy_(out)

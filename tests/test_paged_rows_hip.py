@@ -1,9 +1,9 @@
-"""Rows that are views of the cache's own pages, through the kernels (GPU)."""
+"""Rows and outputs in unusual places, through the kernels (GPU)."""
 
 import pytest
 import torch
 
-from refinekv import PagedCache, paged_append
+from refinekv import PagedCache, paged_append, paged_decode
 from test_paged_overlap_cpu import rows_of_pages
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +27,28 @@ def test_append_stores_what_its_rows_held_before():
         return out.cpu()
 
     rows_of_pages(append)
+
+
+def test_decode_into_an_output_at_any_address():
+    """An output that starts anywhere its type may: the kernel stores whole
+    vectors, so that the result goes there by a copy."""
+    gen = torch.Generator().manual_seed(3)
+    keys, values = (torch.randn(6, 2, 16, 64, generator=gen).to(torch.bfloat16).cuda()
+                    for _ in range(2))
+    table = torch.arange(6, dtype=torch.int32, device="cuda").view(2, 3)
+    cache = PagedCache(keys, values, table,
+                       torch.tensor([17, 40], dtype=torch.int32, device="cuda"))
+    query = torch.randn(2, 6, 64, generator=gen).to(torch.bfloat16).cuda()
+    want = paged_decode(query, cache, backend="hip")
+    for first in (1, 4, 8):
+        room = torch.full((query.numel() + 16,), 7.0, dtype=torch.bfloat16, device="cuda")
+        output = room[first:first + query.numel()].view(query.shape)
+        for backend in ("auto", "hip"):
+            output.zero_()
+            assert paged_decode(query, cache, output=output, backend=backend) is output
+            assert torch.equal(output, want)
+        assert (room[:first] == 7).all() and (room[first + query.numel():] == 7).all()
+    odd = keys.view(-1)[3:3 + query.numel()].view(query.shape)
+    for backend in ("auto", "hip"):
+        with pytest.raises(ValueError, match="overlaps the cache"):
+            paged_decode(query, cache, output=odd, backend=backend)
