@@ -320,7 +320,8 @@ int rkv_paged_append(const rkv_paged_cache* cache, const void* query, int64_t q_
  * ones, or a length past the table, gives NaN in that sequence's rows.  What
  * lies behind a sequence's end is not read.  Scores of +inf or NaN make a row
  * NaN, as a softmax does, and so do scores of -inf alone; an infinite visible
- * value makes its dim infinite or NaN.
+ * value makes its dim infinite, and NaN if its weight is 0 (below 2^-126 of the
+ * row's largest) or another one has the other sign.
  */
 int rkv_paged_decode(const rkv_paged_cache* cache, const void* query, int64_t q_sequence_stride,
                      int64_t q_head_stride, int64_t group, float scale, void* output,

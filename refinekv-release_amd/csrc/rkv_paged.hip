@@ -406,6 +406,34 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
       begun = c.tile == 0;
     };
 
+    // Whether any of the tile's values is infinite or NaN: its product with
+    // zeros shows it as NaN.  (8 products more a tile at head_dim 128, on matrix
+    // cores that wait for memory: 131072 tokens 91.6 -> 92.1 us, 2003 tokens
+    // 11.85 -> 11.94, 128 short sequences at head_dim 64 71.6 -> 72.2.)
+    auto has_infinite = [&](const Tile<D>& t) -> bool {
+      F32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto add = [&](U32x4 words) { sum = T::mma(__builtin_bit_cast(V8, words), V8{}, sum); };
+#pragma unroll
+      for (int c8 = 0; c8 < P::k8; ++c8)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) add(t.v8[c8][e]);
+      if constexpr (P::k4 > 0)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+          add(U32x4{t.v4[e][0], t.v4[e][1], t.v4[e + 1][0], t.v4[e + 1][1]});
+      if constexpr (P::k2 > 0)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) add(U32x4{t.v2[e], t.v2[e + 1], t.v2[e + 2], t.v2[e + 3]});
+      return __builtin_amdgcn_ballot_w64(sum[0] + sum[1] + sum[2] + sum[3] != 0.0f) != 0;
+    };
+
+    // Ones over the halves of a word that are infinite or NaN (the sum's top
+    // bits: exponents of all ones).
+    auto infinite_of = [](uint32_t w) -> uint32_t {
+      const uint32_t top = (w & 0x7fff7fffu) + (kHalf ? 0x04000400u : 0x00800080u);
+      return (top >> 15 & 0x00010001u) * 0xffffu;
+    };
+
     auto compute = [&](const Cursor& c, Tile<D>& t, bool bad, bool last_tile) {
       bad_row |= bad;
       {
@@ -443,56 +471,87 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
           for (int n = 0; n < P::kBlocks; ++n) acc[n] *= by;
         }
         const float base = m == kNegInf ? 0.0f : m;
-        V8 hi, lo, last;
+        float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           // (fp16 weights go up to 2^15 instead of 1, and the sum with them, so
           // that those of 2^-24 to 2^-39 of the largest, many in a long
           // context, do not round to zero)
-          const float p = __builtin_amdgcn_exp2f(x[e] - base) * (kHalf ? 32768.0f : 1.0f);
-          l += p;
+          p[e] = __builtin_amdgcn_exp2f(x[e] - base) * (kHalf ? 32768.0f : 1.0f);
+          l += p[e];
+        }
+        // dims' products: byte permutes gather one dim of two tokens a word
+        auto each_product = [&](auto add) {
+          constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
+#pragma unroll
+          for (int n = 0; n < P::kBlocks; ++n) {
+            U32x4 words;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t even, odd;
+              int d;
+              if (n < 8 * P::k8) {
+                d = n % 8;
+                even = t.v8[n / 8][2 * e][d / 2];
+                odd = t.v8[n / 8][2 * e + 1][d / 2];
+              } else if (n < 8 * P::k8 + 4 * P::k4) {
+                d = n - 8 * P::k8;
+                even = t.v4[2 * e][d / 2];
+                odd = t.v4[2 * e + 1][d / 2];
+              } else {
+                d = n - 8 * P::k8 - 4 * P::k4;
+                even = t.v2[2 * e];
+                odd = t.v2[2 * e + 1];
+              }
+              words[e] = __builtin_amdgcn_perm(odd, even, d % 2 ? kHigh : kLow);
+            }
+            add(n, words);
+          }
+        };
+        if (has_infinite(t)) {
+          // Parts of a weight may be 0, and 0 times infinity is NaN: infinities
+          // and NaN count here, times 1 (0 where the weight itself is), and as
+          // 0 below.
+          V8 some;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) some[e] = (E)(p[e] == 0.0f ? 0.0f : 1.0f);
+          each_product([&](int n, U32x4 words) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) words[e] &= infinite_of(words[e]);
+            acc[n] = T::mma(__builtin_bit_cast(V8, words), some, acc[n]);
+          });
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+#pragma unroll
+            for (int c8 = 0; c8 < P::k8; ++c8)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) t.v8[c8][e][i] &= ~infinite_of(t.v8[c8][e][i]);
+            if constexpr (P::k4 > 0)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) t.v4[e][i] &= ~infinite_of(t.v4[e][i]);
+            if constexpr (P::k2 > 0) t.v2[e] &= ~infinite_of(t.v2[e]);
+          }
+        }
+        V8 hi, lo, last;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
           // the weight as a sum of 16-bit parts that holds all of it: two of
           // fp16 (to 2^-23), three of bf16 (exact).  (Two of bf16 hold it to
           // 2^-17: 1.4 times as many outputs rounded the other way at 131072
           // tokens, and the same 92 us; 128 short sequences at head_dim 64 70.9
           // us against 73.3.)
-          hi[e] = (E)p;
-          const float rest = p - (float)hi[e];
+          hi[e] = (E)p[e];
+          const float rest = p[e] - (float)hi[e];
           lo[e] = (E)rest;
           if constexpr (!kHalf) last[e] = (E)(rest - (float)lo[e]);
         }
-        // dims' products: byte permutes gather one dim of two tokens a word
-        auto product = [&](int n, uint32_t (&words)[4]) {
-          const V8 v = __builtin_bit_cast(V8, U32x4{words[0], words[1], words[2], words[3]});
+        auto add_product = [&](int n, U32x4 words) {
+          const V8 v = __builtin_bit_cast(V8, words);
           acc[n] = T::mma(v, hi, acc[n]);
           acc[n] = T::mma(v, lo, acc[n]);
           if constexpr (!kHalf) acc[n] = T::mma(v, last, acc[n]);
         };
-        constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
-#pragma unroll
-        for (int n = 0; n < P::kBlocks; ++n) {
-          uint32_t words[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t even, odd;
-            int d;
-            if (n < 8 * P::k8) {
-              d = n % 8;
-              even = t.v8[n / 8][2 * e][d / 2];
-              odd = t.v8[n / 8][2 * e + 1][d / 2];
-            } else if (n < 8 * P::k8 + 4 * P::k4) {
-              d = n - 8 * P::k8;
-              even = t.v4[2 * e][d / 2];
-              odd = t.v4[2 * e + 1][d / 2];
-            } else {
-              d = n - 8 * P::k8 - 4 * P::k4;
-              even = t.v2[2 * e];
-              odd = t.v2[2 * e + 1];
-            }
-            words[e] = __builtin_amdgcn_perm(odd, even, d % 2 ? kHigh : kLow);
-          }
-          product(n, words);
-        }
+        each_product(add_product);
       }
       const bool ends = c.tile + 1 == c.tiles;
       if (!ends && !last_tile) return;
