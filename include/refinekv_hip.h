@@ -313,7 +313,7 @@ int rkv_paged_append(const rkv_paged_cache* cache, const void* query, int64_t q_
  * over t < lengths[b] (rkv_dense_decode for many sequences in pages).
  *   query: (sequences, heads * group, dim) with sequence and head strides;
  *   output: the same shape, dense, apart from the query and (else refused)
- *   from the cache.  bf16 or fp16, dim 32..256 step 32, group
+ *   from the cache.  bf16 or fp16 (no fp32, unlike the append), dim 32..256 step 32, group
  *   <= 16; query, output and cache 16-byte aligned, strides multiples of 8.
  *   workspace: rkv_paged_plan's bytes.
  * lengths[b] <= 0 gives zeros.  A page outside the cache among the visible

@@ -11,9 +11,10 @@ token per sequence over its visible tokens.  A decode step::
     query = paged_append(key, value, cache, query=query, rotary=rotary)
     output = paged_decode(query, cache, workspace=workspace)
 
-Lengths and block table are read on the device, so one captured HIP graph
-serves every step of a batch.  ROCm tensors use the gfx950 kernels, others
-(and the types and shapes the kernels do not take) torch operations.
+The kernels read lengths and block table on the device, so one captured HIP
+graph serves every step of a batch.  ROCm tensors use the gfx950 kernels,
+others (and the types and shapes the kernels do not take) torch operations,
+which read lengths on the host: those calls cannot be captured and say so.
 Inference only, as the whole package: the results carry no gradient.
 """
 
@@ -115,6 +116,13 @@ def _check_rows(name, rows, cache, tokens, heads=None):
         raise ValueError(f"{name} must have the cache's dtype and device")
 
 
+def _check_capture(rows, why):
+    """The torch operations ask the device for values, which a capture does not
+    allow."""
+    if rows.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"this call cannot be captured in a graph: {why}")
+
+
 def _keys_meet_values(cache):
     """Whether the cache's keys and values may share memory: the C entry's own
     rule, for the torch operations."""
@@ -197,10 +205,12 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
             check_out("query_out", query_out, query, (key, value))
     elif query_out is not None:
         raise ValueError("query_out without a query")
-    if pick_backend(key, backend, key.dtype in DTYPES,
-                    "the HIP append needs a bf16, fp16 or fp32 cache") == "hip":
+    why = None if key.dtype in DTYPES else "the HIP append needs a bf16, fp16 or fp32 cache"
+    if pick_backend(key, backend, why is None, why) == "hip":
         return _hip.paged_append(key, value, cache, query, rotary, token_starts, query_out)
     from .reference_paged import append
+
+    _check_capture(key, why or "backend='torch'")
 
     if _keys_meet_values(cache):
         raise ValueError("the cache's keys and values share memory")
@@ -264,6 +274,8 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
     hip = pick_backend(query, backend, why is None, why) == "hip"
     if hip and (output is None or output.data_ptr() % 16 == 0):
         return _hip.paged_decode(query, cache, scaling, workspace, output)
+    if not hip:
+        _check_capture(query, why or "backend='torch'")
     from .reference_paged import decode
 
     if output is not None and _meet_pages(output, cache):

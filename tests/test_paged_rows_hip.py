@@ -52,3 +52,27 @@ def test_decode_into_an_output_at_any_address():
     for backend in ("auto", "hip"):
         with pytest.raises(ValueError, match="overlaps the cache"):
             paged_decode(query, cache, output=odd, backend=backend)
+
+
+def test_calls_that_cannot_be_captured_say_so():
+    """What the kernels do not take goes to torch operations that read the
+    lengths on the host: under a capture that is refused before any of them."""
+    cache = PagedCache.empty(4, 1, 16, 64, 2, 2, dtype=torch.float32, device="cuda")
+    wide = PagedCache.empty(4, 1, 16, 64, 2, 2, dtype=torch.float64, device="cuda")
+    query = torch.zeros(2, 1, 64, device="cuda")
+    paged_append(query, query, cache, backend="hip")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged_append(query, query, cache, backend="hip")
+        with pytest.raises(RuntimeError, match="cannot be captured.*bf16 or fp16"):
+            paged_decode(query, cache)
+        with pytest.raises(RuntimeError, match="cannot be captured.*backend='torch'"):
+            paged_append(query, query, cache, backend="torch")
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            paged_append(query.new_zeros(0, 1, 64, dtype=torch.float64),
+                         query.new_zeros(0, 1, 64, dtype=torch.float64), wide,
+                         token_starts=cache.block_table.new_empty(3))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not paged_decode(query, cache).any()
