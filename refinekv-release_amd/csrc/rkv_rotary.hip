@@ -23,10 +23,14 @@ constexpr int kThreads = 256;
 // heads 611, 551 and 592 against 555, eight tokens of 40 heads 4.2, - and 5.1
 // against 4.2).
 constexpr int kBatch = 2;
-// A call that moves more than the caches hold stores past them (64 K tokens of
-// 28 + 4 heads, 537 MB written: 210 -> 198 us); what a smaller one writes is
-// left there for whoever reads it next.
-constexpr int64_t kStreamBytes = int64_t(64) << 20;
+// A call that writes more than the last-level cache holds (256 MB) stores past
+// it; what a smaller one writes is left there for whoever reads it next.
+// Rotation of 28 + 4 heads, in parentheses with an elementwise kernel that then
+// reads the queries, us by bytes written: stored past the cache and not, 64 MB
+// 27.1 (46.9) and 26.8 (44.2), 128 MB 49.1 (85.2) and 47.5 (80.4), 192 MB 70.6
+// (123) and 66.5 (119), 256 MB 92.9 (176) and 86.5 (180), 384 MB 137 (258) and
+// 150 (268), 512 MB 182 (340) and 199 (357).
+constexpr int64_t kStreamBytes = int64_t(256) << 20;
 // From so many threads on the device is full (4 waves per SIMD), and fewer
 // threads turn more heads each with the same cos and sin.
 constexpr int64_t kManyThreads = 4 * 1024 * 64;

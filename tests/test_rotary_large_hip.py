@@ -10,7 +10,7 @@ from refinekv import PagedCache, Rotary, RotaryConfig, paged_append, rotate_head
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
-STREAM_BYTES = 64 << 20
+STREAM_BYTES = 256 << 20
 
 
 def bits(t):
@@ -24,11 +24,12 @@ def _in_pieces(rows, positions, rotary, piece):
 
 
 CASES = [  # tokens, heads, KV heads, dim, rotary_dim, interleaved, dtype, passes the caches
-    (5003, 17, 3, 128, 128, False, BF16, False), (14003, 17, 3, 128, 128, False, BF16, True),
-    (9001, 7, 2, 256, 64, True, F32, True), (21011, 13, 4, 96, 48, True, F16, True),
-    (6007, 40, 5, 128, 64, False, BF16, True), (100003, 43, 7, 7, 6, False, F16, True),
-    (100003, 43, 7, 7, 6, True, BF16, True), (30011, 9, 1, 128, 128, True, BF16, True),
-    (1021, 131, 2, 256, 256, False, F32, True), (7001, 16, 3, 88, 48, True, F16, False),
+    (5003, 17, 3, 128, 128, False, BF16, False), (14003, 17, 3, 128, 128, False, BF16, False),
+    (53003, 17, 3, 128, 128, False, BF16, True), (30001, 7, 2, 256, 64, True, F32, True),
+    (21011, 13, 4, 96, 48, True, F16, False), (83011, 13, 4, 96, 48, True, F16, True),
+    (24007, 40, 5, 128, 64, False, BF16, True), (100003, 43, 7, 7, 6, False, F16, False),
+    (390011, 43, 7, 7, 6, True, BF16, True), (106013, 9, 1, 128, 128, True, BF16, True),
+    (2039, 131, 2, 256, 256, False, F32, True), (7001, 16, 3, 88, 48, True, F16, False),
 ]
 
 
@@ -43,7 +44,7 @@ def test_rotate_heads_of_many_tokens(tokens, heads, kv, dim, rotary_dim, interle
                           interleaved=interleaved)
     rotary = Rotary(config, "cuda")
     assert (tokens * (heads + kv) * dim * fused.element_size() >= STREAM_BYTES) == streams
-    want = [_in_pieces(x, positions, rotary, 97 if tokens < 50000 else 499) for x in (query, key)]
+    want = [_in_pieces(x, positions, rotary, 97 if tokens < 20000 else 499) for x in (query, key)]
     pick = torch.cat([torch.arange(40), torch.arange(tokens - 40, tokens),
                       torch.randint(0, tokens, (100,), generator=torch.Generator().manual_seed(1))])
     for x, y in zip((query, key), want):
@@ -81,7 +82,7 @@ def test_append_of_many_tokens(tokens, heads, kv, dim, rotary_dim, interleaved, 
                           scaling="yarn", factor=4.0, original_length=32768)
     rotary = Rotary(config, "cuda")
     positions = torch.cat([torch.arange(n) for n in lengths]).cuda()
-    turned = [_in_pieces(x[:tokens - 3], positions, rotary, 97 if tokens < 50000 else 499)
+    turned = [_in_pieces(x[:tokens - 3], positions, rotary, 97 if tokens < 20000 else 499)
               for x in (query, key)]
     out = paged_append(key, value, cache, query=query, rotary=rotary,
                        token_starts=torch.tensor(starts, dtype=torch.int32, device="cuda"),
