@@ -43,6 +43,13 @@ constexpr int kOpenStride = 16;
 // of their pages lose what the caches would have held: 16 on the same 32768
 // tokens 172 -> 276 us, 64 on the same 4096 95 -> 99; the call cannot know.)
 constexpr int kStreamLoad = 2;
+// That of a row's last 32 value dims, which lie in the half of a 128-byte line:
+// kept where other loads take the rest of the line (head_dim 96, 32 x 8000
+// tokens, 85.8 us against 87.2 non-temporal, 160 81.9 against 83.8, 224 82.2
+// against 83.2), non-temporal where there are no others (head_dim 32, 64
+// sequences of up to 20000 tokens, 129.4 against 134).
+template <int D>
+constexpr int kTailLoad = D == 32 ? kStreamLoad : 0;
 
 typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
@@ -389,7 +396,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedAr
                 vr, (int)(vo + li * 8u + 256u * P::k8), 0, kStreamLoad);
           if constexpr (P::k2 > 0)
             t.v2[4 * s + e] = __builtin_amdgcn_raw_buffer_load_b32(
-                vr, (int)(vo + li * 4u + 256u * P::k8 + 128u * P::k4), 0, 0);
+                vr, (int)(vo + li * 4u + 256u * P::k8 + 128u * P::k4), 0, kTailLoad<D>);
         }
       }
       return bad;
