@@ -598,6 +598,7 @@ def rotary(query, key, positions, table, query_out=None, key_out=None, inverse=F
 
 
 ROWS_IN_CACHE = 5  # RKV_ROWS_IN_CACHE
+MAX_HEAD_STRIDE = 1 << 25  # of rkv_paged_decode's query, elements
 
 
 def _cache_struct(cache):
@@ -665,6 +666,8 @@ def paged_decode(query, cache, scaling, workspace=None, output=None):
             return paged_decode(query, cache, scaling, workspace, output)
     group = query.shape[1] // cache.heads
     query = _row_aligned(query, 16)
+    if query.stride(1) > MAX_HEAD_STRIDE:
+        query = query.contiguous()
     if output is None:
         output = _like(query)
     nbytes = _paged_bytes(cache, group)

@@ -76,3 +76,19 @@ def test_calls_that_cannot_be_captured_say_so():
     graph.replay()
     torch.cuda.synchronize()
     assert not paged_decode(query, cache).any()
+
+
+def test_decode_of_queries_with_far_heads():
+    """Heads further apart than the kernel's 32-bit offsets reach are copied
+    together, like rows that are not aligned."""
+    gen = torch.Generator().manual_seed(4)
+    keys, values = (torch.randn(4, 1, 16, 64, generator=gen).to(torch.bfloat16).cuda()
+                    for _ in range(2))
+    cache = PagedCache(keys, values, torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2),
+                       torch.tensor([9, 30], dtype=torch.int32, device="cuda"))
+    near = torch.randn(2, 2, 64, generator=gen).to(torch.bfloat16).cuda()
+    far = torch.empty((1 << 25) + 1024, dtype=torch.bfloat16, device="cuda").as_strided(
+        (2, 2, 64), (64, (1 << 25) + 8, 1)).copy_(near)
+    want = paged_decode(near, cache, backend="hip")
+    for backend in ("auto", "hip"):
+        assert torch.equal(paged_decode(far, cache, backend=backend), want)
