@@ -246,7 +246,8 @@ int rkv_dense_plan(int64_t heads, int64_t group, int64_t dim, int64_t length, in
  *   inverse != 0 turns by -t (the transposed rotation; scale applies alike).
  *   query_out / key_out may be query / key themselves (in place), else must
  *   not overlap any input.
- * The angle is reduced in fp64, the products are fp32, rounded once.
+ * The angle is reduced in fp64 (position * rate below 2^49 turns), the products
+ * are fp32, rounded once.
  */
 int rkv_rotary(const void* query, int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
                const void* key, int64_t k_token_stride, int64_t k_head_stride, int64_t k_heads,

@@ -26,9 +26,10 @@ constexpr int kTileTokens = 32;  // tokens a wave takes at a time: two halves of
 
 // Workgroups per CU that share the tiles.  One keeps the CU's loads full (each
 // of its waves has two tiles on their way) and leaves the fewest parts to
-// join; at head_dim 32 a tile is 4 KB and two are needed (64 sequences of up
-// to 20000 tokens 77.5 -> 67.5 us; head_dim 64, 8 x 60000 tokens 165 -> 167,
-// 96, 100000 tokens 35.9 -> 37.9, 128, 131072 tokens 92.2 -> 93.4).
+// join; at head_dim 32 a tile is 4 KB and two are needed.  From one to two: 32,
+// 64 sequences of up to 20000 tokens 157 -> 129.5 us; 64, 128 of up to 2000
+// 72.5 -> 72.2; 96, 32 of up to 8000 85.9 -> 87.9; 128, 131072 tokens 92.4 ->
+// 94.0; 160, 24 of up to 4000 61.3 -> 67.7.
 template <int D>
 constexpr int kPerCu = D < 64 ? 2 : 1;
 
@@ -38,10 +39,11 @@ constexpr int kPerCu = D < 64 ? 2 : 1;
 constexpr int kOpenStride = 16;
 
 // Cache policy of the key and value loads: non-temporal.  A token is read once
-// a step, and kept lines only push out others: 16 x 131072 tokens 1470 -> 1327
-// us, one 103.5 -> 92, 64 ragged ones 112 -> 100.  (Sequences that share most
+// a step, and kept lines only push out others: 16 x 131072 tokens 1465 -> 1322
+// us, one 103.5 -> 92.4, 64 ragged ones 111 -> 99.  (Sequences that share most
 // of their pages lose what the caches would have held: 16 on the same 32768
-// tokens 172 -> 276 us, 64 on the same 4096 95 -> 99; the call cannot know.)
+// tokens 156 -> 206 us, 172 -> 276 on another card, 64 on the same 4096 79 ->
+// 82; the host, which picks the kernel, does not know.)
 constexpr int kStreamLoad = 2;
 // That of a row's last 32 value dims, which lie in the half of a 128-byte line:
 // kept where other loads take the rest of the line (head_dim 96, 32 x 8000
@@ -279,10 +281,11 @@ __device__ __forceinline__ void fold_parts(uint32_t first, uint32_t step, uint32
 //     transposes them with byte permutes; the m-th of 8 products takes dim
 //     8 (l % 16) + m for its row l % 16.  (Rows of 64 and 32 dims: 4 and 2.)
 // HBM bounds it: 8.6 GB of 16 x 131072 tokens (8 KV heads, group 4, d 128) in
-// 1253-1327 us, 6.5-6.9 TB/s, by the box; the matrix cores are at 6 % and the
-// vector ALUs at 11 %.  Small calls are a chain of latencies: 504 tiles of
-// 2003 tokens take 7 us, of which 2 to know the share and its pages, 2 for
-// the loads, 1.3 to join the waves; then 4 for the join kernel.
+// 1250-1325 us, 6.5-6.9 TB/s, by the card; the matrix cores are at 10 % and the
+// vector ALUs at 15 %.  Small calls are a chain of latencies: 504 tiles of
+// 2003 tokens take 7.2 us, of which 1.4 to know the share and its pages, 2.6
+// until the first tile is done, 1.4 to join the waves; then 4.6 for the join
+// kernel.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void paged_kernel(PagedArgs a) {

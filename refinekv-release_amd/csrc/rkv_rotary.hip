@@ -19,9 +19,9 @@ namespace {
 
 constexpr int kThreads = 256;
 // Heads of a thread's loads in flight together (1, 3 and 4 instead of 2: 64 K
-// tokens of 28 + 4 heads 194, 198 and 186 us against 187, 131001 tokens of 48
-// heads 611, 551 and 592 against 555, eight tokens of 40 heads 4.2, - and 5.1
-// against 4.2).
+// tokens of 28 + 4 heads 187, 185 and 181 us against 183, 131001 tokens of 48
+// heads 553, 561 and 546 against 541, 24 K ragged ones of 36 heads 37, 38 and
+// 41 against 36, eight tokens of 40 heads 4.1, 4.5 and 4.8 against 4.0).
 constexpr int kBatch = 2;
 // A call that writes more than the last-level cache holds (256 MB) stores past
 // it; what a smaller one writes is left there for whoever reads it next.
@@ -147,7 +147,7 @@ __device__ __forceinline__ Place place_of(const RotaryArgs& a, int64_t t) {
 // pairs each; W 1: one pair), and side by side too where dims pass.  A part
 // that is an odd number of vectors has one in its last item.  (One vector an
 // item where dims pass: 50266 tokens of 28 + 4 heads, 64 of 128 dims turning,
-// 207 us.)  The thread works out the item's cos and sin once and
+// 207 us against 182.)  The thread works out the item's cos and sin once and
 // applies them to every slots-th head of its token, kBatch heads at a time
 // whose loads are all in flight before the first use; those of the first
 // batch are on their way before the position is known.
@@ -288,8 +288,8 @@ int launch_w(RotaryArgs& a, hipStream_t stream) {
   const int wide = a.items < kThreads ? a.items : kThreads;
   // Few tokens: every thread kBatch heads, for latency.  Many: a wave holds
   // one token's consecutive heads (d 128: 8 heads, 2 KB), each thread every
-  // 8th of them (against every 4th and 16th, 64 K tokens of 28 + 4 heads: 187
-  // against 197 and 200 us, 131001 of 48 heads 555 against 576 and 620).
+  // 8th of them (against every 4th and 16th, 64 K tokens of 28 + 4 heads: 183
+  // against 197 and 192 us, 131001 of 48 heads 541 against 584 and 553).
   a.slots = (a.heads + kBatch - 1) / kBatch;
   if (a.tokens * wide * a.slots >= kManyThreads) a.slots = wide < kWave ? kWave / wide : 1;
   a.slots = a.slots < a.heads ? a.slots : a.heads;

@@ -212,7 +212,8 @@ def rotate_heads(query, key, positions, rotary, *, query_out=None, key_out=None,
                  backend="auto"):
     """Turn (tokens, heads, head_dim) query and key rows to their positions.
 
-    ``positions`` (tokens,) int32 or int64; ``key`` may be None.  Returns
+    ``positions`` (tokens,) int32 or int64, of less than 2^49 turns; ``key``
+    may be None.  Returns
     (query, key), new tensors unless ``query_out`` / ``key_out`` are given,
     which may be the inputs themselves.  ``inverse`` turns by the opposite
     angles (the factor of a yarn rotation multiplies either way).
