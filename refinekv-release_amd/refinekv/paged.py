@@ -39,8 +39,8 @@ class PagedCache:
     (sequences, max_blocks) int32, the page of each page_size tokens; entries
     past a sequence's length are not read.  ``lengths``: (sequences,) int32,
     the visible tokens, those being appended included; 0 marks an idle place.
-    The tensors' contents may change, and where they lie; their sizes and
-    strides are read once.
+    The tensors' contents may change; their sizes, strides and alignment are
+    read once.
     """
 
     keys: torch.Tensor
