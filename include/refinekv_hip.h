@@ -328,6 +328,84 @@ int rkv_paged_decode(const rkv_paged_cache* cache, const void* query, int64_t q_
                      int64_t q_head_stride, int64_t group, float scale, void* output,
                      void* workspace, size_t workspace_bytes, rkv_stream_t stream);
 
+/* The dense (tokens, heads, dim) keys and values of the sequences' last tokens,
+ * as rkv_paged_append with the same token_starts stored them.  Zeros for a row
+ * of no sequence or without a position, NaN for one whose page is outside the
+ * cache.  The rows lie apart from each other and from the cache. */
+int rkv_paged_read(const rkv_paged_cache* cache, int64_t tokens, const int32_t* token_starts,
+                   void* key_out, void* value_out, rkv_stream_t stream);
+
+/* What an attention's scores are besides scaled products x = scale q . k, in
+ * this order; NULL, or all fields 0, for nothing:
+ *   softcap > 0:  softcap * tanh(x / softcap);
+ *   slopes:       fp32 per query head (device, 4-byte aligned), x - slope *
+ *                 |position of q - position of k|;
+ *   window > 0:   a query sees the last `window` tokens up to its own. */
+typedef struct {
+  float softcap;
+  const float* slopes;
+  int64_t window;
+} rkv_scores;
+
+/* rkv_paged_decode with such scores.  Pages that hold only tokens before the
+ * window are not read, and their table entries may be anything. */
+int rkv_paged_decode_scores(const rkv_paged_cache* cache, const void* query,
+                            int64_t q_sequence_stride, int64_t q_head_stride, int64_t group,
+                            float scale, const rkv_scores* scores, void* output, void* workspace,
+                            size_t workspace_bytes, rkv_stream_t stream);
+
+/*
+ * A paged cache in 4 bits (no counterpart in the reference).  Every 32 dims of
+ * a row have an fp16 zero z = min and scale s = (max - min) / 15 rounded up to
+ * 7 significant bits, and codes c = round((x - z) / s) in 0..15 that stand for
+ * z + s c; a group with a value that is not finite, or past 4096 in magnitude,
+ * stands for NaN.  The four arrays are dense over (pages, heads, page_size),
+ * 16-byte aligned and share no memory:
+ *   key_codes, value_codes:    dim / 2 bytes a row;
+ *   key_scales, value_scales:  dim / 32 pairs of fp16 a row,
+ * in the kernels' own order within 4 rows (csrc/rkv_quantized.hip's head):
+ * written by rkv_quantized_append, read by rkv_quantized_read.  dtype: RKV_BF16
+ * or RKV_F16, of the rows and queries; dim 32..256 in steps of 32.  The other
+ * fields as rkv_paged_cache's.
+ */
+typedef struct {
+  void* key_codes;
+  void* key_scales;
+  void* value_codes;
+  void* value_scales;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  int64_t pages, heads, page_size, dim, sequences, max_blocks;
+  int dtype;
+} rkv_quantized_cache;
+
+/* rkv_paged_append to a cache in 4 bits: keys are turned, rounded to the rows'
+ * type, then coded.  Rows and query_out are 16-byte aligned with strides in
+ * multiples of 8 and lie outside the cache; query_out is apart from the query. */
+int rkv_quantized_append(const rkv_quantized_cache* cache, const void* query,
+                         int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads,
+                         void* query_out, int64_t qo_token_stride, int64_t qo_head_stride,
+                         const void* key, int64_t k_token_stride, int64_t k_head_stride,
+                         const void* value, int64_t v_token_stride, int64_t v_head_stride,
+                         int64_t tokens, const int32_t* token_starts, const double* rates,
+                         int64_t rotary_dim, int interleaved, float scale, rkv_stream_t stream);
+
+/* The dense (tokens, heads, dim) keys and values that the sequences' last
+ * tokens stand for, rounded to the rows' type; tokens and token_starts as the
+ * append's.  Zeros for a row of no sequence or without a position, NaN for one
+ * whose page is outside the cache. */
+int rkv_quantized_read(const rkv_quantized_cache* cache, int64_t tokens,
+                       const int32_t* token_starts, void* key_out, void* value_out,
+                       rkv_stream_t stream);
+
+/* rkv_paged_decode_scores over a cache in 4 bits, and its workspace. */
+int rkv_quantized_decode(const rkv_quantized_cache* cache, const void* query,
+                         int64_t q_sequence_stride, int64_t q_head_stride, int64_t group,
+                         float scale, const rkv_scores* scores, void* output, void* workspace,
+                         size_t workspace_bytes, rkv_stream_t stream);
+int rkv_quantized_plan(const rkv_quantized_cache* cache, int64_t group, size_t* workspace_bytes);
+
 /* Workspace bytes of rkv_paged_decode for this cache on the current device. */
 int rkv_paged_plan(const rkv_paged_cache* cache, int64_t group, size_t* workspace_bytes);
 

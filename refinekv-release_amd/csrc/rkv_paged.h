@@ -114,4 +114,24 @@ inline bool rows_meet_pages(const rkv_paged_cache* c, const void* rows, int64_t 
          meets(c->values, c->value_page_stride, c->value_head_stride, c->value_token_stride);
 }
 
+// Whether a call's scores are more than scaled products.
+inline bool scores_any(const rkv_scores* s) {
+  return s && (s->softcap > 0.0f || s->slopes || s->window > 0);
+}
+
+// Tokens that a query sees up to its own (all: 2^31 - 1).
+inline int scores_window(const rkv_scores* s) {
+  const int64_t all = (int64_t(1) << 31) - 1;
+  return (int)(s && s->window > 0 && s->window < all ? s->window : all);
+}
+
+inline int check_scores(const char* who, const rkv_scores* s) {
+  if (!s) return kOk;
+  if (!(s->softcap >= 0.0f) || s->softcap > 3.0e38f)
+    return set_error(kInvalidArgument, "%s: softcap must be finite, and 0 for none", who);
+  if (s->window < 0) return set_error(kInvalidArgument, "%s: negative window", who);
+  if (!aligned(s->slopes, 4)) return set_error(kInvalidArgument, "%s: unaligned slopes", who);
+  return kOk;
+}
+
 }  // namespace rkv

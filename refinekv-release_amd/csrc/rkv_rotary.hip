@@ -13,6 +13,7 @@
 #include "rkv_common.h"
 #include "rkv_internal.h"
 #include "rkv_paged.h"
+#include "rkv_places.h"
 
 namespace rkv {
 namespace {
@@ -46,100 +47,23 @@ struct Rows {
   int paged;                 // dst is the cache's pages (keys and values alike)
 };
 
-struct RotaryArgs {
+struct RotaryArgs : Places {
   Rows rows[3];              // queries, keys, values (heads 0: absent)
   int heads;                 // all of them
   int64_t tokens;
   int dim, rotary_dim;
-  const void* positions;     // int32 or int64 per token (null: from the sequences)
-  int wide_positions;
   const double* rates;       // turns per position of each pair, rotary_dim / 2
   float scale, sign;         // attention factor; -1 turns back
-  // paged: token t belongs to the sequence b with starts[b] <= t < starts[b + 1]
-  // (null: sequence t), at position lengths[b] - (starts[b + 1] - t)
-  const int32_t* starts;
-  const int32_t* lengths;
-  const int32_t* table;
-  int64_t table_stride;
-  int sequences, max_blocks, pages, shift;
   int items, turning;        // items of a head's row; those that turn come first
   int step, gap;             // dims from one turning item to the next, of an item's two vectors
   int slots, per_block;      // heads that a token's threads hold at a time, a workgroup's tokens
 };
-
-// cos and sin of `quarters` quarter turns, to an ulp or two of fp32.  The
-// angle of a far position needs more than fp32's 24 bits (131071 * 1 rad has
-// an ulp of 0.008 rad there), so the whole quarters are taken off in fp64:
-// adding 1.5 * 2^52 leaves them in the sum's low bits, rounded to nearest.
-// What is left, at most pi/4, goes through the Taylor series of sin (to a^9,
-// truncation 2e-9) and cos (to a^10, 2e-10).
-__device__ __forceinline__ void cos_sin(double quarters, float& c, float& s) {
-  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52
-  const double sum = quarters + kWhole;
-  const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, sum);
-  const float a = (float)(quarters - (sum - kWhole)) * 1.57079632679489662f;
-  const float a2 = a * a;
-  float p = 2.75573192239858907e-06f;                    // 1/9!
-  p = __builtin_fmaf(p, a2, -1.98412698412698413e-04f);  // 1/7!
-  p = __builtin_fmaf(p, a2, 8.33333333333333333e-03f);   // 1/5!
-  p = __builtin_fmaf(p, a2, -1.66666666666666667e-01f);  // 1/3!
-  const float sn = __builtin_fmaf(p * a2, a, a);
-  float q = -2.75573192239858907e-07f;                   // 1/10!
-  q = __builtin_fmaf(q, a2, 2.48015873015873016e-05f);   // 1/8!
-  q = __builtin_fmaf(q, a2, -1.38888888888888889e-03f);  // 1/6!
-  q = __builtin_fmaf(q, a2, 4.16666666666666667e-02f);   // 1/4!
-  q = __builtin_fmaf(q, a2, -0.5f);
-  const float cn = __builtin_fmaf(q, a2, 1.0f);
-  // quarter 0 (c, s), 1 (-s, c), 2 (-c, -s), 3 (s, -c)
-  const bool swap = (k & 1u) != 0u;
-  c = bits_f32(f32_bits(swap ? sn : cn) ^ ((k + 1u) << 30 & 0x80000000u));
-  s = bits_f32(f32_bits(swap ? cn : sn) ^ (k << 30 & 0x80000000u));
-}
 
 // One of three values, chosen as values: a choice between variables would be
 // one of addresses, and put them in scratch.
 template <typename T>
 __device__ __forceinline__ T pick(bool q, bool v, T of_query, T of_key, T of_value) {
   return q ? of_query : v ? of_value : of_key;
-}
-
-// Where a token's rows go: its position, and its page and row in a cache
-// (page < 0: not in the cache).
-struct Place {
-  int64_t position;
-  int page, row;
-  bool live;  // has a position: its rows turn
-};
-
-__device__ __forceinline__ Place place_of(const RotaryArgs& a, int64_t t) {
-  Place p{0, -1, 0, true};
-  if (a.positions) {
-    p.position = a.wide_positions ? static_cast<const int64_t*>(a.positions)[t]
-                                  : static_cast<const int32_t*>(a.positions)[t];
-    return p;
-  }
-  int64_t b = t, behind = 1;  // tokens of the sequence from this one on
-  if (a.starts) {
-    // the first sequence that ends after t (empty ones end where they start)
-    int lo = 0, hi = a.sequences;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (a.starts[mid + 1] <= t) lo = mid + 1;
-      else hi = mid;
-    }
-    b = lo;
-    if (b >= a.sequences || a.starts[b] > t) return Place{0, -1, 0, false};
-    behind = a.starts[b + 1] - t;
-  }
-  p.position = (int64_t)a.lengths[b] - behind;
-  if (p.position < 0) return Place{0, -1, 0, false};
-  const int64_t block = p.position >> a.shift;
-  if (block < a.max_blocks) {
-    const int page = a.table[b * a.table_stride + block];
-    p.page = page >= 0 && page < a.pages ? page : -1;
-  }
-  p.row = (int)(p.position & ((1 << a.shift) - 1));
-  return p;
 }
 
 // A thread holds one item of a row, two vectors of W dims: in the half layout
@@ -331,6 +255,54 @@ int launch(RotaryArgs& a, int dtype, bool interleaved, hipStream_t stream) {
   return launch_t<float>(a, interleaved, stream);
 }
 
+// Rows of a cache's pages copied out, `bytes` of a vector at a time.
+struct ReadArgs : Places {
+  const char* src[2];           // keys, values
+  char* dst[2];                 // (tokens, heads, dim) dense
+  int64_t ps[2], hs[2], ts[2];  // page, head and row strides of src, bytes
+  int64_t tokens;
+  int heads, row_bytes, dtype;
+};
+
+template <typename V>
+__global__ __launch_bounds__(kThreads) void paged_read_kernel(ReadArgs a) {
+  const int items = a.row_bytes / (int)sizeof(V), each = 2 * a.heads * items;
+  const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t t = id / each;
+  if (t >= a.tokens) return;
+  const int rest = (int)(id % each);
+  const int item = rest % items, h = rest / items % a.heads, k = rest / items / a.heads;
+  const Place p = place_of(a, t);
+  V v{};
+  if (p.page >= 0) {
+    v = *reinterpret_cast<const V*>((k ? a.src[1] : a.src[0]) +
+                                    p.page * (k ? a.ps[1] : a.ps[0]) +
+                                    h * (k ? a.hs[1] : a.hs[0]) +
+                                    p.row * (k ? a.ts[1] : a.ts[0]) + item * sizeof(V));
+  } else if (p.live) {
+    // NaN of the type, in every element of the vector
+    const uint32_t nan = a.dtype == RKV_F32    ? 0x7fc00000u
+                         : a.dtype == RKV_BF16 ? 0x7fc07fc0u
+                                               : 0x7e007e00u;
+    __builtin_memcpy(&v, &nan, sizeof(V) < 4 ? sizeof(V) : 4);
+    if constexpr (sizeof(V) > 4)
+      for (size_t i = 4; i < sizeof(V); i += 4)
+        __builtin_memcpy(reinterpret_cast<char*>(&v) + i, &nan, 4);
+  }
+  *reinterpret_cast<V*>((k ? a.dst[1] : a.dst[0]) + (t * a.heads + h) * a.row_bytes +
+                        item * (int64_t)sizeof(V)) = v;
+}
+
+template <typename V>
+int launch_read(const ReadArgs& a, hipStream_t stream) {
+  const int64_t each = 2 * (int64_t)a.heads * (a.row_bytes / (int)sizeof(V));
+  if (a.tokens > INT64_MAX / each || (a.tokens * each + kThreads - 1) / kThreads > 0x7fffffff)
+    return set_error(kInvalidArgument, "rkv_paged_read: too many tokens");
+  const int64_t blocks = (a.tokens * each + kThreads - 1) / kThreads;
+  paged_read_kernel<V><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
+  return check_launch("paged_read_kernel");
+}
+
 int check_table(const char* who, const double* rates, int64_t rotary_dim, int64_t dim) {
   if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > dim || (rotary_dim > 0 && !rates))
     return set_error(kInvalidArgument, "%s: rotary_dim %lld must be even, at most head_dim %lld, "
@@ -454,4 +426,57 @@ extern "C" int rkv_paged_append(const rkv_paged_cache* cache, const void* query,
   a.pages = (int)cache->pages;
   a.shift = page_shift(cache->page_size);
   return launch(a, cache->dtype, interleaved != 0, stream);
+}
+
+extern "C" int rkv_paged_read(const rkv_paged_cache* cache, int64_t tokens,
+                              const int32_t* token_starts, void* key_out, void* value_out,
+                              hipStream_t stream) {
+  const char* who = "rkv_paged_read";
+  clear_error();
+  const int rc = check_cache(who, cache);
+  if (rc) return rc;
+  if (tokens < 0 || (!token_starts && tokens != cache->sequences))
+    return set_error(kInvalidArgument, "%s: without token_starts one token per sequence", who);
+  if (tokens == 0) return kOk;
+  if (!key_out || !value_out) return set_error(kInvalidArgument, "%s: null pointer argument", who);
+  const int64_t size = dtype_bytes(cache->dtype), row = cache->heads * cache->dim;
+  if (!aligned(key_out, size) || !aligned(value_out, size))
+    return set_error(kInvalidArgument, "%s: rows not aligned to their type", who);
+  const uint64_t k0 = reinterpret_cast<uint64_t>(key_out), v0 = reinterpret_cast<uint64_t>(value_out);
+  const uint64_t bytes = (uint64_t)(tokens * row * size);
+  if (rows_meet_pages(cache, key_out, row, cache->dim, tokens, cache->heads) ||
+      rows_meet_pages(cache, value_out, row, cache->dim, tokens, cache->heads) ||
+      (k0 < v0 + bytes && v0 < k0 + bytes))
+    return set_error(kInvalidArgument, "%s: the rows overlap each other or the cache", who);
+  ReadArgs a{};
+  a.src[0] = static_cast<const char*>(cache->keys);
+  a.src[1] = static_cast<const char*>(cache->values);
+  a.dst[0] = static_cast<char*>(key_out);
+  a.dst[1] = static_cast<char*>(value_out);
+  a.ps[0] = read_stride(cache->key_page_stride, cache->pages) * size;
+  a.ps[1] = read_stride(cache->value_page_stride, cache->pages) * size;
+  a.hs[0] = read_stride(cache->key_head_stride, cache->heads) * size;
+  a.hs[1] = read_stride(cache->value_head_stride, cache->heads) * size;
+  a.ts[0] = cache->key_token_stride * size;
+  a.ts[1] = cache->value_token_stride * size;
+  a.tokens = tokens;
+  a.heads = (int)cache->heads;
+  a.row_bytes = (int)(cache->dim * size);
+  a.dtype = cache->dtype;
+  a.starts = token_starts;
+  a.lengths = cache->lengths;
+  a.table = cache->block_table;
+  a.table_stride = cache->table_stride;
+  a.sequences = (int)cache->sequences;
+  a.max_blocks = (int)cache->max_blocks;
+  a.pages = (int)cache->pages;
+  a.shift = page_shift(cache->page_size);
+  // the widest vector that every row's address allows
+  int64_t all = a.row_bytes;
+  for (int i = 0; i < 2; ++i)
+    all |= (int64_t)reinterpret_cast<uint64_t>(a.src[i]) | (int64_t)reinterpret_cast<uint64_t>(a.dst[i]) |
+           a.ps[i] | a.hs[i] | a.ts[i];
+  if (all % 16 == 0) return launch_read<uint4>(a, stream);
+  if (all % 4 == 0) return launch_read<uint32_t>(a, stream);
+  return launch_read<uint16_t>(a, stream);
 }

@@ -6,7 +6,8 @@ Same public API as the reference package (src/refinekv/__init__.py:3-25);
 
 from .attention import AttentionResult, select_blocks, select_blocks_union, sparse_attention
 from .config import RefineKVConfig
-from .paged import PagedCache, paged_append, paged_decode
+from .paged import PagedCache, paged_append, paged_decode, paged_read
+from .quantized import QuantizedCache
 from .rotary import Rotary, RotaryConfig, rotate_heads
 from .summary import BlockSummary, build_summary
 
@@ -15,12 +16,14 @@ __all__ = [
     "AttentionResult",
     "BlockSummary",
     "PagedCache",
+    "QuantizedCache",
     "RefineKVConfig",
     "Rotary",
     "RotaryConfig",
     "build_summary",
     "paged_append",
     "paged_decode",
+    "paged_read",
     "rotate_heads",
     "select_blocks",
     "select_blocks_union",

@@ -51,6 +51,19 @@ class _PagedCache(ctypes.Structure):
                 ("dim", _i64), ("sequences", _i64), ("max_blocks", _i64), ("dtype", _int)]
 
 
+class _QuantizedCache(ctypes.Structure):
+    """rkv_quantized_cache."""
+    _fields_ = [("key_codes", _p), ("key_scales", _p), ("value_codes", _p), ("value_scales", _p),
+                ("block_table", _p), ("table_stride", _i64), ("lengths", _p), ("pages", _i64),
+                ("heads", _i64), ("page_size", _i64), ("dim", _i64), ("sequences", _i64),
+                ("max_blocks", _i64), ("dtype", _int)]
+
+
+class _Scores(ctypes.Structure):
+    """rkv_scores."""
+    _fields_ = [("softcap", _f32), ("slopes", _p), ("window", _i64)]
+
+
 def _bind(lib):
     lib.rkv_last_error.restype = ctypes.c_char_p
     lib.rkv_version.restype = _int
@@ -117,6 +130,18 @@ def _bind(lib):
     lib.rkv_paged_decode.restype = _int
     lib.rkv_paged_plan.argtypes = [_p, _i64, _p]
     lib.rkv_paged_plan.restype = _int
+    lib.rkv_paged_decode_scores.argtypes = [_p, _p, _i64, _i64, _i64, _f32, _p, _p, _p, _size, _p]
+    lib.rkv_paged_decode_scores.restype = _int
+    lib.rkv_paged_read.argtypes = [_p, _i64, _p, _p, _p, _p]
+    lib.rkv_paged_read.restype = _int
+    lib.rkv_quantized_append.argtypes = lib.rkv_paged_append.argtypes
+    lib.rkv_quantized_append.restype = _int
+    lib.rkv_quantized_read.argtypes = lib.rkv_paged_read.argtypes
+    lib.rkv_quantized_read.restype = _int
+    lib.rkv_quantized_decode.argtypes = lib.rkv_paged_decode_scores.argtypes
+    lib.rkv_quantized_decode.restype = _int
+    lib.rkv_quantized_plan.argtypes = [_p, _i64, _p]
+    lib.rkv_quantized_plan.restype = _int
     return lib
 
 
@@ -602,10 +627,16 @@ MAX_HEAD_STRIDE = 1 << 25  # of rkv_paged_decode's query, elements
 
 
 def _cache_struct(cache):
-    """The C view of a PagedCache (made on its first call; the pointers are
+    """The C view of a PagedCache or QuantizedCache (made on its first call; the pointers are
     taken from the tensors on every call) and a reference to it."""
     made = cache.__dict__.get("_hip_view")
-    if made is None:
+    if made is None and not hasattr(cache, "keys"):
+        view = _QuantizedCache(
+            table_stride=cache.block_table.stride(0), pages=cache.pages, heads=cache.heads,
+            page_size=cache.page_size, dim=cache.head_dim, sequences=cache.sequences,
+            max_blocks=cache.max_blocks, dtype=DTYPE_CODES[cache.dtype])
+        made = cache.__dict__["_hip_view"] = (view, ctypes.byref(view))
+    elif made is None:
         view = _PagedCache(
             key_strides=(_i64 * 3)(*cache.keys.stride()[:3]),
             value_strides=(_i64 * 3)(*cache.values.stride()[:3]),
@@ -614,7 +645,12 @@ def _cache_struct(cache):
             max_blocks=cache.max_blocks, dtype=DTYPE_CODES[cache.dtype])
         made = cache.__dict__["_hip_view"] = (view, ctypes.byref(view))
     view = made[0]
-    view.keys, view.values = cache.keys.data_ptr(), cache.values.data_ptr()
+    if type(view) is _QuantizedCache:
+        view.key_codes, view.value_codes = cache.key_codes.data_ptr(), cache.value_codes.data_ptr()
+        view.key_scales = cache.key_scales.data_ptr()
+        view.value_scales = cache.value_scales.data_ptr()
+    else:
+        view.keys, view.values = cache.keys.data_ptr(), cache.values.data_ptr()
     view.block_table, view.lengths = cache.block_table.data_ptr(), cache.lengths.data_ptr()
     return made[1]
 
@@ -647,23 +683,87 @@ def paged_append(key, value, cache, query=None, table=None, token_starts=None, q
     return query_out
 
 
+def quantized_append(key, value, cache, query=None, table=None, token_starts=None,
+                     query_out=None):
+    """rkv_quantized_append on checked rows; returns the turned query or None."""
+    device = cache.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return quantized_append(key, value, cache, query, table, token_starts, query_out)
+    key, value = _row_aligned(key, 16), _row_aligned(value, 16)
+    rows, target = (0, 0, 0, 0, 0, 0, 0), query_out
+    if query is not None:
+        query = _row_aligned(query, 16)
+        # (the kernel writes whole vectors, and not over the query)
+        if query_out is None or not _takes_rows(query_out) or _spans_meet(query, query_out):
+            target = _like(query)
+        rows = (*_rows(query), query.shape[1], *_rows(target))
+    turns = (0, 0, 0, 1.0) if table is None else (
+        table.turns.data_ptr(), table.config.rotary_dim, table.config.interleaved, table.scale)
+    rc = lib().rkv_quantized_append(
+        _cache_struct(cache), *rows, *_rows(key), *_rows(value), key.shape[0],
+        0 if token_starts is None else token_starts.data_ptr(), *turns, _raw_stream(device))
+    if rc:
+        _check(rc, "rkv_quantized_append")
+    return target if query_out is None or target is query_out else query_out.copy_(target)
+
+
+def _takes_rows(t):
+    """Whether a kernel can store whole vectors to (tokens, heads, dim) rows."""
+    return t.data_ptr() % 16 == 0 and all(s * t.element_size() % 16 == 0 for s in t.stride()[:2])
+
+
+def _spans_meet(a, b):
+    first, end = ([t.data_ptr() for t in (a, b)], [
+        t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(
+            t.shape, t.stride()))) for t in (a, b)])
+    return a.numel() > 0 and first[0] < end[1] and first[1] < end[0]
+
+
+def paged_read(cache, tokens, token_starts, quantized):
+    """rkv_paged_read or rkv_quantized_read: (keys, values) rows."""
+    device = cache.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return paged_read(cache, tokens, token_starts, quantized)
+    keys, values = (torch.empty((tokens, cache.heads, cache.head_dim), dtype=cache.dtype,
+                                device=device) for _ in range(2))
+    read = lib().rkv_quantized_read if quantized else lib().rkv_paged_read
+    rc = read(_cache_struct(cache), tokens,
+              0 if token_starts is None else token_starts.data_ptr(), keys.data_ptr(),
+              values.data_ptr(), _raw_stream(device))
+    if rc:
+        _check(rc, "rkv_quantized_read" if quantized else "rkv_paged_read")
+    return keys, values
+
+
+def _scores(scores):
+    """A reference to the C view of a call's scores (0: products alone)."""
+    if scores is None:
+        return 0
+    return ctypes.byref(_Scores(
+        softcap=scores.softcap, window=scores.window,
+        slopes=0 if scores.slopes is None else scores.slopes.data_ptr()))
+
+
 def _paged_bytes(cache, group):
     """Workspace bytes of paged_decode on the current device."""
     sizes = cache.__dict__.setdefault("_hip_sizes", {})
     if group not in sizes:
         nbytes = _size()
-        _check(lib().rkv_paged_plan(_cache_struct(cache), group, ctypes.byref(nbytes)),
-               "rkv_paged_plan")
+        plan = lib().rkv_paged_plan if hasattr(cache, "keys") else lib().rkv_quantized_plan
+        _check(plan(_cache_struct(cache), group, ctypes.byref(nbytes)), "rkv_paged_plan")
         sizes[group] = nbytes.value
     return sizes[group]
 
 
-def paged_decode(query, cache, scaling, workspace=None, output=None):
-    """rkv_paged_decode on a checked (sequences, q_heads, dim) query."""
+def paged_decode(query, cache, scaling, workspace=None, output=None, scores=None):
+    """rkv_paged_decode, rkv_paged_decode_scores or rkv_quantized_decode on a
+    checked (sequences, q_heads, dim) query."""
     device = cache.device
     if _elsewhere(device):
         with torch.cuda.device(device):
-            return paged_decode(query, cache, scaling, workspace, output)
+            return paged_decode(query, cache, scaling, workspace, output, scores)
     group = query.shape[1] // cache.heads
     query = _row_aligned(query, 16)
     if query.stride(1) > MAX_HEAD_STRIDE:
@@ -675,9 +775,15 @@ def paged_decode(query, cache, scaling, workspace=None, output=None):
     # the one it was captured with)
     scratch = _buffer(workspace, ("hip_paged_scratch", nbytes, device.index), (nbytes,), device,
                       torch.uint8)
-    rc = lib().rkv_paged_decode(_cache_struct(cache), *_rows(query), group, scaling,
-                                output.data_ptr(), scratch.data_ptr(), nbytes,
-                                _raw_stream(device))
+    if scores is None and hasattr(cache, "keys"):
+        rc = lib().rkv_paged_decode(_cache_struct(cache), *_rows(query), group, scaling,
+                                    output.data_ptr(), scratch.data_ptr(), nbytes,
+                                    _raw_stream(device))
+    else:
+        decode = (lib().rkv_paged_decode_scores if hasattr(cache, "keys")
+                  else lib().rkv_quantized_decode)
+        rc = decode(_cache_struct(cache), *_rows(query), group, scaling, _scores(scores),
+                    output.data_ptr(), scratch.data_ptr(), nbytes, _raw_stream(device))
     if rc:
         _check(rc, "rkv_paged_decode")
     return output

@@ -3,9 +3,10 @@
 The reference's caches hold one sequence, contiguous; a server that decodes
 many at once keeps their tokens in pages of one allocation.  ``PagedCache``
 describes such a cache (the tensors are the caller's, and so is the
-allocation of pages), ``paged_append`` writes new keys and values to it,
-turned to their positions on the way, and ``paged_decode`` attends one new
-token per sequence over its visible tokens.  A decode step::
+allocation of pages; ``QuantizedCache`` holds the same in 4 bits),
+``paged_append`` writes new keys and values to it, turned to their positions
+on the way, ``paged_read`` gives rows back, and ``paged_decode`` attends one
+new token per sequence over its visible tokens.  A decode step::
 
     cache.lengths.add_(1)                 # the new token counts as visible
     query = paged_append(key, value, cache, query=query, rotary=rotary)
@@ -19,13 +20,14 @@ Inference only, as the whole package: the results carry no gradient.
 """
 
 from dataclasses import dataclass, field
+import math
 
 import torch
 
 from . import _hip
+from .quantized import PAGE_SIZES, QuantizedCache
 from .rotary import DTYPES, check_out, overlaps_itself, pick_backend, rows_overlap
 
-PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_ROW_STRIDE = 1 << 25  # elements between a page's rows, at most
 
 
@@ -150,6 +152,13 @@ def _keys_meet_values(cache):
     return meet(0, cache.values.data_ptr() - cache.keys.data_ptr())
 
 
+def _parts(cache):
+    """The tensors that hold a cache's tokens."""
+    if isinstance(cache, QuantizedCache):
+        return cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales
+    return cache.keys, cache.values
+
+
 def _meet_pages(rows, cache):
     """Whether (tokens, heads, head_dim) rows may lie among the cache's pages,
     by the C entries' rule: their spans meet."""
@@ -160,7 +169,7 @@ def _meet_pages(rows, cache):
     if rows.numel() == 0:
         return False
     first, end = span(rows)
-    return any(first < e and f < end for f, e in map(span, (cache.keys, cache.values)))
+    return any(first < e and f < end for f, e in map(span, _parts(cache)))
 
 
 def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=None,
@@ -181,7 +190,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     stored.  No two rows of a call may fall on the same place: a page written
     here belongs to one sequence, and a cache whose keys and values share
     memory is refused.  Rows that are views of the cache's pages are copied
-    first: the call stores what they hold before it.
+    first: the call stores what they hold before it.  To a ``QuantizedCache``
+    the rows go in 4 bits, keys turned and rounded to their type before.
 
     (A prompt's own attention needs its turned keys as well: turn both with
     rotate_heads, then append without ``rotary``.)
@@ -189,13 +199,7 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     tokens, device = key.shape[0] if key.ndim else 0, cache.device
     _check_rows("key", key, cache, tokens, cache.heads)
     _check_rows("value", value, cache, tokens, cache.heads)
-    if token_starts is not None:
-        if (token_starts.shape != (cache.sequences + 1,) or token_starts.dtype != torch.int32
-                or token_starts.device != device or not token_starts.is_contiguous()):
-            raise ValueError("token_starts must be contiguous int32 with shape (sequences + 1,) "
-                             "on the cache's device")
-    elif tokens != cache.sequences:
-        raise ValueError("without token_starts there is one token per sequence")
+    _check_starts(token_starts, cache, tokens)
     if rotary is not None and (rotary.config.head_dim != cache.head_dim
                                or rotary.device != device):
         raise ValueError("rotary must have the cache's head_dim and device")
@@ -207,20 +211,83 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
             check_out("query_out", query_out, query, (key, value))
     elif query_out is not None:
         raise ValueError("query_out without a query")
+    quantized = isinstance(cache, QuantizedCache)
     why = None if key.dtype in DTYPES else "the HIP append needs a bf16, fp16 or fp32 cache"
     if pick_backend(key, backend, why is None, why) == "hip":
-        return _hip.paged_append(key, value, cache, query, rotary, token_starts, query_out)
+        hip = _hip.quantized_append if quantized else _hip.paged_append
+        return hip(key, value, cache, query, rotary, token_starts, query_out)
     from .reference_paged import append
 
     _check_capture(key, why or "backend='torch'")
 
-    if _keys_meet_values(cache):
+    if not quantized and _keys_meet_values(cache):
         raise ValueError("the cache's keys and values share memory")
     if query_out is not None and _meet_pages(query_out, cache):
         raise ValueError("query_out overlaps the cache")
     with torch.no_grad():
         turned = append(cache, key, value, query, rotary, token_starts)
         return turned if query_out is None else query_out.copy_(turned)
+
+
+def _check_starts(token_starts, cache, tokens):
+    if token_starts is not None:
+        if (token_starts.shape != (cache.sequences + 1,) or token_starts.dtype != torch.int32
+                or token_starts.device != cache.device or not token_starts.is_contiguous()):
+            raise ValueError("token_starts must be contiguous int32 with shape (sequences + 1,) "
+                             "on the cache's device")
+    elif tokens != cache.sequences:
+        raise ValueError("without token_starts there is one token per sequence")
+
+
+def paged_read(cache, tokens, *, token_starts=None, backend="auto"):
+    """The keys and values of the sequences' last tokens, as new dense
+    (tokens, kv_heads, head_dim) rows of the cache's dtype: what ``paged_append``
+    with the same ``token_starts`` has stored.
+
+    With ``token_starts`` (sequences + 1,) int32, rows token_starts[b] up to
+    token_starts[b + 1] are sequence b's last tokens, ending at position
+    lengths[b] - 1; without it every sequence has one.  Rows of no sequence or
+    without a position are zeros; a row whose page is outside the cache, or past
+    the block table, is NaN.
+    """
+    if not isinstance(tokens, int) or isinstance(tokens, bool) or tokens < 0:
+        raise ValueError("tokens must be an integer of at least 0")
+    _check_starts(token_starts, cache, tokens)
+    quantized = isinstance(cache, QuantizedCache)
+    why = None if cache.dtype in DTYPES else "the HIP read needs a bf16, fp16 or fp32 cache"
+    if pick_backend(cache.lengths, backend, why is None, why) == "hip":
+        return _hip.paged_read(cache, tokens, token_starts, quantized)
+    from .reference_paged import read
+
+    _check_capture(cache.lengths, why or "backend='torch'")
+    with torch.no_grad():
+        return read(cache, tokens, token_starts)
+
+
+@dataclass(frozen=True)
+class Scores:
+    """What scores are besides scaled products (None, or 0: nothing)."""
+
+    softcap: float = 0.0
+    slopes: torch.Tensor | None = None
+    window: int = 0
+
+
+def check_scores(softcap, slopes, window, q_heads, device):
+    """The checked options of a call, or None where they ask for nothing."""
+    if softcap is None and slopes is None and window is None:
+        return None
+    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
+        raise ValueError("softcap must be finite and positive")
+    if window is not None and (not isinstance(window, int) or isinstance(window, bool)
+                               or window <= 0):
+        raise ValueError("window must be a positive integer")
+    if slopes is not None:
+        if slopes.shape != (q_heads,) or slopes.dtype != torch.float32:
+            raise ValueError("slopes must be float32 with shape (q_heads,)")
+        if slopes.device != device or not slopes.is_contiguous():
+            raise ValueError("slopes must be contiguous on the query's device")
+    return Scores(0.0 if softcap is None else float(softcap), slopes, window or 0)
 
 
 def _decode_support(cache, group):
@@ -234,6 +301,12 @@ def _decode_support(cache, group):
 
 def _why_not(cache, group):
     dim = cache.head_dim
+    if isinstance(cache, QuantizedCache):
+        if group > _hip.MAX_GROUP:
+            return "the HIP paged decode needs group <= 16"
+        if cache.sequences * cache.heads * (cache.capacity // 32 + 1) >= 2 ** 31:
+            return "the HIP paged decode needs a block table of fewer tokens"
+        return None
     if cache.dtype not in (torch.bfloat16, torch.float16):
         return "the HIP paged decode needs a bf16 or fp16 cache"
     if dim not in _hip.SUPPORTED_DIMS or group > _hip.MAX_GROUP:
@@ -248,7 +321,8 @@ def _why_not(cache, group):
     return None
 
 
-def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, backend="auto"):
+def paged_decode(query, cache, *, scaling=None, softcap=None, slopes=None, window=None,
+                 workspace=None, output=None, backend="auto"):
     """Attention of one new token per sequence over its visible tokens.
 
     ``query`` (sequences, q_heads, head_dim), q_heads a multiple of the
@@ -257,6 +331,12 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
     (apart from the query and the cache).
     ``workspace`` (a dict) keeps the partial results' buffer from call to
     call; calls that share one must be ordered on one stream.
+
+    A score is the scaled product of query and key; ``softcap`` makes it
+    softcap * tanh(score / softcap), then ``slopes`` (q_heads,) float32 take
+    slope * (distance of the token from the newest) off, and of ``window``
+    tokens, the newest among them, the query sees no others: pages that hold
+    none of them may be gone (their table entries are not read as pages).
 
     A sequence of length 0 gives zeros; one with a page outside the cache
     among its visible ones, or a length past its table, gives NaN.
@@ -272,10 +352,11 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
         if rows_overlap(output, query):
             raise ValueError("output must not overlap the query")
     scaling = cache.head_dim ** -0.5 if scaling is None else float(scaling)
+    scores = check_scores(softcap, slopes, window, query.shape[1], query.device)
     why = _decode_support(cache, group) if query.is_cuda else None
     hip = pick_backend(query, backend, why is None, why) == "hip"
     if hip and (output is None or output.data_ptr() % 16 == 0):
-        return _hip.paged_decode(query, cache, scaling, workspace, output)
+        return _hip.paged_decode(query, cache, scaling, workspace, output, scores)
     if not hip:
         _check_capture(query, why or "backend='torch'")
     from .reference_paged import decode
@@ -283,7 +364,7 @@ def paged_decode(query, cache, *, scaling=None, workspace=None, output=None, bac
     if output is not None and _meet_pages(output, cache):
         raise ValueError("output overlaps the cache")
     if hip:  # (the kernel stores whole vectors)
-        return output.copy_(_hip.paged_decode(query, cache, scaling, workspace))
+        return output.copy_(_hip.paged_decode(query, cache, scaling, workspace, None, scores))
     with torch.no_grad():
-        out = decode(query, cache, scaling)
+        out = decode(query, cache, scaling, scores)
         return out if output is None else output.copy_(out)

@@ -7,6 +7,9 @@ import math
 
 import torch
 
+from . import quantized
+from .quantized import QuantizedCache
+
 
 def _wide(x):
     return x if x.dtype == torch.float64 else x.float()
@@ -32,10 +35,11 @@ def rotate(x, positions, rotary, inverse=False, live=None):
     return y if live is None else torch.where(live[:, None, None], y, x)
 
 
-def append(cache, key, value, query, rotary, token_starts):
-    """paged_append's rows; returns the turned query or None."""
-    tokens = key.shape[0]
-    token = torch.arange(tokens, device=key.device)
+def places(cache, tokens, token_starts):
+    """(position, live, stored, page) of new tokens' rows: live ones have a
+    position, stored ones a page of the cache."""
+    device = cache.device
+    token = torch.arange(tokens, device=device)
     lengths = cache.lengths.long()
     if token_starts is None:
         sequence, live = token, torch.ones_like(token, dtype=torch.bool)
@@ -52,31 +56,117 @@ def append(cache, key, value, query, rotary, token_starts):
     block = position // cache.page_size
     page = cache.block_table[sequence, block.clamp_max(cache.max_blocks - 1)].long()
     stored = live & (block < cache.max_blocks) & (page >= 0) & (page < cache.pages)
+    return position, live, stored, page
+
+
+def append(cache, key, value, query, rotary, token_starts):
+    """paged_append's rows; returns the turned query or None."""
+    position, live, stored, page = places(cache, key.shape[0], token_starts)
     turned = key if rotary is None else rotate(key, position, rotary)
     at, row = page[stored], (position % cache.page_size)[stored]
     # (all rows are read before any is stored: they may be views of the pages)
     out = None if query is None else rotate(query, position, rotary, live=live)
     turned, value = turned[stored], value[stored]
+    if isinstance(cache, QuantizedCache):
+        pools = ((cache.key_codes, cache.key_scales, KEYS, turned),
+                 (cache.value_codes, cache.value_scales, VALUES, value))
+        # (a token's codes lie among its neighbours': whole pages are coded anew)
+        pages, local = at.unique(return_inverse=True)
+        for codes, scales, order, rows in pools:
+            plain = [order[0](codes[pages]), order[1](scales[pages])]
+            for pool, new in zip(plain, quantized.quantize(rows)):
+                pool[local, :, row] = new
+            codes[pages], scales[pages] = order[2](plain[0]), order[3](plain[1])
+        return out
     cache.keys[at, :, row] = turned
     cache.values[at, :, row] = value
     return out
 
 
-def decode(query, cache, scaling):
+# unpack codes and scales, pack codes and scales
+KEYS = (quantized.unpack_keys, torch.clone, quantized.pack_keys, torch.clone)
+VALUES = (quantized.unpack_values, quantized.unpack_scales, quantized.pack_values,
+          quantized.pack_scales)
+
+
+def pages_of(cache, pages):
+    """(pages, heads, page_size, head_dim) keys and values, in 32 bits or more."""
+    if isinstance(cache, QuantizedCache):
+        return tuple(quantized.dequantize(order[0](codes[pages]), order[1](scales[pages]))
+                     for codes, scales, order in (
+                         (cache.key_codes, cache.key_scales, KEYS),
+                         (cache.value_codes, cache.value_scales, VALUES)))
+    return _wide(cache.keys[pages]), _wide(cache.values[pages])
+
+
+def read(cache, tokens, token_starts):
+    """paged_read's rows."""
+    position, live, stored, page = places(cache, tokens, token_starts)
+    at, local = page[stored].unique(return_inverse=True)
+    rows = (position % cache.page_size)[stored]
+    found = []
+    for pool in pages_of(cache, at):
+        out = torch.zeros((tokens, cache.heads, cache.head_dim), dtype=cache.dtype,
+                          device=cache.device)
+        out[live & ~stored] = math.nan
+        out[stored] = pool[local, :, rows].to(cache.dtype)
+        found.append(out)
+    return tuple(found)
+
+
+def attend(q, k, v, position, scaling, scores, prefix=0):
+    """(heads, group, rows, dim) outputs of query rows at their positions over
+    (heads, tokens, dim) keys and values, in the inputs' type (32 bits or
+    more); rows that see nothing are zeros."""
+    token = torch.arange(k.shape[1], device=k.device)
+    distance = position[:, None] - token
+    x = torch.matmul(q, k[:, None].transpose(2, 3).contiguous()) * scaling
+    if scores.softcap:
+        x = torch.tanh(x / scores.softcap) * scores.softcap
+    if scores.slopes is not None:
+        x = x - scores.slopes.view(q.shape[0], q.shape[1], 1, 1) * distance.abs()
+    seen = (distance >= 0) | (token < prefix)
+    if scores.window:
+        seen &= distance < scores.window
+    p = torch.softmax(x.masked_fill(~seen, -math.inf), -1)
+    p = p.masked_fill(~seen.any(-1, keepdim=True), 0.0)
+    v = v[:, None]
+    finite = v.isfinite()
+    if bool(finite.all()):
+        return torch.matmul(p, v)
+    # (0 times infinity is NaN: infinities and NaN count for the rows that see them)
+    out = torch.matmul(p, v.masked_fill(~finite, 0.0))
+    for value in (math.inf, -math.inf, math.nan):
+        there = v.isnan() if math.isnan(value) else v == value
+        out = out + torch.where(torch.matmul(seen.to(v.dtype), there.to(v.dtype)) > 0, value, 0.0)
+    return out
+
+
+def decode(query, cache, scaling, scores=None):
     heads, dim = cache.heads, cache.head_dim
     group = query.shape[1] // heads
     out = torch.zeros(query.shape, dtype=query.dtype, device=query.device)
     for b, length in enumerate(cache.lengths.tolist()):
         if length <= 0:
             continue
-        pages = cache.block_table[b, :-(-length // cache.page_size)].long()
+        # (pages before the window may be gone)
+        first = 0
+        if scores is not None and scores.window:
+            first = max(length - scores.window, 0) // cache.page_size
+        pages = cache.block_table[b, first:-(-length // cache.page_size)].long()
         if length > cache.capacity or not bool(((pages >= 0) & (pages < cache.pages)).all()):
             out[b] = math.nan
             continue
+        first *= cache.page_size
         # (blocks, heads, page, dim) -> (heads, length, dim)
-        k, v = (_wide(x[pages].transpose(0, 1).reshape(heads, -1, dim)[:, :length])
-                for x in (cache.keys, cache.values))
+        k, v = (x.transpose(0, 1).reshape(heads, -1, dim)[:, :length - first]
+                for x in pages_of(cache, pages))
         q = _wide(query[b].reshape(heads, group, dim))
-        p = torch.softmax(torch.matmul(q, k.transpose(1, 2)) * scaling, -1)
-        out[b] = torch.matmul(p, v).reshape(heads * group, dim).to(query.dtype)
+        if scores is None:
+            p = torch.softmax(torch.matmul(q, k.transpose(1, 2)) * scaling, -1)
+            out[b] = torch.matmul(p, v).reshape(heads * group, dim).to(query.dtype)
+            continue
+        position = torch.full((1,), length - 1 - first, device=query.device)
+        rows = attend(q[:, :, None], k, v, position, scaling, scores)
+        out[b] = rows.reshape(heads * group, dim).to(query.dtype)
     return out
