@@ -406,6 +406,45 @@ int rkv_quantized_decode(const rkv_quantized_cache* cache, const void* query,
                          size_t workspace_bytes, rkv_stream_t stream);
 int rkv_quantized_plan(const rkv_quantized_cache* cache, int64_t group, size_t* workspace_bytes);
 
+/*
+ * Attention of ragged prompts' rows (no counterpart in the reference, which
+ * leaves it to the model): rows token_starts[b] up to token_starts[b + 1] of
+ * the query are sequence b's (null: all are one sequence's), over its key rows
+ * key_starts[b] up to key_starts[b + 1] (null: as token_starts) of the
+ * (key_tokens, heads, dim) keys and values; the query rows are the last ones of
+ * the key rows.  A row sees the keys up to its own, all of the sequence's first
+ * prefix[b] (device int32 per sequence, null: none), and of these at most
+ * scores->window back; one that sees nothing is zeros.  An infinite or NaN value
+ * counts for the rows that see it.  Query heads h group .. + group - 1 belong
+ * to KV head h.  output: dense (tokens, heads group, dim); rows of no sequence
+ * become zeros with zero_rest, else stay as they were.  bf16 or fp16, head_dim
+ * 32..256 in steps of 32, 16-byte aligned rows, strides in multiples of 8.
+ * Calls with few rows share out their keys and join them through the workspace
+ * (rkv_prompt_plan; 0 bytes: none needed; most_keys: key_tokens, or the tokens
+ * a row of the block table can address).
+ */
+int rkv_prompt_attention(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* key, int64_t k_token_stride, int64_t k_head_stride,
+                         const void* value, int64_t v_token_stride, int64_t v_head_stride,
+                         int dtype, int64_t tokens, int64_t key_tokens, int64_t heads,
+                         int64_t group, int64_t dim, int64_t sequences,
+                         const int32_t* token_starts, const int32_t* key_starts,
+                         const int32_t* prefix, float scale, const rkv_scores* scores,
+                         void* output, int zero_rest, void* workspace, size_t workspace_bytes,
+                         rkv_stream_t stream);
+int rkv_prompt_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t group, int64_t dim,
+                    int64_t most_keys, size_t* workspace_bytes);
+
+/* The same over a paged cache: the query rows are the sequences' last tokens,
+ * which the cache holds (token_starts as rkv_paged_append's).  A row that sees a
+ * token whose page is outside the cache, or of a sequence longer than its
+ * table, is NaN. */
+int rkv_paged_prompt(const rkv_paged_cache* cache, const void* query, int64_t q_token_stride,
+                     int64_t q_head_stride, int64_t group, int64_t tokens,
+                     const int32_t* token_starts, const int32_t* prefix, float scale,
+                     const rkv_scores* scores, void* output, int zero_rest, void* workspace,
+                     size_t workspace_bytes, rkv_stream_t stream);
+
 /* Workspace bytes of rkv_paged_decode for this cache on the current device. */
 int rkv_paged_plan(const rkv_paged_cache* cache, int64_t group, size_t* workspace_bytes);
 

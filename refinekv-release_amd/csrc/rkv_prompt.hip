@@ -1,0 +1,780 @@
+// Attention of prompts' rows, over rows of their own sequences
+// (rkv_prompt_attention) or over a paged cache (rkv_paged_prompt):
+//   out[i, h] = softmax_j(f(scale q[i, h] . K[j])) V
+// over the tokens j of i's sequence that i sees: those up to i, and those of
+// the sequence's prefix, at most `window` back; f caps the scores and biases
+// them by distance.
+#include "rkv_paged_walk.h"
+
+namespace rkv {
+namespace {
+
+constexpr int kPromptThreads = 256;
+constexpr int kWaveRows = 32;                     // query rows of a wave
+constexpr int kTileRows = 4 * kWaveRows;          // of a workgroup
+
+typedef short S16x4 __attribute__((ext_vector_type(4)));
+typedef float F32x16 __attribute__((ext_vector_type(16)));
+
+template <bool kHalf>
+__device__ __forceinline__ F32x16 mma32(const U32x4& a, const U32x4& b, F32x16 c) {
+  if constexpr (kHalf)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        __builtin_bit_cast(typename Type16<true>::V8, a),
+        __builtin_bit_cast(typename Type16<true>::V8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+        __builtin_bit_cast(typename Type16<false>::V8, a),
+        __builtin_bit_cast(typename Type16<false>::V8, b), c, 0, 0, 0);
+}
+
+struct PromptArgs {
+  const char* query;           // (tokens, H G, D)
+  int64_t q_ts, q_hs;          // token and head strides, elements
+  const char* keys;            // rows (key tokens, H, D), or a cache's pages
+  const char* values;
+  int64_t k_ps, k_hs, v_ps, v_hs;  // page (rows: none) and head strides, elements
+  uint32_t k_ts, v_ts;         // row strides, bytes
+  const int32_t* starts;       // [sequences + 1] of the query rows (null: one sequence)
+  const int32_t* key_starts;   // of the key rows (null: as starts)
+  const int32_t* lengths;      // paged: the sequences' tokens
+  const int32_t* table;        // paged (null: rows)
+  int64_t table_stride;
+  const int32_t* prefix;       // [sequences] tokens that all rows see (null: none)
+  int sequences, heads, group, max_blocks, pages, shift;
+  int tokens, key_tokens;
+  int step;                    // starts are implied: sequence b has row b alone
+  float scale;                 // magnitude, times log2 e
+  uint32_t flip;               // on the query's words: the scale's sign
+  float cap, per_cap;          // as WalkArgs
+  const float* slopes;
+  int window;
+  char* out;                   // (tokens, H G, D) dense
+  int zero_rest;               // rows of no sequence become zeros (else: as they were)
+  int tiles;                   // at most so many in the grid
+  int splits;                  // workgroups that share a tile's keys
+  float2* part_ml;             // [splits][tokens H G] (splits > 1)
+  float* part_acc;             // [..][D]
+};
+
+// Keys of a tile in LDS: 64, 32 at head dims whose accumulators take the
+// registers of two waves.
+template <int D>
+struct PromptTile {
+  static constexpr int kTokens = D <= 128 ? 64 : 32;
+  // Rows 16 bytes more than a multiple of 32 apart: 16 lanes that read one
+  // column of 16 rows take all banks.
+  static constexpr int kKeyRow = 2 * D + 16;
+  // An odd multiple of 64 bytes: 4 rows of 64 bytes, as a transposing read of
+  // half a wave takes them, lie in different banks.
+  static constexpr int kValueRow = 2 * D + (D / 32 % 2 ? 0 : 64);
+  static constexpr int kValueAt = kTokens * kKeyRow;
+  static constexpr int kBytes = kValueAt + kTokens * kValueRow;
+};
+
+// A sequence's query rows, and where the workgroup's tile stands in them.
+struct PromptRows {
+  int b, first, count;  // sequence, its first row, its rows
+  int tile;             // of kTileRows (row, head of the group) pairs
+};
+
+__device__ __forceinline__ void rows_of(const PromptArgs& a, int b, int& first, int& count) {
+  int from, to;
+  if (a.step) {
+    from = b;
+    to = b + 1;
+  } else if (a.starts) {
+    from = a.starts[b];
+    to = a.starts[b + 1];
+  } else {
+    from = 0;
+    to = a.tokens;
+  }
+  first = min(max(from, 0), a.tokens);
+  count = min(max(to, first), a.tokens) - first;
+}
+
+__device__ __forceinline__ uint32_t tiles_for(const PromptArgs& a, int count) {
+  return (uint32_t)(((int64_t)count * a.group + kTileRows - 1) / kTileRows);
+}
+
+// The slot-th of the tiles, the last ones of the last sequence first: a
+// sequence's later tiles have more keys.  False: there are fewer.
+__device__ __forceinline__ bool find_tile(const PromptArgs& a, uint32_t slot, PromptRows& r) {
+  const int lane = threadIdx.x % kWave;
+  const int per = (a.sequences + kWave - 1) / kWave;
+  uint32_t sum = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = lane * per + i;
+    if (b >= a.sequences) break;
+    int first, count;
+    rows_of(a, b, first, count);
+    sum += tiles_for(a, count);
+  }
+  const uint32_t upto = wave_scan(sum);
+  const uint32_t total = (uint32_t)uniform((int)__shfl((int)upto, kWave - 1, kWave));
+  if (slot >= total) return false;
+  const uint32_t at = total - 1u - slot;
+  const int owner = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
+  uint32_t rest = at - (uint32_t)uniform(__shfl((int)(upto - sum), owner, kWave));
+  for (r.b = owner * per;; ++r.b) {
+    rows_of(a, r.b, r.first, r.count);
+    r.first = uniform(r.first);
+    r.count = uniform(r.count);
+    const uint32_t here = tiles_for(a, r.count);
+    if (rest < here || r.b + 1 >= a.sequences) break;
+    rest -= here;
+  }
+  r.tile = (int)rest;
+  return true;
+}
+
+// Rows of no sequence: this head group's part of them becomes zeros.
+template <int D>
+__device__ __forceinline__ void zero_rows(const PromptArgs& a, int head) {
+  int first, count, last;
+  rows_of(a, 0, first, count);
+  rows_of(a, a.sequences - 1, last, count);
+  last += count;
+  const int per_row = a.group * (D / 8);
+  const int64_t n = (int64_t)(a.tokens - last + first) * per_row;
+  for (int64_t i = threadIdx.x; i < n; i += kPromptThreads) {
+    const int64_t row = i / per_row, token = row < first ? row : row - first + last;
+    reinterpret_cast<U32x4*>(a.out)[(token * a.heads + head) * per_row + i % per_row] =
+        U32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+// An infinite or NaN value makes NaN of every row whose products it is in, those
+// that do not see it as well.  A workgroup that ends with such rows goes over
+// its keys again: once for the outputs that see +inf or NaN, once for those that
+// see -inf or NaN, each with ones for such values and for the weights of keys
+// that are seen; then with zeros for all of them.
+enum Pass : int { kPlain, kUp, kDown, kFinite };
+
+// What a word of two values is in a pass.
+template <bool kHalf>
+__device__ __forceinline__ uint32_t value_words(uint32_t w, int pass) {
+  constexpr uint32_t kExp = kHalf ? 0x7c00u : 0x7f80u, kOne = kHalf ? 0x3c00u : 0x3f80u;
+  uint32_t to = 0;
+#pragma unroll
+  for (int k = 0; k < 32; k += 16) {
+    const uint32_t v = w >> k & 0xffffu;
+    const bool odd = (v & kExp) == kExp, nan = (v & 0x7fffu) > kExp;
+    const bool counts = odd && (nan || (v >> 15 != 0u) == (pass == kDown));
+    to |= (pass == kFinite ? (odd ? 0u : v) : counts ? kOne : 0u) << k;
+  }
+  return to;
+}
+
+// A workgroup has 128 (row, head of the group) pairs of one sequence and KV
+// head, 32 a wave, and goes over the keys they see in tiles that two LDS buffers
+// hold: the next one's rows are on their way to registers while one is computed.
+// As in the decode the query rows are the products' columns, so that a lane's
+// maximum, sum and accumulators belong to one of them (lanes l and l + 32
+// share row l % 32):
+//   S^T = K Q^T: A = 32 keys (lane l: key l % 32, dims 16 j + 8 (l / 32) ..),
+//     B = the query rows; lane l gets the keys 8 (i / 4) + 4 (l / 32) + i % 4,
+//     i = 0..15.
+//   O^T = V^T P^T: B = 16 keys' weights as the lane has them, slot e of 8: key
+//     8 (e / 4) + 4 (l / 32) + e % 4.  A = V^T over the same slots: two
+//     transposing reads of 4 keys x 16 dims.
+template <int D, bool kHalf, bool kScores>
+__global__ __launch_bounds__(kPromptThreads)
+__attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(PromptArgs a) {
+  using Tile = PromptTile<D>;
+  using E = typename Type16<kHalf>::E;
+  constexpr int T = Tile::kTokens, kGroups = T / 16, kLoads = D / 32;
+  constexpr int kOwn = T == 64 ? 2 : 1;  // tensors of which a wave loads 16 rows a tile
+  constexpr int kMarks = (D / 32 + 1) / 2;
+  __shared__ alignas(16) char smem[2][Tile::kBytes];
+  __shared__ uint32_t marks[2][kMarks][kPromptThreads];  // outputs that kUp and kDown found
+  const int head = (int)(blockIdx.x % (uint32_t)a.heads);
+  const uint32_t slot = blockIdx.x / (uint32_t)a.heads;
+  PromptRows rows;
+  if (!find_tile(a, slot, rows)) {
+    if (a.zero_rest && (int)slot == a.tiles && blockIdx.y == 0) zero_rows<D>(a, head);
+    return;
+  }
+  const int lane = threadIdx.x % kWave, wave = uniform((int)threadIdx.x / kWave);
+  const int l32 = lane & 31, h = lane >> 5;
+
+  // ---- the sequence's keys
+  int length, key_first = 0;
+  bool bad = false;
+  if (a.table) {
+    length = scalar_at(a.lengths, rows.b);
+    bad = length > 0 && (length - 1) >> a.shift >= a.max_blocks;
+    length = bad || length < 0 ? 0 : length;
+  } else if (a.key_starts) {
+    key_first = min(max(scalar_at(a.key_starts, rows.b), 0), a.key_tokens);
+    length = min(max(scalar_at(a.key_starts, rows.b + 1), key_first), a.key_tokens) - key_first;
+  } else {
+    key_first = rows.first;
+    length = rows.count;
+  }
+  int prefix = a.prefix ? scalar_at(a.prefix, rows.b) : 0;
+  prefix = min(max(prefix, 0), length);
+
+  // ---- this lane's row, and the keys that the workgroup and the wave see
+  const int pairs = rows.count * a.group;
+  const int base_pos = length - rows.count;
+  auto position_of = [&](int pair) { return base_pos + pair / a.group; };
+  const int pair0 = rows.tile * kTileRows, pair = pair0 + wave * kWaveRows + l32;
+  const bool mine = pair < pairs;
+  const int in_seq = mine ? pair / a.group : 0, g = mine ? pair % a.group : 0;
+  const int pos = base_pos + in_seq;
+  // keys low < j <= lim are seen
+  const bool sees = mine && pos >= 0;
+  const int lim = sees ? max(pos, prefix - 1) : -1;
+  const int low = sees ? (pos >= a.window ? pos - a.window : -1) : -1;
+  auto range = [&](int from, int to, int& begin, int& end) {  // of pairs from .. to - 1
+    const int p0 = max(position_of(from), 0), p1 = position_of(min(to, pairs) - 1);
+    begin = p0 >= a.window ? p0 - a.window + 1 : 0;
+    end = from >= pairs || p1 < 0 ? 0 : min(max(p1 + 1, prefix), length);
+  };
+  int wg_begin, wg_end, wave_begin, wave_end;
+  range(pair0, pair0 + kTileRows, wg_begin, wg_end);
+  range(pair0 + wave * kWaveRows, pair0 + (wave + 1) * kWaveRows, wave_begin, wave_end);
+  // keys that every row of the wave sees: whole_begin .. whole_end - 1
+  int whole_begin, whole_end;
+  {
+    const int from = pair0 + wave * kWaveRows, to = min(from + kWaveRows, pairs) - 1;
+    const int p0 = position_of(from), p1 = position_of(max(to, from));
+    whole_end = p0 < 0 ? 0 : max(p0 + 1, prefix);
+    whole_begin = p1 >= a.window ? p1 - a.window + 1 : 0;
+  }
+  int tile_begin = wg_begin / T, tile_end = (wg_end + T - 1) / T;
+  if (a.splits > 1) {
+    const int64_t n = max(tile_end - tile_begin, 0), s = blockIdx.y;
+    tile_end = tile_begin + (int)(n * (s + 1) / a.splits);
+    tile_begin += (int)(n * s / a.splits);
+  }
+
+  // ---- the query rows
+  U32x4 q[D / 16];
+  {
+    const char* from = a.query + ((int64_t)(rows.first + in_seq) * a.q_ts +
+                                  (int64_t)(head * a.group + g) * a.q_hs) * 2 + h * 16;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      q[j] = mine ? *reinterpret_cast<const U32x4*>(from + 32 * j) : U32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[j][i] ^= a.flip;
+    }
+  }
+  float slope = 0.0f;
+  if constexpr (kScores)
+    if (a.slopes) slope = a.slopes[head * a.group + g] * kLog2e;
+
+  int pass = kPlain;
+
+  // ---- a wave's 16 rows of a tile: of keys and values, or (32 tokens) of one
+  const int group16 = wave % kGroups;
+  const bool of_values = kOwn == 1 && wave >= 2;
+  U32x4 staged[kOwn][kLoads];
+  bool staged_bad = false;
+  const int64_t block_row = (int64_t)rows.b * a.table_stride;
+  auto page_of = [&](int tile) {
+    const int at = tile * T + 16 * group16;
+    return a.table ? scalar_at(a.table, block_row + (at < length ? at >> a.shift : 0)) : 0;
+  };
+  // (row, byte) of the lane's i-th 16 bytes of a unit
+  auto unit_row = [&](int i) { return (i * kWave + lane) / (D / 8); };
+  auto unit_byte = [&](int i) { return (i * kWave + lane) % (D / 8) * 16; };
+  auto load = [&](int tile, int page) {
+    const int at = tile * T + 16 * group16;
+    const int n = min(length - at, 16);
+    const bool out = a.table && (uint32_t)page >= (uint32_t)a.pages;
+    staged_bad = out && n > 0;
+    const bool any = n > 0 && !out;
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const bool values = kOwn == 2 ? k == 1 : of_values;
+      const uint32_t ts = values ? a.v_ts : a.k_ts;
+      const int64_t hs = values ? a.v_hs : a.k_hs, ps = values ? a.v_ps : a.k_ps;
+      const char* base = (values ? a.values : a.keys) + (int64_t)head * hs * 2;
+      if (a.table)
+        base += (any ? (int64_t)page * ps * 2 : 0) +
+                (int64_t)(any ? at & ((1 << a.shift) - 1) : 0) * ts;
+      else
+        base += (int64_t)(any ? key_first + at : 0) * ts;
+      const auto view = view_of(base, any ? (uint32_t)(n - 1) * ts + D * 2u : 0u);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        staged[k][i] = __builtin_amdgcn_raw_buffer_load_b128(
+            view, (int)((uint32_t)unit_row(i) * ts + (uint32_t)unit_byte(i)), 0, 0);
+    }
+  };
+  auto store = [&](char* buffer) {
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const bool values = kOwn == 2 ? k == 1 : of_values;
+      if (staged_bad && !values) {
+        // (keys of a page that is not there: whoever sees them gets NaN)
+        constexpr uint32_t kNan = kHalf ? 0x7e007e00u : 0x7fc07fc0u;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) staged[k][i] = U32x4{kNan, kNan, kNan, kNan};
+      }
+      if (pass != kPlain && values) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) staged[k][i][j] = value_words<kHalf>(staged[k][i][j], pass);
+      }
+      char* to = buffer + (values ? Tile::kValueAt : 0);
+      const int stride = values ? Tile::kValueRow : Tile::kKeyRow;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        *reinterpret_cast<U32x4*>(to + (16 * group16 + unit_row(i)) * stride + unit_byte(i)) =
+            staged[k][i];
+    }
+  };
+
+  F32x16 acc[D / 32];
+  float m, l;
+  for (;;) {
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[n][i] = 0.0f;
+    m = kNegInf;
+    l = 0.0f;
+    int page_next = 0;
+    if (tile_begin < tile_end) {
+      load(tile_begin, page_of(tile_begin));
+      page_next = page_of(tile_begin + 1);
+      store(smem[0]);
+    }
+    __syncthreads();
+    for (int tile = tile_begin; tile < tile_end; ++tile) {
+      const char* buffer = smem[(tile - tile_begin) & 1];
+      const bool more = tile + 1 < tile_end;
+      if (more) {
+        load(tile + 1, page_next);
+        page_next = page_of(tile + 2);
+      }
+      const int t0 = tile * T;
+      if (t0 < wave_end && t0 + T > wave_begin) {
+        // ---- scores
+        F32x16 s[T / 32];
+#pragma unroll
+        for (int u = 0; u < T / 32; ++u) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+          const char* keys = buffer + (32 * u + l32) * Tile::kKeyRow + 16 * h;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+            s[u] = mma32<kHalf>(*reinterpret_cast<const U32x4*>(keys + 32 * j), q[j], s[u]);
+        }
+        auto token = [&](int u, int i) { return t0 + 32 * u + 8 * (i / 4) + 4 * h + i % 4; };
+        if constexpr (kScores) {
+          const float by = a.cap > 0.0f ? a.per_cap : a.scale;
+#pragma unroll
+          for (int u = 0; u < T / 32; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x = s[u][i] * by;
+              if (a.cap > 0.0f) x = tanh_hw(x) * a.cap;
+              if (a.slopes) x -= slope * __builtin_fabsf((float)(pos - token(u, i)));
+              s[u][i] = x;
+            }
+        }
+        const float scale = kScores ? 1.0f : a.scale;
+        if (t0 + T > whole_end || t0 < whole_begin) {
+#pragma unroll
+          for (int u = 0; u < T / 32; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              s[u][i] = token(u, i) <= lim && token(u, i) > low ? s[u][i] : kNegInf;
+        }
+        // ---- weights
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < T / 32; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[u][i]);
+        float x, y;
+        xor32_pair(top, x, y);
+        top = __builtin_fmaxf(x, y) * scale;
+        // (the maximum may lag by 2^8: weights up to that, and fewer rescalings)
+        if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {
+          const float mn = __builtin_fmaxf(m, top);
+          const float by = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          m = mn;
+          l *= by;
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) acc[n] *= by;
+        }
+        // (fp16 weights start from 2^7: those under 2^-24 of the largest, many
+        // in a long context, do not all round to zero)
+        const float base = m == kNegInf ? 0.0f : kHalf ? m - 7.0f : m;
+        U32x4 p[T / 16];
+#pragma unroll
+        for (int u = 0; u < T / 32; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            typedef E E2 __attribute__((ext_vector_type(2)));
+            const float p0 =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], scale, -base));
+            const float p1 =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i + 1], scale, -base));
+            l += p0;
+            l += p1;
+            // A weight is rounded to 16 bits, as the products take it: 2^-9 of it in
+            // bf16, half of what an output's own rounding may be off by.
+            p[2 * u + i / 8][i % 8 / 2] = __builtin_bit_cast(uint32_t, E2{(E)p0, (E)p1});
+          }
+        if (pass == kUp || pass == kDown) {  // every key that is seen counts once
+#pragma unroll
+          for (int u = 0; u < T / 32; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              constexpr uint32_t kOne = kHalf ? 0x3c00u : 0x3f80u;
+              auto seen = [&](int e) { return token(u, e) <= lim && token(u, e) > low; };
+              p[2 * u + i / 8][i % 8 / 2] = (seen(i) ? kOne : 0u) | (seen(i + 1) ? kOne << 16 : 0u);
+            }
+        }
+        // ---- products
+        const int l16 = lane & 15;
+        const char* values = buffer + Tile::kValueAt + (4 * h + l16 / 4) * Tile::kValueRow +
+                             32 * (lane >> 4 & 1) + 8 * (l16 % 4);
+#pragma unroll
+        for (int c = 0; c < T / 16; ++c)
+#pragma unroll
+          for (int n = 0; n < D / 32; ++n) {
+            U32x4 v;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              typedef __attribute__((address_space(3))) S16x4 Lds;
+              const auto w = __builtin_bit_cast(
+                  U32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                             (Lds*)(values + (16 * c + 8 * k) * Tile::kValueRow + 64 * n)));
+              v[2 * k] = w[0];
+              v[2 * k + 1] = w[1];
+            }
+            acc[n] = mma32<kHalf>(v, p[c], acc[n]);
+          }
+      }
+      if (more) store(smem[(tile + 1 - tile_begin) & 1]);
+      __syncthreads();
+    }
+    if (pass == kFinite) break;
+    if (pass == kPlain) {
+      float sum = 0.0f;  // finite values times 0: NaN if one is not
+#pragma unroll
+      for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[n][i], 0.0f, sum);
+      if (!__syncthreads_or(sum != 0.0f)) break;
+      pass = kUp;
+      continue;
+    }
+#pragma unroll
+    for (int w = 0; w < kMarks; ++w) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (2 * w + i / 16 < D / 32) bits |= acc[2 * w + i / 16][i % 16] != 0.0f ? 1u << i : 0u;
+      marks[pass - kUp][w][threadIdx.x] = bits;
+    }
+    pass = pass == kUp ? kDown : kFinite;
+  }
+  if (pass == kFinite) {
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) {
+      const uint32_t up = marks[0][n / 2][threadIdx.x] >> (16 * (n % 2));
+      const uint32_t down = marks[1][n / 2][threadIdx.x] >> (16 * (n % 2));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const bool u = up >> i & 1u, d = down >> i & 1u;
+        acc[n][i] += u && d ? __builtin_nanf("") : u ? kPosInf : d ? kNegInf : 0.0f;
+      }
+    }
+  }
+
+  // ---- the rows
+  float x, y;
+  xor32_pair(l, x, y);
+  l = x + y;
+  if (!mine) return;
+  if (bad) l = __builtin_nanf("");
+  const int64_t row = (int64_t)(rows.first + in_seq) * (a.heads * a.group) + head * a.group + g;
+  if (a.splits > 1) {
+    const int64_t at = (int64_t)blockIdx.y * a.tokens * (a.heads * a.group) + row;
+    float* to = a.part_acc + at * D + 4 * h;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<F32x4*>(to + 32 * n + 8 * k) =
+            F32x4{acc[n][4 * k], acc[n][4 * k + 1], acc[n][4 * k + 2], acc[n][4 * k + 3]};
+    if (h == 0) a.part_ml[at] = make_float2(m, l);
+    return;
+  }
+  const float by = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees nothing: zeros)
+  char* to = a.out + row * (D * 2) + 8 * h;
+#pragma unroll
+  for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      typedef E E4 __attribute__((ext_vector_type(4)));
+      E4 v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (E)(acc[n][4 * k + i] * by);
+      *reinterpret_cast<E4*>(to + 64 * n + 16 * k) = v;
+    }
+}
+
+// Joins the parts of a tile's rows, each D / 4 threads one row at a time.
+template <int D, bool kHalf>
+__global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs a) {
+  using E = typename Type16<kHalf>::E;
+  constexpr int kAcross = D / 4, kRows = kPromptThreads / kAcross;
+  const int head = (int)(blockIdx.x % (uint32_t)a.heads);
+  PromptRows rows;
+  if (!find_tile(a, blockIdx.x / (uint32_t)a.heads, rows)) return;
+  const int c = (int)threadIdx.x % kAcross, in = (int)threadIdx.x / kAcross;
+  const int pairs = min(rows.count * a.group - rows.tile * kTileRows, kTileRows);
+  const int64_t all = (int64_t)a.tokens * (a.heads * a.group);
+  for (int i = (int)blockIdx.y * kRows + in; in < kRows && i < pairs;
+       i += kRows * (int)gridDim.y) {
+    const int pair = rows.tile * kTileRows + i;
+    const int64_t row = (int64_t)(rows.first + pair / a.group) * (a.heads * a.group) +
+                        head * a.group + pair % a.group;
+    float m = kNegInf, l = 0.0f;
+    F32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    fold_parts(0u, 1u, (uint32_t)a.splits, m, l, o,
+               [&](uint32_t j) { return a.part_ml[j * all + row]; },
+               [&](uint32_t j) {
+                 return *reinterpret_cast<const float4*>(a.part_acc + (j * all + row) * D + 4 * c);
+               });
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    E4 v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (E)(o[k] * by);
+    *reinterpret_cast<E4*>(a.out + (row * D + 4 * c) * 2) = v;
+  }
+}
+
+struct PromptPlan {
+  int tiles = 0, splits = 1;
+  size_t acc_off = 0, total = 0;
+};
+
+// Tiles: at most those of all rows together and one more a sequence.  Few
+// tiles share their keys out until the device has two workgroups a CU, 256 keys
+// each at least.
+PromptPlan prompt_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t group, int64_t dim,
+                       int64_t most_keys) {
+  PromptPlan P;
+  const int64_t some = tokens < sequences ? tokens : sequences;
+  P.tiles = (int)(tokens * group / kTileRows + some);
+  const int64_t blocks = P.tiles * heads, want = 2 * compute_units();
+  int64_t splits = blocks > 0 && blocks < want ? want / blocks : 1;
+  const int64_t most = (most_keys + 255) / 256;
+  splits = splits < most ? splits : most;
+  P.splits = (int)(splits > 1 ? splits : 1);
+  if (P.splits > 1) {
+    const size_t rows = (size_t)(tokens * heads * group) * P.splits;
+    P.acc_off = (rows * sizeof(float2) + 255) & ~(size_t)255;
+    P.total = P.acc_off + rows * dim * sizeof(float);
+  }
+  return P;
+}
+
+int check_prompt(const char* who, int dtype, int64_t tokens, int64_t sequences, int64_t heads,
+                 int64_t group, int64_t dim) {
+  if (dtype != RKV_BF16 && dtype != RKV_F16)
+    return set_error(kUnsupported, "%s: rows must be bfloat16 or float16", who);
+  if (!supported_dim(dim))
+    return set_error(kUnsupported, "%s: head_dim %lld not in 32..256 step 32", who,
+                     (long long)dim);
+  const int64_t lim = (int64_t(1) << 31) - 1;
+  if (tokens < 0 || sequences <= 0 || heads <= 0 || group <= 0 || sequences > lim ||
+      heads > 65535 || group > 65535)
+    return set_error(kInvalidArgument, "%s: empty or oversized shape", who);
+  // (pairs of a sequence, and the grid, are counted in 32 bits)
+  if (tokens > lim / group - kTileRows || heads * group > lim ||
+      (tokens * group / kTileRows + (tokens < sequences ? tokens : sequences) + 1) > lim / heads)
+    return set_error(kUnsupported, "%s: too many rows", who);
+  return kOk;
+}
+
+int prompt(const char* who, PromptArgs& a, int dtype, int64_t tokens, int64_t sequences,
+           int64_t heads, int64_t group, int64_t dim, int64_t most_keys, const void* query,
+           int64_t q_ts, int64_t q_hs, float scale, const rkv_scores* scores, void* output,
+           int zero_rest, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (tokens == 0) return kOk;
+  if (!query || !output) return set_error(kInvalidArgument, "%s: null pointer argument", who);
+  q_ts = read_stride(q_ts, tokens);
+  q_hs = read_stride(q_hs, heads * group);
+  if (q_ts < 0 || q_hs < 0 || q_ts % 8 || q_hs % 8 || !aligned(query, 16) || !aligned(output, 16))
+    return set_error(kInvalidArgument, "%s: query and output must be 16-byte aligned with strides "
+                     "in multiples of 8", who);
+  int rc = check_scores(who, scores);
+  if (rc) return rc;
+  const PromptPlan P = prompt_plan(tokens, sequences, heads, group, dim, most_keys);
+  if (P.total) {
+    if (!workspace || workspace_bytes < P.total)
+      return set_error(kWorkspaceTooSmall, "%s: workspace of %zu bytes, %zu needed", who,
+                       workspace_bytes, P.total);
+    if (!aligned(workspace, 16))
+      return set_error(kInvalidArgument, "%s: workspace must be 16-byte aligned", who);
+    a.part_ml = static_cast<float2*>(workspace);
+    a.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + P.acc_off);
+  }
+  a.query = static_cast<const char*>(query);
+  a.q_ts = q_ts;
+  a.q_hs = q_hs;
+  a.sequences = (int)sequences;
+  a.heads = (int)heads;
+  a.group = (int)group;
+  a.tokens = (int)tokens;
+  const float size = scale < 0.0f ? -scale : scale;
+  a.scale = size * kLog2e;
+  a.flip = scale < 0.0f ? 0x80008000u : 0u;
+  a.window = scores_window(scores);
+  if (scores) {
+    a.slopes = scores->slopes;
+    if (scores->softcap > 0.0f) {
+      a.cap = scores->softcap * kLog2e;
+      a.per_cap = size / scores->softcap;
+    }
+  }
+  a.out = static_cast<char*>(output);
+  a.zero_rest = zero_rest;
+  a.tiles = P.tiles;
+  a.splits = P.splits;
+  // (a window alone changes no score; a scale of 0 times a hidden score would)
+  const bool plain = !(a.cap > 0.0f) && !a.slopes && a.scale > 0.0f && a.scale < kPosInf;
+  const dim3 grid((unsigned)((P.tiles + (zero_rest ? 1 : 0)) * heads), (unsigned)P.splits);
+  const dim3 join((unsigned)(P.tiles * heads), 8), threads(kPromptThreads);
+  RKV_DISPATCH_DIM(dim, D, {
+    if (dtype == RKV_F16) {
+      if (plain) prompt_kernel<D, true, false><<<grid, threads, 0, stream>>>(a);
+      else prompt_kernel<D, true, true><<<grid, threads, 0, stream>>>(a);
+      if (P.splits > 1) prompt_join_kernel<D, true><<<join, threads, 0, stream>>>(a);
+    } else {
+      if (plain) prompt_kernel<D, false, false><<<grid, threads, 0, stream>>>(a);
+      else prompt_kernel<D, false, true><<<grid, threads, 0, stream>>>(a);
+      if (P.splits > 1) prompt_join_kernel<D, false><<<join, threads, 0, stream>>>(a);
+    }
+  });
+  return check_launch("prompt_kernel");
+}
+
+}  // namespace
+}  // namespace rkv
+
+using namespace rkv;
+
+extern "C" int rkv_prompt_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t group,
+                               int64_t dim, int64_t most_keys, size_t* workspace_bytes) {
+  const char* who = "rkv_prompt_plan";
+  clear_error();
+  if (!workspace_bytes) return set_error(kInvalidArgument, "%s: null pointer", who);
+  const int rc = check_prompt(who, RKV_BF16, tokens, sequences, heads, group, dim);
+  if (rc) return rc;
+  *workspace_bytes = prompt_plan(tokens, sequences, heads, group, dim, most_keys).total;
+  return kOk;
+}
+
+extern "C" int rkv_prompt_attention(const void* query, int64_t q_token_stride,
+                                    int64_t q_head_stride, const void* key, int64_t k_token_stride,
+                                    int64_t k_head_stride, const void* value,
+                                    int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                                    int64_t tokens, int64_t key_tokens, int64_t heads,
+                                    int64_t group, int64_t dim, int64_t sequences,
+                                    const int32_t* token_starts, const int32_t* key_starts,
+                                    const int32_t* prefix, float scale, const rkv_scores* scores,
+                                    void* output, int zero_rest, void* workspace,
+                                    size_t workspace_bytes, hipStream_t stream) {
+  const char* who = "rkv_prompt_attention";
+  clear_error();
+  int rc = check_prompt(who, dtype, tokens, sequences, heads, group, dim);
+  if (rc) return rc;
+  const int64_t lim = (int64_t(1) << 31) - 1;
+  if (key_tokens < 0 || key_tokens > lim)
+    return set_error(kInvalidArgument, "%s: bad key count", who);
+  if (!token_starts && (sequences != 1 || key_starts))
+    return set_error(kInvalidArgument, "%s: several sequences need token_starts", who);
+  if (!key_starts && key_tokens != tokens)
+    return set_error(kInvalidArgument, "%s: without key_starts as many keys as rows", who);
+  if (tokens == 0) return kOk;
+  if (key_tokens && (!key || !value))
+    return set_error(kInvalidArgument, "%s: null pointer argument", who);
+  PromptArgs a{};
+  const int64_t strides[4] = {read_stride(k_token_stride, key_tokens),
+                              read_stride(k_head_stride, heads),
+                              read_stride(v_token_stride, key_tokens),
+                              read_stride(v_head_stride, heads)};
+  for (int64_t s : strides)
+    if (s < 0 || s % 8)
+      return set_error(kInvalidArgument, "%s: strides must be multiples of 8, not negative", who);
+  if (!aligned(key, 16) || !aligned(value, 16))
+    return set_error(kInvalidArgument, "%s: rows must be 16-byte aligned", who);
+  // 16 rows are addressed with 32-bit byte offsets
+  if (strides[0] > (1 << 25) || strides[2] > (1 << 25))
+    return set_error(kUnsupported, "%s: rows more than 64 MiB apart", who);
+  a.keys = static_cast<const char*>(key);
+  a.values = static_cast<const char*>(value);
+  a.k_ts = (uint32_t)(strides[0] * 2);
+  a.k_hs = strides[1];
+  a.v_ts = (uint32_t)(strides[2] * 2);
+  a.v_hs = strides[3];
+  a.key_tokens = (int)key_tokens;
+  a.starts = token_starts;
+  a.key_starts = key_starts;
+  a.prefix = prefix;
+  return prompt(who, a, dtype, tokens, sequences, heads, group, dim, key_tokens, query,
+                q_token_stride, q_head_stride, scale, scores, output, zero_rest, workspace,
+                workspace_bytes, stream);
+}
+
+extern "C" int rkv_paged_prompt(const rkv_paged_cache* cache, const void* query,
+                                int64_t q_token_stride, int64_t q_head_stride, int64_t group,
+                                int64_t tokens, const int32_t* token_starts,
+                                const int32_t* prefix, float scale, const rkv_scores* scores,
+                                void* output, int zero_rest, void* workspace,
+                                size_t workspace_bytes, hipStream_t stream) {
+  const char* who = "rkv_paged_prompt";
+  clear_error();
+  int rc = check_cache(who, cache);
+  if (!rc)
+    rc = check_prompt(who, cache->dtype, tokens, cache->sequences, cache->heads, group, cache->dim);
+  if (rc) return rc;
+  if (!token_starts && tokens != cache->sequences)
+    return set_error(kInvalidArgument, "%s: without token_starts one token per sequence", who);
+  PromptArgs a{};
+  a.k_ps = read_stride(cache->key_page_stride, cache->pages);
+  a.k_hs = read_stride(cache->key_head_stride, cache->heads);
+  a.v_ps = read_stride(cache->value_page_stride, cache->pages);
+  a.v_hs = read_stride(cache->value_head_stride, cache->heads);
+  if (a.k_ps % 8 || a.k_hs % 8 || a.v_ps % 8 || a.v_hs % 8 || cache->key_token_stride % 8 ||
+      cache->value_token_stride % 8 || !aligned(cache->keys, 16) || !aligned(cache->values, 16))
+    return set_error(kInvalidArgument, "%s: the cache must be 16-byte aligned with strides in "
+                     "multiples of 8", who);
+  if (cache->key_token_stride > (1 << 25) || cache->value_token_stride > (1 << 25))
+    return set_error(kUnsupported, "%s: rows more than 64 MiB apart", who);
+  if (rows_meet_pages(cache, output, cache->heads * group * cache->dim, cache->dim, tokens,
+                      cache->heads * group))
+    return set_error(kInvalidArgument, "%s: output overlaps the cache", who);
+  a.keys = static_cast<const char*>(cache->keys);
+  a.values = static_cast<const char*>(cache->values);
+  a.k_ts = (uint32_t)(cache->key_token_stride * 2);
+  a.v_ts = (uint32_t)(cache->value_token_stride * 2);
+  a.starts = token_starts;
+  a.step = !token_starts;
+  a.lengths = cache->lengths;
+  a.table = cache->block_table;
+  a.table_stride = cache->table_stride;
+  a.prefix = prefix;
+  a.max_blocks = (int)cache->max_blocks;
+  a.pages = (int)cache->pages;
+  a.shift = page_shift(cache->page_size);
+  return prompt(who, a, cache->dtype, tokens, cache->sequences, cache->heads, group, cache->dim,
+                cache->max_blocks * cache->page_size, query, q_token_stride, q_head_stride, scale,
+                scores, output, zero_rest, workspace, workspace_bytes, stream);
+}

@@ -7,6 +7,7 @@ Same public API as the reference package (src/refinekv/__init__.py:3-25);
 from .attention import AttentionResult, select_blocks, select_blocks_union, sparse_attention
 from .config import RefineKVConfig
 from .paged import PagedCache, paged_append, paged_decode, paged_read
+from .prompt import paged_prompt, prompt_attention
 from .quantized import QuantizedCache
 from .rotary import Rotary, RotaryConfig, rotate_heads
 from .summary import BlockSummary, build_summary
@@ -23,7 +24,9 @@ __all__ = [
     "build_summary",
     "paged_append",
     "paged_decode",
+    "paged_prompt",
     "paged_read",
+    "prompt_attention",
     "rotate_heads",
     "select_blocks",
     "select_blocks_union",

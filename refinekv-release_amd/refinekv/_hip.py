@@ -142,6 +142,15 @@ def _bind(lib):
     lib.rkv_quantized_decode.restype = _int
     lib.rkv_quantized_plan.argtypes = [_p, _i64, _p]
     lib.rkv_quantized_plan.restype = _int
+    lib.rkv_prompt_attention.argtypes = [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _int,
+                                         _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _f32, _p,
+                                         _p, _int, _p, _size, _p]
+    lib.rkv_prompt_attention.restype = _int
+    lib.rkv_paged_prompt.argtypes = [_p, _p, _i64, _i64, _i64, _i64, _p, _p, _f32, _p, _p, _int,
+                                     _p, _size, _p]
+    lib.rkv_paged_prompt.restype = _int
+    lib.rkv_prompt_plan.argtypes = [_i64, _i64, _i64, _i64, _i64, _i64, _p]
+    lib.rkv_prompt_plan.restype = _int
     return lib
 
 
@@ -787,6 +796,98 @@ def paged_decode(query, cache, scaling, workspace=None, output=None, scores=None
     if rc:
         _check(rc, "rkv_paged_decode")
     return output
+
+
+# ---------------------------------------------------------------------------
+# Prompts
+# ---------------------------------------------------------------------------
+
+MAX_ROW_STRIDE = 1 << 25  # of prompts' key and value rows, elements
+_prompt_sizes = {}
+
+
+def _prompt_scratch(workspace, tokens, sequences, heads, group, dim, most_keys, device):
+    """(buffer or None, bytes) for a prompt's call: sizes are rounded up to powers
+    of two, so that a workspace keeps few buffers (none ever replaced: a
+    captured graph keeps using the one it was captured with)."""
+    shape = (tokens, sequences, heads, group, dim, most_keys, device.index)
+    nbytes = _prompt_sizes.get(shape)
+    if nbytes is None:
+        found = _size()
+        _check(lib().rkv_prompt_plan(*shape[:6], ctypes.byref(found)), "rkv_prompt_plan")
+        nbytes = 1 << max(found.value - 1, (1 << 20) - 1).bit_length() if found.value else 0
+        if len(_prompt_sizes) >= 4096:
+            _prompt_sizes.clear()
+        _prompt_sizes[shape] = nbytes
+    if not nbytes:
+        return None, 0
+    return _buffer(workspace, ("hip_prompt_scratch", nbytes, device.index), (nbytes,), device,
+                   torch.uint8), nbytes
+
+
+def _prompt_output(output, query):
+    """A call's output, and whether its rows of no sequence become zeros."""
+    return (_like(query), 1) if output is None else (output, 0)
+
+
+def prompt_attention(query, key, value, sequences, token_starts, key_starts, prefix, scaling,
+                     scores, workspace=None, output=None):
+    """rkv_prompt_attention on checked rows."""
+    device = query.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return prompt_attention(query, key, value, sequences, token_starts, key_starts,
+                                    prefix, scaling, scores, workspace, output)
+    query, key, value = (_row_aligned(t, 16) for t in (query, key, value))
+    key, value = (t.contiguous() if t.stride(0) > MAX_ROW_STRIDE else t for t in (key, value))
+    if output is not None and output.data_ptr() % 16:  # (the kernel stores whole vectors)
+        return output.copy_(prompt_attention(query, key, value, sequences, token_starts,
+                                             key_starts, prefix, scaling, scores, workspace,
+                                             output.clone()))
+    tokens, q_heads, dim = query.shape
+    heads = key.shape[1]
+    out, zero_rest = _prompt_output(output, query)
+    scratch, nbytes = _prompt_scratch(workspace, tokens, sequences, heads, q_heads // heads, dim,
+                                      key.shape[0], device)
+    rc = lib().rkv_prompt_attention(
+        *_rows(query), *_rows(key), *_rows(value), DTYPE_CODES[query.dtype], tokens, key.shape[0],
+        heads, q_heads // heads, dim, sequences,
+        0 if token_starts is None else token_starts.data_ptr(),
+        0 if key_starts is None else key_starts.data_ptr(),
+        0 if prefix is None else prefix.data_ptr(), scaling, _scores(scores), out.data_ptr(),
+        zero_rest if token_starts is not None else 0,
+        0 if scratch is None else scratch.data_ptr(), nbytes, _raw_stream(device))
+    if rc:
+        _check(rc, "rkv_prompt_attention")
+    return out
+
+
+def paged_prompt(query, cache, token_starts, prefix, scaling, scores, workspace=None,
+                 output=None):
+    """rkv_paged_prompt on a checked query."""
+    device = query.device
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return paged_prompt(query, cache, token_starts, prefix, scaling, scores, workspace,
+                                output)
+    query = _row_aligned(query, 16)
+    if output is not None and output.data_ptr() % 16:  # (the kernel stores whole vectors)
+        return output.copy_(paged_prompt(query, cache, token_starts, prefix, scaling, scores,
+                                         workspace, output.clone()))
+    tokens, q_heads, dim = query.shape
+    group = q_heads // cache.heads
+    out, zero_rest = _prompt_output(output, query)
+    scratch, nbytes = _prompt_scratch(workspace, tokens, cache.sequences, cache.heads, group, dim,
+                                      cache.capacity, device)
+    rc = lib().rkv_paged_prompt(
+        _cache_struct(cache), *_rows(query), group, tokens,
+        0 if token_starts is None else token_starts.data_ptr(),
+        0 if prefix is None else prefix.data_ptr(), scaling, _scores(scores), out.data_ptr(),
+        zero_rest if token_starts is not None else 0,
+        0 if scratch is None else scratch.data_ptr(), nbytes, _raw_stream(device))
+    if rc:
+        _check(rc, "rkv_paged_prompt")
+    return out
 
 
 def set_decode_path(name):

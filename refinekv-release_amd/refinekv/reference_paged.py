@@ -121,13 +121,14 @@ def attend(q, k, v, position, scaling, scores, prefix=0):
     token = torch.arange(k.shape[1], device=k.device)
     distance = position[:, None] - token
     x = torch.matmul(q, k[:, None].transpose(2, 3).contiguous()) * scaling
-    if scores.softcap:
-        x = torch.tanh(x / scores.softcap) * scores.softcap
-    if scores.slopes is not None:
-        x = x - scores.slopes.view(q.shape[0], q.shape[1], 1, 1) * distance.abs()
-    seen = (distance >= 0) | (token < prefix)
-    if scores.window:
-        seen &= distance < scores.window
+    seen = ((distance >= 0) | (token < prefix)) & (position >= 0)[:, None]
+    if scores is not None:
+        if scores.softcap:
+            x = torch.tanh(x / scores.softcap) * scores.softcap
+        if scores.slopes is not None:
+            x = x - scores.slopes.view(q.shape[0], q.shape[1], 1, 1) * distance.abs()
+        if scores.window:
+            seen &= distance < scores.window
     p = torch.softmax(x.masked_fill(~seen, -math.inf), -1)
     p = p.masked_fill(~seen.any(-1, keepdim=True), 0.0)
     v = v[:, None]
@@ -140,6 +141,70 @@ def attend(q, k, v, position, scaling, scores, prefix=0):
         there = v.isnan() if math.isnan(value) else v == value
         out = out + torch.where(torch.matmul(seen.to(v.dtype), there.to(v.dtype)) > 0, value, 0.0)
     return out
+
+
+ATTENDED = 1 << 26  # scores held at a time
+
+
+def _prompt(query, heads, starts, keys_of, scaling, scores, prefix, output):
+    """Prompts' rows, a sequence at a time: keys_of(b) gives its (heads, tokens,
+    dim) keys and values, or None where its rows are NaN."""
+    tokens, q_heads, dim = query.shape
+    group = q_heads // heads
+    out = torch.zeros_like(query, memory_format=torch.contiguous_format) if output is None \
+        else output
+    for b in range(len(starts) - 1):
+        first = min(max(starts[b], 0), tokens)
+        end = min(max(starts[b + 1], first), tokens)
+        if first == end:
+            continue
+        rows = keys_of(b)
+        if rows is None:
+            out[first:end] = math.nan
+            continue
+        k, v = rows
+        n = k.shape[1]
+        seen = 0 if prefix is None else min(max(int(prefix[b]), 0), n)
+        together = max(1, ATTENDED // max(n * q_heads, 1))
+        for row in range(first, end, together):
+            take = slice(row, min(row + together, end))
+            position = n - end + torch.arange(take.start, take.stop, device=query.device)
+            q = _wide(query[take]).unflatten(1, (heads, group)).permute(1, 2, 0, 3)
+            y = attend(q, k, v, position, scaling, scores, seen)
+            out[take] = y.permute(2, 0, 1, 3).flatten(1, 2).to(query.dtype)
+    return out
+
+
+def prompt_rows(query, key, value, token_starts, key_starts, prefix, scaling, scores, output):
+    starts = [0, query.shape[0]] if token_starts is None else token_starts.tolist()
+    ends = starts if key_starts is None else key_starts.tolist()
+
+    def keys_of(b):
+        first = min(max(ends[b], 0), key.shape[0])
+        end = min(max(ends[b + 1], first), key.shape[0])
+        return tuple(_wide(t[first:end]).transpose(0, 1) for t in (key, value))
+
+    return _prompt(query, key.shape[1], starts, keys_of, scaling, scores, prefix, output)
+
+
+def prompt_pages(query, cache, token_starts, prefix, scaling, scores, output):
+    starts = (list(range(query.shape[0] + 1)) if token_starts is None
+              else token_starts.tolist())
+    lengths = cache.lengths.tolist()
+
+    def keys_of(b):
+        n = max(lengths[b], 0)
+        if n > cache.capacity:
+            return None
+        pages = cache.block_table[b, :-(-n // cache.page_size)].long()
+        there = (pages >= 0) & (pages < cache.pages)
+        k, v = pages_of(cache, torch.where(there, pages, 0))
+        # (rows that see a page that is not there are NaN)
+        k = k.masked_fill(~there[:, None, None, None], math.nan)
+        v = v.masked_fill(~there[:, None, None, None], 0.0)
+        return tuple(t.transpose(0, 1).flatten(1, 2)[:, :n] for t in (k, v))
+
+    return _prompt(query, cache.heads, starts, keys_of, scaling, scores, prefix, output)
 
 
 def decode(query, cache, scaling, scores=None):
