@@ -44,6 +44,12 @@ __device__ __forceinline__ uint32_t word_of(Half2 h) { return __builtin_bit_cast
 
 constexpr int kRowThreads = 256;
 constexpr int kItem = 8;  // dims of a thread: 16 bytes of a row
+// From so many threads on the device is full, and fewer threads turn more heads
+// each with the same cos and sin.
+constexpr int64_t kManyRowThreads = 4 * 1024 * 64;
+
+template <typename T>
+using Item = T __attribute__((ext_vector_type(kItem)));
 
 struct Pool {
   char* codes;
@@ -84,86 +90,95 @@ __device__ __forceinline__ ValuePiece value_piece(int dim, int d0) {
   return ValuePiece{(whole + half) * 2, 2, (d0 - whole - half) / 2};
 }
 
-// Max (min of the negatives) over a quad's lanes, the 4 items of a group.
+// The largest value and (min of the negatives) the smallest over a quad's
+// lanes, the 4 items of a group.
+template <int kCtrl>
+__device__ __forceinline__ float quad_lane(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl,
+                                                               0xF, 0xF, false));
+}
 __device__ __forceinline__ float quad_max(float v) {
-  v = __builtin_fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
-                             0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, false)));
-  return __builtin_fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
-                                0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, false)));
+  v = __builtin_fmaxf(v, quad_lane<0xB1>(v));
+  return __builtin_fmaxf(v, quad_lane<0x4E>(v));
 }
 
-// A group's scale and zero from its lanes' values, and the item's codes.
-__device__ __forceinline__ void quantize(const float (&x)[kItem], uint32_t& scale_zero,
-                                         uint32_t (&code)[kItem]) {
-  float low = x[0], high = x[0];
-  uint32_t size = 0;  // the largest magnitude's bits: above kLargest's for NaN
+// A group's scale and zero from its lanes' values, and the item's codes as whole
+// floats.
+template <typename T>
+__device__ __forceinline__ void quantize(const Item<T>& v, uint32_t& scale_zero,
+                                         float (&code)[kItem]) {
+  float x[kItem];
 #pragma unroll
-  for (int e = 0; e < kItem; ++e) {
+  for (int e = 0; e < kItem; ++e) x[e] = (float)v[e];
+  float low = x[0], high = x[0];
+#pragma unroll
+  for (int e = 1; e < kItem; ++e) {
     low = __builtin_fminf(low, x[e]);
     high = __builtin_fmaxf(high, x[e]);
-    const uint32_t bits = f32_bits(x[e]) & 0x7fffffffu;
-    size = size > bits ? size : bits;
   }
+  // the largest magnitude as an integer: NaN's are the largest of all (min and
+  // max would skip them)
+  typedef uint16_t U16x2 __attribute__((ext_vector_type(2)));
+  const U32x4 words = __builtin_bit_cast(U32x4, v);
+  U16x2 size = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    size = __builtin_elementwise_max(size, __builtin_bit_cast(U16x2, words[i] & 0x7fff7fffu));
+  uint32_t top = size[0] > size[1] ? size[0] : size[1];
+  constexpr uint32_t kTop = __builtin_bit_cast(uint16_t, (T)kLargest);
+  const float over = top > kTop ? 1.0f : 0.0f;
   high = quad_max(high);
   low = -quad_max(-low);
-  // (as floats NaN's bits would be skipped; as integers below 2^31 they order)
-  auto other = [](uint32_t v, auto ctrl) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl(), 0xF, 0xF, false);
-  };
-  uint32_t o = other(size, std::integral_constant<int, 0xB1>());
-  size = size > o ? size : o;
-  o = other(size, std::integral_constant<int, 0x4E>());
-  size = size > o ? size : o;
-  const bool held = size <= f32_bits(kLargest);
+  const bool held = quad_max(over) == 0.0f;
   const _Float16 near = (_Float16)((high - low) / 15.0f), zero = (_Float16)low;
   const uint32_t up = ((uint32_t)__builtin_bit_cast(uint16_t, near) + 15u) & 0xfff0u;
   const float step = (float)__builtin_bit_cast(_Float16, (uint16_t)up), base = (float)zero;
   scale_zero = held ? up | (uint32_t)__builtin_bit_cast(uint16_t, zero) << 16 : 0x7e007e00u;
+  // (x - zero) / scale, correctly rounded: with the reciprocal so, a quotient's
+  // remainder corrects it (Markstein).  A reciprocal of 0 where there is no
+  // scale gives codes of 0 (and NaN, which the maximum makes 0).
+  const float per = held && step > 0.0f ? 1.0f / step : 0.0f;
 #pragma unroll
   for (int e = 0; e < kItem; ++e) {
-    const float q = __builtin_rintf((x[e] - base) / step);
-    code[e] = held && step > 0.0f ? (uint32_t)__builtin_fminf(__builtin_fmaxf(q, 0.0f), 15.0f) : 0u;
+    const float d = x[e] - base, near_q = d * per;
+    const float q = __builtin_fmaf(__builtin_fmaf(-near_q, step, d), per, near_q);
+    code[e] = __builtin_rintf(__builtin_fminf(__builtin_fmaxf(q, 0.0f), 15.0f));
   }
 }
 
-template <typename T>
+// Four codes, 4 bits each, low first.
+__device__ __forceinline__ uint32_t pack(float c0, float c1, float c2, float c3) {
+  return (uint32_t)__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(c3, 16.0f, c2), 16.0f, c1), 16.0f,
+                                  c0);
+}
+
 __device__ __forceinline__ void store_key(const QuantRows& a, int64_t row, int d0,
-                                          uint32_t scale_zero, const uint32_t (&code)[kItem]) {
+                                          uint32_t scale_zero, const float (&code)[kItem]) {
   const int groups = a.dim / kGroupDims, group = d0 / kGroupDims, lg = d0 % kGroupDims / kItem;
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < kItem; ++e) w |= code[e] << (4 * (e / 2) + 16 * (e % 2));
+  const uint32_t w = pack(code[0], code[2], code[4], code[6]) |
+                     pack(code[1], code[3], code[5], code[7]) << 16;
   reinterpret_cast<uint32_t*>(a.keys.codes + row * (a.dim / 2))[lg * groups + group] = w;
   if (lg == 0) reinterpret_cast<uint32_t*>(a.keys.scales)[row * groups + group] = scale_zero;
 }
 
-template <typename T>
 __device__ __forceinline__ void store_value(const QuantRows& a, int64_t row, int d0,
-                                            uint32_t scale_zero, const uint32_t (&code)[kItem]) {
+                                            uint32_t scale_zero, const float (&code)[kItem]) {
   const int token = (int)(row & 3), pair = token / 2, second = token % 2;
   const ValuePiece at = value_piece(a.dim, d0);
   char* block = a.values.codes + (row >> 2) * (2 * a.dim) + at.base;
-  if (at.dims == 8) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t w = code[4 * k] | code[4 * k + 1] << 4 | code[4 * k + 2] << 8 |
-                         code[4 * k + 3] << 12;
-      *reinterpret_cast<uint16_t*>(block + at.column * 16 + pair * 8 + k * 4 + second * 2) =
-          (uint16_t)w;
-    }
-  } else if (at.dims == 4) {
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const uint32_t w = code[4 * k] | code[4 * k + 1] << 4 | code[4 * k + 2] << 8 |
-                         code[4 * k + 3] << 12;
-      *reinterpret_cast<uint16_t*>(block + (at.column + k) * 8 + pair * 4 + second * 2) =
-          (uint16_t)w;
-    }
+  const uint32_t low = pack(code[0], code[1], code[2], code[3]),
+                 high = pack(code[4], code[5], code[6], code[7]);
+  if (at.dims > 2) {
+    // (8 dims: two words of a column; 4: one each of two columns)
+    char* to = block + (at.dims == 8 ? at.column * 16 + pair * 8 : at.column * 8 + pair * 4) +
+               second * 2;
+    *reinterpret_cast<uint16_t*>(to) = (uint16_t)low;
+    *reinterpret_cast<uint16_t*>(to + (at.dims == 8 ? 4 : 8)) = (uint16_t)high;
   } else {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       *reinterpret_cast<uint8_t*>(block + (at.column + k) * 4 + second * 2 + pair) =
-          (uint8_t)(code[2 * k] | code[2 * k + 1] << 4);
+          (uint8_t)((k < 2 ? low : high) >> (8 * (k % 2)));
   }
   if (d0 % kGroupDims == 0) {
     char* s = a.values.scales + (row >> 2) * (a.dim / 2) + d0 / kGroupDims * 16 + token * 2;
@@ -172,89 +187,132 @@ __device__ __forceinline__ void store_value(const QuantRows& a, int64_t row, int
   }
 }
 
-// The item's partners in a turn, as a row has them: the dims rotary_dim / 2
-// away, or (interleaved) the neighbours.
-template <typename T>
-__device__ __forceinline__ void partners(const QuantRows& a, const T* row, int d0,
-                                         const float (&x)[kItem], float (&y)[kItem]) {
-  typedef T V __attribute__((ext_vector_type(kItem)));
-  if (a.interleaved) {
-#pragma unroll
-    for (int e = 0; e < kItem; ++e) y[e] = x[e ^ 1];
-    return;
-  }
-  const int half = a.rotary_dim / 2;
-  if (half % kItem == 0) {
-    const V v = *reinterpret_cast<const V*>(row + (d0 < half ? d0 + half : d0 - half));
-#pragma unroll
-    for (int e = 0; e < kItem; ++e) y[e] = (float)v[e];
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < kItem; ++e) {
-    const int d = d0 + e;
-    y[e] = d < a.rotary_dim ? (float)row[d < half ? d + half : d - half] : 0.0f;
-  }
-}
+// Where an item's partners in a turn are, the dims rotary_dim / 2 away or
+// (interleaved) the neighbours: in the item itself, in an item of their own, in
+// parts of two; or (the whole head turns) in the thread's second item.
+enum Partner : int { kWithin, kWhole, kParts, kHalves };
 
-// A thread holds 8 dims of a token's rows: it works out their cos and sin once
-// and applies them to every slots-th head, queries, then keys, then values;
-// the 4 lanes of a group meet for its bounds.
-template <typename T>
+// A thread holds 8 dims of a token's rows (kHalves: twice 8, half a row apart):
+// it works out their cos and sin once and applies them to every slots-th head,
+// queries, then keys, then values, the next head's row on its way while one is
+// turned; the 4 lanes of a group meet for its bounds.
+template <typename T, int kPartner>
 __global__ __launch_bounds__(kRowThreads) void quantize_rows_kernel(QuantRows a) {
-  typedef T V __attribute__((ext_vector_type(kItem)));
-  const int items = a.dim / kItem, wide = items * a.slots;
+  using V = Item<T>;
+  constexpr int kVecs = kPartner == kHalves ? 2 : 1;
+  const int items = a.dim / (kItem * kVecs), wide = items * a.slots;
   const int in_block = (int)threadIdx.x / wide, rest = (int)threadIdx.x % wide;
   const int slot = rest / items, d0 = rest % items * kItem;
   const int64_t t = (int64_t)blockIdx.x * a.per_block + in_block;
   if (in_block >= a.per_block || t >= a.tokens) return;
-  const Place place = place_of(a, t);
-  const bool turns = place.live && d0 < a.rotary_dim;
   const int half = a.rotary_dim / 2;
-  float c[kItem], s[kItem];
+  const bool in_part = d0 < a.rotary_dim;
+  // the second load: the partners' (kWhole), or the second item
+  const int from = kPartner == kHalves ? d0 + half
+                   : !in_part          ? d0
+                   : d0 < half         ? d0 + half
+                                       : d0 - half;
+  V v, w;
+  const T* row;
+  auto load = [&]() {
+    v = *reinterpret_cast<const V*>(row + d0);
+    if constexpr (kPartner == kWhole || kPartner == kHalves)
+      w = *reinterpret_cast<const V*>(row + from);
+  };
+  // (the thread's heads: every slots-th of the queries, then of keys and values)
+  auto to_key_value = [&](int n) {
+    const bool value = n >= a.heads;
+    row = reinterpret_cast<const T*>(value ? a.src[2] : a.src[1]) +
+          t * (value ? a.src_ts[2] : a.src_ts[1]) +
+          (value ? n - a.heads : n) * (value ? a.src_hs[2] : a.src_hs[1]);
+  };
+  if (slot < a.q_heads)
+    row = reinterpret_cast<const T*>(a.src[0]) + t * a.src_ts[0] + slot * a.src_hs[0];
+  else
+    to_key_value(min(slot, 2 * a.heads - 1));
+  load();
+  const Place place = place_of(a, t);
+  const bool turns = place.live && in_part;
+  float c[kItem], s[kItem];  // (s with the sign that the item's dims take it with)
+  if (turns) {
+    const double position4 = 4.0 * (double)place.position;  // rates are whole turns
+    constexpr int kPairs = kPartner == kWithin ? kItem / 2 : kItem;
+    double rate[kPairs];
 #pragma unroll
-  for (int e = 0; e < kItem; ++e) {
-    const int d = d0 + e;
-    c[e] = 1.0f;
-    s[e] = 0.0f;
-    if (turns && d < a.rotary_dim) {
-      const int pair = a.interleaved ? d / 2 : d < half ? d : d - half;
-      const bool first = a.interleaved ? d % 2 == 0 : d < half;
-      cos_sin(4.0 * (double)place.position * a.rates[pair], c[e], s[e]);
-      c[e] *= a.scale;
-      s[e] *= first ? -a.scale : a.scale;
+    for (int e = 0; e < kPairs; ++e) {
+      // (dims of the last item that pass have no pair)
+      const int d = kPartner == kWithin ? d0 / 2 + e : d0 + e < half ? d0 + e : d0 + e - half;
+      rate[e] = a.rates[min(d, half - 1)];
+    }
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) {
+      float cs, sn;
+      cos_sin(position4 * rate[e], cs, sn);
+      cs *= a.scale;
+      sn *= a.scale;
+      if constexpr (kPartner == kWithin) {
+        c[2 * e] = c[2 * e + 1] = cs;
+        s[2 * e] = -sn;
+        s[2 * e + 1] = sn;
+      } else {
+        c[e] = cs;
+        s[e] = d0 + e < half ? -sn : sn;
+      }
     }
   }
-  const bool stored = place.page >= 0;
-  const int total = a.q_heads + 2 * a.heads;
-  for (int n = slot; n < total; n += a.slots) {
-    const int kind = n < a.q_heads ? 0 : n < a.q_heads + a.heads ? 1 : 2;
-    if (kind > 0 && !stored) break;
-    const int h = n - (kind == 0 ? 0 : kind == 1 ? a.q_heads : a.q_heads + a.heads);
-    const T* row = reinterpret_cast<const T*>(a.src[kind]) + t * a.src_ts[kind] +
-                   h * a.src_hs[kind];
-    V v = *reinterpret_cast<const V*>(row + d0);
-    if (kind < 2 && turns) {
-      float x[kItem], y[kItem];
+  auto turn = [&](V& x, V& y, const T* from_row) {
+    const V x0 = x, y0 = y;
 #pragma unroll
-      for (int e = 0; e < kItem; ++e) x[e] = (float)v[e];
-      partners<T>(a, row, d0, x, y);
-#pragma unroll
-      for (int e = 0; e < kItem; ++e)
-        if (d0 + e < a.rotary_dim) v[e] = (T)__builtin_fmaf(x[e], c[e], y[e] * s[e]);
+    for (int e = 0; e < kItem; ++e) {
+      const int d = d0 + e;
+      if constexpr (kPartner == kHalves) {
+        x[e] = (T)__builtin_fmaf((float)x0[e], c[e], (float)y0[e] * s[e]);
+        y[e] = (T)__builtin_fmaf((float)y0[e], c[e], -((float)x0[e] * s[e]));
+      } else {
+        float other;
+        if constexpr (kPartner == kWithin) other = (float)x0[e ^ 1];
+        else if constexpr (kPartner == kWhole) other = (float)y0[e];
+        else other = d < a.rotary_dim ? (float)from_row[d < half ? d + half : d - half] : 0.0f;
+        if (d < a.rotary_dim) x[e] = (T)__builtin_fmaf((float)x0[e], c[e], other * s[e]);
+      }
     }
-    if (kind == 0) {
-      *reinterpret_cast<V*>(reinterpret_cast<T*>(a.dst[0]) + t * a.dst_ts + h * a.dst_hs + d0) = v;
-      continue;
+  };
+  if (a.q_heads > 0) {
+    T* to = reinterpret_cast<T*>(a.dst[0]) + t * a.dst_ts + slot * a.dst_hs;
+    for (int n = slot; n < a.q_heads; n += a.slots) {
+      V x = v, y = w;
+      const T* const from_row = row;
+      if (n + a.slots < a.q_heads) row += a.slots * a.src_hs[0];
+      else to_key_value(min(slot, 2 * a.heads - 1));
+      load();
+      if (turns) turn(x, y, from_row);
+      *reinterpret_cast<V*>(to + d0) = x;
+      if constexpr (kPartner == kHalves) *reinterpret_cast<V*>(to + from) = y;
+      to += a.slots * a.dst_hs;
     }
-    float x[kItem];
+  }
+  if (place.page < 0) return;
+  // (keys and values after the queries: the wave's lanes code together)
+  for (int n = slot; n < 2 * a.heads;) {
+    V x = v, y = w;
+    const T* const from_row = row;
+    const int here = n;
+    n += a.slots;
+    if (n < 2 * a.heads) {
+      to_key_value(n);
+      load();
+    }
+    const bool key = here < a.heads;
+    if (key && turns) turn(x, y, from_row);
+    const int64_t at = row_at(a, place, key ? here : here - a.heads);
 #pragma unroll
-    for (int e = 0; e < kItem; ++e) x[e] = (float)v[e];
-    uint32_t scale_zero, code[kItem];
-    quantize(x, scale_zero, code);
-    const int64_t at = row_at(a, place, h);
-    if (kind == 1) store_key<T>(a, at, d0, scale_zero, code);
-    else store_value<T>(a, at, d0, scale_zero, code);
+    for (int k = 0; k < kVecs; ++k) {
+      uint32_t scale_zero;
+      float code[kItem];
+      quantize<T>(k ? y : x, scale_zero, code);
+      if (key) store_key(a, at, k ? from : d0, scale_zero, code);
+      else store_value(a, at, k ? from : d0, scale_zero, code);
+    }
   }
 }
 
@@ -723,10 +781,11 @@ int rows_args(const char* who, QuantRows& a, const rkv_quantized_cache* c, int64
 }
 
 // Heads that a token's threads hold at a time, and the grid: `heads` rows a
-// token.  Few tokens: a thread per row and item, for latency.
-int rows_grid(QuantRows& a, int heads, int64_t& blocks) {
-  const int items = a.dim / kItem;
+// token, `items` threads a row.  Few tokens: all threads of a workgroup, for
+// latency.
+int rows_grid(QuantRows& a, int heads, int items, int64_t& blocks) {
   a.slots = kRowThreads / items;
+  if (a.tokens * items * a.slots >= kManyRowThreads) a.slots = items < kWave / 2 ? kWave / 2 / items : 1;
   a.slots = a.slots < heads ? a.slots : heads;
   a.per_block = kRowThreads / (items * a.slots);
   blocks = (a.tokens + a.per_block - 1) / a.per_block;
@@ -800,11 +859,24 @@ extern "C" int rkv_quantized_append(const rkv_quantized_cache* cache, const void
   a.rates = rates;
   a.scale = scale;
   int64_t blocks;
-  rc = rows_grid(a, a.q_heads + 2 * a.heads, blocks);
+  const bool halves = !a.interleaved && rotary_dim == cache->dim && rotary_dim / 2 % kGroupDims == 0;
+  rc = rows_grid(a, a.q_heads + 2 * a.heads, a.dim / (halves ? 2 * kItem : kItem), blocks);
   if (rc) return rc;
   const dim3 grid((unsigned)blocks), threads(kRowThreads);
-  if (cache->dtype == RKV_F16) quantize_rows_kernel<_Float16><<<grid, threads, 0, stream>>>(a);
-  else quantize_rows_kernel<__bf16><<<grid, threads, 0, stream>>>(a);
+  const bool half = cache->dtype == RKV_F16;
+  if (halves) {
+    if (half) quantize_rows_kernel<_Float16, kHalves><<<grid, threads, 0, stream>>>(a);
+    else quantize_rows_kernel<__bf16, kHalves><<<grid, threads, 0, stream>>>(a);
+  } else if (a.interleaved || rotary_dim == 0) {
+    if (half) quantize_rows_kernel<_Float16, kWithin><<<grid, threads, 0, stream>>>(a);
+    else quantize_rows_kernel<__bf16, kWithin><<<grid, threads, 0, stream>>>(a);
+  } else if (rotary_dim / 2 % kItem == 0) {
+    if (half) quantize_rows_kernel<_Float16, kWhole><<<grid, threads, 0, stream>>>(a);
+    else quantize_rows_kernel<__bf16, kWhole><<<grid, threads, 0, stream>>>(a);
+  } else {
+    if (half) quantize_rows_kernel<_Float16, kParts><<<grid, threads, 0, stream>>>(a);
+    else quantize_rows_kernel<__bf16, kParts><<<grid, threads, 0, stream>>>(a);
+  }
   return check_launch("quantize_rows_kernel");
 }
 
@@ -830,7 +902,7 @@ extern "C" int rkv_quantized_read(const rkv_quantized_cache* cache, int64_t toke
   a.dst[1] = static_cast<char*>(key_out);
   a.dst[2] = static_cast<char*>(value_out);
   int64_t blocks;
-  rc = rows_grid(a, 2 * a.heads, blocks);
+  rc = rows_grid(a, 2 * a.heads, a.dim / kItem, blocks);
   if (rc) return rc;
   const dim3 grid((unsigned)blocks), threads(kRowThreads);
   if (cache->dtype == RKV_F16) quantized_read_kernel<_Float16><<<grid, threads, 0, stream>>>(a);
