@@ -51,7 +51,7 @@ struct PagedArgs : WalkArgs {
 template <int D, bool kHalf_, bool kScores>
 struct Pages16 {
   static constexpr int kDim = D;
-  static constexpr bool kHalf = kHalf_, kHalfWeights = kHalf_;
+  static constexpr bool kHalf = kHalf_, kScaleLate = false, kRareEnds = false;
   using Args = PagedArgs;
   using T = Type16<kHalf>;
   using V8 = typename T::V8;
@@ -342,14 +342,15 @@ int paged_decode(const char* who, const rkv_paged_cache* cache, const void* quer
   a.v_ts = (uint32_t)(cache->value_token_stride * 2);
   const dim3 grid((unsigned)P.grid), join((unsigned)P.grid, (unsigned)group);
   const bool plain = !scores_any(scores);
+  const size_t parts = part_bytes(group, cache->dim);
   RKV_DISPATCH_DIM(cache->dim, D, {
     if (cache->dtype == RKV_F16) {
-      if (plain) paged_kernel<D, true, false><<<grid, dim3(kThreads), 0, stream>>>(a);
-      else paged_kernel<D, true, true><<<grid, dim3(kThreads), 0, stream>>>(a);
+      if (plain) paged_kernel<D, true, false><<<grid, dim3(kThreads), parts, stream>>>(a);
+      else paged_kernel<D, true, true><<<grid, dim3(kThreads), parts, stream>>>(a);
       paged_join_kernel<D, true><<<join, dim3(kJoinThreads), 0, stream>>>(a);
     } else {
-      if (plain) paged_kernel<D, false, false><<<grid, dim3(kThreads), 0, stream>>>(a);
-      else paged_kernel<D, false, true><<<grid, dim3(kThreads), 0, stream>>>(a);
+      if (plain) paged_kernel<D, false, false><<<grid, dim3(kThreads), parts, stream>>>(a);
+      else paged_kernel<D, false, true><<<grid, dim3(kThreads), parts, stream>>>(a);
       paged_join_kernel<D, false><<<join, dim3(kJoinThreads), 0, stream>>>(a);
     }
   });

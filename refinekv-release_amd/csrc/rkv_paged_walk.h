@@ -188,13 +188,6 @@ __device__ __forceinline__ void next_tile(const WalkArgs& a, Cursor& c) {
   }
 }
 
-// A wave's results of a row that it does not hold whole.
-template <int D>
-struct Part {
-  float acc[kMaxGroup][D];
-  float2 ml[kMaxGroup];
-};
-
 struct PartHead {
   int row;              // -1: unused
   int begins, ends;     // the row's first / last tile is in the wave
@@ -282,7 +275,11 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
   using E = typename Type16<Store::kHalf>::E;
   using P = Pieces<D>;
   using Tile = typename Store::Tile;
-  __shared__ alignas(16) Part<D> parts[kWaves][2];
+  // a wave's results of rows that it does not hold whole: [wave][0: the row
+  // began before, 1: it begins here]
+  extern __shared__ float4 lds[];
+  float* const part_acc = reinterpret_cast<float*>(lds);  // [part][group][D]
+  float2* const part_ml = reinterpret_cast<float2*>(part_acc + kWaves * 2 * a.group * D);
   __shared__ PartHead heads_s[kWaves][2];
   __shared__ float weight_s[kMaxGroup][16];
   __shared__ float2 total_s[kMaxGroup];
@@ -388,12 +385,12 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] -= slope * (float)(behind - 1 - token(e));
           }
-        } else {
-          const float by = store.unit(q) * a.scale;
+        } else if constexpr (!Store::kScaleLate) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= by;
+          for (int e = 0; e < 8; ++e) x[e] *= a.scale;
         }
         if (behind < kTileTokens) {
+          if constexpr (Store::kRareEnds) asm volatile("");
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = token(e) < behind ? x[e] : kNegInf;
         }
@@ -409,6 +406,10 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
         top = __builtin_fmaxf(u, w);
         xor32_pair(top, u, w);
         top = __builtin_fmaxf(u, w);
+        // (kScaleLate: the scores are multiplied on the way into the exponential)
+        constexpr bool kLate = Store::kScaleLate && !kScores;
+        const float late = kLate ? store.unit(q) * a.scale : 1.0f;
+        if constexpr (kLate) top *= late;
         if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
           const float mn = __builtin_fmaxf(m, top);
           const float by = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -424,7 +425,10 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
           // (fp16 weights go up to 2^15 instead of 1, and the sum with them, so
           // that those of 2^-24 to 2^-39 of the largest, many in a long
           // context, do not round to zero)
-          p[e] = __builtin_amdgcn_exp2f(x[e] - base) * (Store::kHalfWeights ? 32768.0f : 1.0f);
+          if constexpr (Store::kScaleLate)
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], late, 15.0f - base));
+          else
+            p[e] = __builtin_amdgcn_exp2f(x[e] - base) * (Store::kHalf ? 32768.0f : 1.0f);
           l += p[e];
         }
         store.products(acc, t, p, from, behind);
@@ -457,14 +461,14 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
         return;
       }
       const int slot = begun ? 1 : 0;
-      Part<D>& part = parts[wave][slot];
+      const int part = (wave * 2 + slot) * a.group;
       if (lane == 0) {
         const uint32_t first = (uint32_t)first_tile<kScores>(c);
         heads_s[wave][slot] = PartHead{row, begun, ends, pos - ((uint32_t)c.tile - first),
                                        (uint32_t)c.tiles - first};
       }
       if (li < a.group) {
-        if (lg == 0) part.ml[li] = make_float2(m, sum_l);
+        if (lg == 0) part_ml[part + li] = make_float2(m, sum_l);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           P::each(4 * lg + r, [&](int n0, int d, auto size) {
@@ -475,7 +479,7 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
               FN y;
 #pragma unroll
               for (int j = 0; j < kN; ++j) y[j] = acc[n0 + i + j][r];
-              *reinterpret_cast<FN*>(&part.acc[li][d + i]) = y;
+              *reinterpret_cast<FN*>(&part_acc[(part + li) * D + d + i]) = y;
             }
           });
       }
@@ -535,7 +539,8 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
     for (int at = tid; at < kMaxGroup * 16; at += kThreads) {
       const int g = at / 16, i = at % 16;
       const bool in = same >> i & 1;
-      const float2 ml = in ? parts[i / 2][i % 2].ml[g] : make_float2(kNegInf, 0.0f);
+      const float2 ml =
+          in && g < a.group ? part_ml[i * a.group + g] : make_float2(kNegInf, 0.0f);
       float M = ml.x;
       M = __builtin_fmaxf(M, row_ror<8>(M));
       M = __builtin_fmaxf(M, row_ror<4>(M));
@@ -554,7 +559,7 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
 #pragma unroll 4
       for (int i = first; i < end; ++i) {
         const float w = weight_s[g][i];
-        const F32x4 p = *reinterpret_cast<const F32x4*>(&parts[i / 2][i % 2].acc[g][d]);
+        const F32x4 p = *reinterpret_cast<const F32x4*>(&part_acc[(i * a.group + g) * D + d]);
         // (a part that is not the row's holds anything)
         o += same >> i & 1 ? p * w : F32x4{0.0f, 0.0f, 0.0f, 0.0f};
       }
@@ -652,6 +657,11 @@ PagedPlan plan_of(int grid, int64_t group, int64_t dim) {
   P.acc_off = P.ml_off + up(parts * group * sizeof(float2));
   P.total = P.acc_off + up(parts * group * dim * sizeof(float));
   return P;
+}
+
+// Bytes of LDS that the walk's parts take.
+size_t part_bytes(int64_t group, int64_t dim) {
+  return (size_t)(kWaves * 2 * group) * (dim * sizeof(float) + sizeof(float2));
 }
 
 // The parts of a call's arguments that do not depend on how the cache holds its

@@ -385,37 +385,50 @@ struct QuantArgs : WalkArgs {
   const char* value_scales;
 };
 
+// Cache policy of the loads of codes and scales: non-temporal, as a token is
+// read once a step (8 x 131072 tokens 258 -> 254 us, 64 ragged ones 57.2 -> 55.9).
+constexpr int kStreamCodes = 2;
+
 // N dwords from consecutive places of a view.
 template <int N>
 __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t view, uint32_t at,
                                            uint32_t (&w)[N]) {
 #pragma unroll
   for (int i = 0; i + 4 <= N; i += 4) {
-    const U32x4 v = __builtin_amdgcn_raw_buffer_load_b128(view, (int)(at + 4u * i), 0, 0);
+    const U32x4 v = __builtin_amdgcn_raw_buffer_load_b128(view, (int)(at + 4u * i), 0, kStreamCodes);
 #pragma unroll
     for (int j = 0; j < 4; ++j) w[i + j] = v[j];
   }
   constexpr int kDone = N / 4 * 4;
   if constexpr (N % 4 == 3) {
-    const U32x3 v = __builtin_amdgcn_raw_buffer_load_b96(view, (int)(at + 4u * kDone), 0, 0);
+    const U32x3 v = __builtin_amdgcn_raw_buffer_load_b96(view, (int)(at + 4u * kDone), 0, kStreamCodes);
 #pragma unroll
     for (int j = 0; j < 3; ++j) w[kDone + j] = v[j];
   } else if constexpr (N % 4 == 2) {
-    const U32x2 v = __builtin_amdgcn_raw_buffer_load_b64(view, (int)(at + 4u * kDone), 0, 0);
+    const U32x2 v = __builtin_amdgcn_raw_buffer_load_b64(view, (int)(at + 4u * kDone), 0, kStreamCodes);
     w[kDone] = v[0];
     w[kDone + 1] = v[1];
   } else if constexpr (N % 4 == 1) {
-    w[kDone] = __builtin_amdgcn_raw_buffer_load_b32(view, (int)(at + 4u * kDone), 0, 0);
+    w[kDone] = __builtin_amdgcn_raw_buffer_load_b32(view, (int)(at + 4u * kDone), 0, kStreamCodes);
   }
 }
 
 // Entry m of 4 that a word holds: the two codes as fp16 numbers 64 + code (in
 // fp16, 64 + code / 16 times 16 units of the last bit: the code shifted to
 // bits 4 .. 7 of 64).
+// Mask and 64 come in registers: as literals they take an instruction each.
+struct CodeBits {
+  uint32_t mask = 0x00f000f0u, sixty_four = 0x54005400u;
+  __device__ __forceinline__ CodeBits() {
+    asm volatile("" : "+s"(mask));
+    asm volatile("" : "+v"(sixty_four));
+  }
+};
+
 template <int M>
-__device__ __forceinline__ Half2 codes_of(uint32_t w) {
+__device__ __forceinline__ Half2 codes_of(const CodeBits& bits, uint32_t w) {
   const uint32_t at = M == 0 ? w << 4 : w >> (4 * M - 4);
-  return half2_of((at & 0x00f000f0u) | 0x54005400u);
+  return half2_of((at & bits.mask) | bits.sixty_four);
 }
 
 // The walk's operands from 4-bit pages.  All products run on fp16: a code times
@@ -428,7 +441,8 @@ __device__ __forceinline__ Half2 codes_of(uint32_t w) {
 template <int D, bool kHalf_, bool kScores>
 struct Pages4 {
   static constexpr int kDim = D;
-  static constexpr bool kHalf = kHalf_, kHalfWeights = true;
+  // (kRareEnds: a row's last tile is a branch, not selects in every tile)
+  static constexpr bool kHalf = kHalf_, kScaleLate = true, kRareEnds = true;
   using Args = QuantArgs;
   using P = Pieces<D>;
   static constexpr int G = D / kGroupDims;
@@ -448,6 +462,7 @@ struct Pages4 {
 
   const Args& a;
   const int li, lg;
+  const CodeBits bits;
   __device__ __forceinline__ Pages4(const Args& args, int li_, int lg_)
       : a(args), li(li_), lg(lg_) {}
 
@@ -470,7 +485,9 @@ struct Pages4 {
     top = __builtin_fmaxf(u, v);
     uint32_t e2 = f32_bits(top) >> 23;
     e2 = e2 < 1u ? 1u : e2 > 253u ? 253u : e2;
-    const float by = bits_f32((254u - e2) << 23);  // 2^(127 - e2)
+    float by = bits_f32((254u - e2) << 23);  // 2^(127 - e2)
+    // (scores that are scaled late are scaled by a magnitude)
+    if constexpr (!kScores) by = a.scale < 0.0f ? -by : by;
     q.back = bits_f32(e2 << 23);
     q.sums = Half8{};
 #pragma unroll
@@ -492,7 +509,9 @@ struct Pages4 {
       q.sums[j] = lg == 0 ? high : lg == 1 ? mid : lg == 2 ? low : (_Float16)0.0f;
     }
   }
-  static __device__ __forceinline__ float unit(const Query& q) { return q.back; }
+  __device__ __forceinline__ float unit(const Query& q) const {
+    return !kScores && a.scale < 0.0f ? -q.back : q.back;
+  }
 
   // A row's zeros' share joins its accumulators.
   static __device__ __forceinline__ void finish(F32x4 (&acc)[kAccs]) {
@@ -559,7 +578,7 @@ struct Pages4 {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(Half8, x), y, z, 0, 0, 0);
   }
 
-  static __device__ __forceinline__ void scores(const Query& q, const Tile& t, float (&x)[8]) {
+  __device__ __forceinline__ void scores(const Query& q, const Tile& t, float (&x)[8]) const {
     const Half2 down = {(_Float16)-64.0f, (_Float16)-64.0f};
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -570,10 +589,10 @@ struct Pages4 {
         const uint32_t sz = t.ks[s][j], w = t.kc[s][j];
         const Half2 step = half2_of(__builtin_amdgcn_perm(sz, sz, 0x01000100u));
         const Half2 base = step * down;
-        const U32x4 k = {word_of(__builtin_elementwise_fma(codes_of<0>(w), step, base)),
-                         word_of(__builtin_elementwise_fma(codes_of<1>(w), step, base)),
-                         word_of(__builtin_elementwise_fma(codes_of<2>(w), step, base)),
-                         word_of(__builtin_elementwise_fma(codes_of<3>(w), step, base))};
+        const U32x4 k = {word_of(__builtin_elementwise_fma(codes_of<0>(bits, w), step, base)),
+                         word_of(__builtin_elementwise_fma(codes_of<1>(bits, w), step, base)),
+                         word_of(__builtin_elementwise_fma(codes_of<2>(bits, w), step, base)),
+                         word_of(__builtin_elementwise_fma(codes_of<3>(bits, w), step, base))};
         s4 = mma(k, q.q[j], s4);
         zeros[j / 2] |= j % 2 ? sz & 0xffff0000u : sz >> 16;
       }
@@ -596,6 +615,7 @@ struct Pages4 {
     }
     if (behind < kTileTokens || (kScores && from > 0)) {
       // hidden tokens' scales may be anything, NaN as well: zeros here
+      asm volatile("");
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -634,10 +654,10 @@ struct Pages4 {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           constexpr int m0 = n, m1 = E + n;
-          words[2 * s] = word_of(__builtin_elementwise_fma(codes_of<m0 % 4>(t.vc[s][w0 + m0 / 4]),
+          words[2 * s] = word_of(__builtin_elementwise_fma(codes_of<m0 % 4>(bits, t.vc[s][w0 + m0 / 4]),
                                                            step[2 * s], base[2 * s]));
           words[2 * s + 1] = word_of(__builtin_elementwise_fma(
-              codes_of<m1 % 4>(t.vc[s][w0 + m1 / 4]), step[2 * s + 1], base[2 * s + 1]));
+              codes_of<m1 % 4>(bits, t.vc[s][w0 + m1 / 4]), step[2 * s + 1], base[2 * s + 1]));
         }
         add(n0 + n, words);
       };
@@ -663,12 +683,16 @@ struct Pages4 {
   }
 };
 
+// Workgroups per CU that share the tiles (as kPerCu): from two to three at head_dim
+// 64, 48 sequences of up to 16000 tokens, 64.2 -> 55.5 us; 96, 40 of them, 31.0
+// -> 36.7; 128, 64 ragged ones 53.6 -> 60.4; from one to two at 256, 24 of up to
+// 12000, 45.6 -> 54.0.
 template <int D>
-constexpr int kPerCu4 = D <= 128 ? 2 : 1;
+constexpr int kPerCu4 = D <= 64 ? 3 : D <= 128 ? 2 : 1;
 
 template <int D, bool kHalf, bool kScores>
 __global__ __launch_bounds__(kThreads)
-__attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void quantized_kernel(QuantArgs a) {
+__attribute__((amdgpu_waves_per_eu(kPerCu4<D>))) void quantized_kernel(QuantArgs a) {
   walk<Pages4<D, kHalf, kScores>, kScores>(a);
 }
 
@@ -946,15 +970,17 @@ extern "C" int rkv_quantized_decode(const rkv_quantized_cache* cache, const void
   a.value_codes = static_cast<const char*>(cache->value_codes);
   a.value_scales = static_cast<const char*>(cache->value_scales);
   const dim3 grid((unsigned)P.grid), join((unsigned)P.grid, (unsigned)group);
-  const bool plain = !scores_any(scores);
+  // (a scale of 0 times a hidden score would be NaN where scores are scaled late)
+  const bool plain = !scores_any(scores) && a.scale != 0.0f;
+  const size_t parts = part_bytes(group, cache->dim);
   RKV_DISPATCH_DIM(cache->dim, D, {
     if (cache->dtype == RKV_F16) {
-      if (plain) quantized_kernel<D, true, false><<<grid, dim3(kThreads), 0, stream>>>(a);
-      else quantized_kernel<D, true, true><<<grid, dim3(kThreads), 0, stream>>>(a);
+      if (plain) quantized_kernel<D, true, false><<<grid, dim3(kThreads), parts, stream>>>(a);
+      else quantized_kernel<D, true, true><<<grid, dim3(kThreads), parts, stream>>>(a);
       paged_join_kernel<D, true><<<join, dim3(kJoinThreads), 0, stream>>>(a);
     } else {
-      if (plain) quantized_kernel<D, false, false><<<grid, dim3(kThreads), 0, stream>>>(a);
-      else quantized_kernel<D, false, true><<<grid, dim3(kThreads), 0, stream>>>(a);
+      if (plain) quantized_kernel<D, false, false><<<grid, dim3(kThreads), parts, stream>>>(a);
+      else quantized_kernel<D, false, true><<<grid, dim3(kThreads), parts, stream>>>(a);
       paged_join_kernel<D, false><<<join, dim3(kJoinThreads), 0, stream>>>(a);
     }
   });
