@@ -52,8 +52,10 @@ struct PromptArgs {
   char* out;                   // (tokens, H G, D) dense
   int zero_rest;               // rows of no sequence become zeros (else: as they were)
   int tiles;                   // at most so many in the grid
-  int splits;                  // workgroups that share a tile's keys
-  float2* part_ml;             // [splits][tokens H G] (splits > 1)
+  // few tiles: so many workgroups share all tiles' keys (0: each has a tile of
+  // its own); keys are counted in units of 2^unit LDS tiles
+  int shares, unit;
+  float2* part_ml;             // [workgroup][kTileRows]
   float* part_acc;             // [..][D]
 };
 
@@ -98,34 +100,141 @@ __device__ __forceinline__ uint32_t tiles_for(const PromptArgs& a, int count) {
   return (uint32_t)(((int64_t)count * a.group + kTileRows - 1) / kTileRows);
 }
 
-// The slot-th of the tiles, the last ones of the last sequence first: a
-// sequence's later tiles have more keys.  False: there are fewer.
-__device__ __forceinline__ bool find_tile(const PromptArgs& a, uint32_t slot, PromptRows& r) {
+// A sequence's keys: their number (0, and `bad`, for a length past its table)
+// and, of rows, the first one.
+__device__ __forceinline__ int keys_of(const PromptArgs& a, const PromptRows& r, int& first,
+                                       bool& bad) {
+  first = 0;
+  bad = false;
+  if (a.table) {
+    const int n = a.lengths[r.b];
+    bad = n > 0 && (n - 1) >> a.shift >= a.max_blocks;
+    return bad || n < 0 ? 0 : n;
+  }
+  if (a.key_starts) {
+    first = min(max(a.key_starts[r.b], 0), a.key_tokens);
+    return min(max(a.key_starts[r.b + 1], first), a.key_tokens) - first;
+  }
+  first = r.first;
+  return r.count;
+}
+
+// The slot-th of the entries that the sequences have `entries(b)` of, with its
+// sequence and its place among that one's entries.  False: there are fewer.
+template <typename Entries>
+__device__ __forceinline__ bool find_entry(const PromptArgs& a, uint32_t slot, bool from_end,
+                                           Entries entries, int& b, uint32_t& place) {
   const int lane = threadIdx.x % kWave;
   const int per = (a.sequences + kWave - 1) / kWave;
   uint32_t sum = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = lane * per + i;
-    if (b >= a.sequences) break;
-    int first, count;
-    rows_of(a, b, first, count);
-    sum += tiles_for(a, count);
-  }
+  for (int i = 0; i < per && lane * per + i < a.sequences; ++i) sum += entries(lane * per + i);
   const uint32_t upto = wave_scan(sum);
   const uint32_t total = (uint32_t)uniform((int)__shfl((int)upto, kWave - 1, kWave));
   if (slot >= total) return false;
-  const uint32_t at = total - 1u - slot;
+  const uint32_t at = from_end ? total - 1u - slot : slot;
   const int owner = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
-  uint32_t rest = at - (uint32_t)uniform(__shfl((int)(upto - sum), owner, kWave));
-  for (r.b = owner * per;; ++r.b) {
-    rows_of(a, r.b, r.first, r.count);
-    r.first = uniform(r.first);
-    r.count = uniform(r.count);
-    const uint32_t here = tiles_for(a, r.count);
-    if (rest < here || r.b + 1 >= a.sequences) break;
-    rest -= here;
+  place = at - (uint32_t)uniform(__shfl((int)(upto - sum), owner, kWave));
+  for (b = owner * per; b + 1 < a.sequences; ++b) {
+    const uint32_t here = (uint32_t)uniform((int)entries(b));
+    if (place < here) break;
+    place -= here;
   }
-  r.tile = (int)rest;
+  return true;
+}
+
+// The slot-th of the tiles, the last ones of the last sequence first: a
+// sequence's later tiles have more keys.
+__device__ __forceinline__ bool find_tile(const PromptArgs& a, uint32_t slot, PromptRows& r) {
+  uint32_t place;
+  auto tiles = [&](int b) {
+    int first, count;
+    rows_of(a, b, first, count);
+    return tiles_for(a, count);
+  };
+  if (!find_entry(a, slot, true, tiles, r.b, place)) return false;
+  rows_of(a, r.b, r.first, r.count);
+  r.first = uniform(r.first);
+  r.count = uniform(r.count);
+  r.tile = (int)place;
+  return true;
+}
+
+// A tile's part of its sequence's keys, for one head.
+struct Share {
+  int head, chunk, chunks;  // of the sequence's keys
+  int begin, end;           // LDS tiles of the chunk
+  int first, apart;         // the tile's first chunk among all shares, and from one to the next
+};
+
+// The sequence's range of LDS tiles with keys that its rows see, in units.
+template <int T>
+__device__ __forceinline__ uint32_t units_of(const PromptArgs& a, const PromptRows& r,
+                                             int& begin) {
+  int first;
+  bool bad;
+  const int length = keys_of(a, r, first, bad), at = max(length - r.count, 0);
+  begin = at >= a.window ? (at - a.window + 1) / T : 0;
+  const int tiles = (int)(((int64_t)length + T - 1) / T) - begin;
+  return tiles > 0 ? (uint32_t)(((int64_t)tiles + (1 << a.unit) - 1) >> a.unit) : 1u;
+}
+
+// Shares of few tiles' keys: chunks of so many units that all fit the grid
+// (rounding up costs a tile one chunk at most), 256 keys at least.  They lie
+// sequence by sequence, chunk by chunk, head by head, tile by tile: a chunk's
+// tiles are neighbours.  The slot-th of them, or (kJoin) the first of the slot-th
+// tile and head.
+template <int T, bool kJoin>
+__device__ __forceinline__ bool find_share(const PromptArgs& a, uint32_t slot, PromptRows& r,
+                                           Share& share) {
+  const int lane = threadIdx.x % kWave;
+  const int per = (a.sequences + kWave - 1) / kWave;
+  auto sizes = [&](int b, uint32_t& tiles, uint32_t& units, int& begin) {
+    PromptRows q;
+    q.b = b;
+    rows_of(a, b, q.first, q.count);
+    tiles = tiles_for(a, q.count);
+    units = tiles ? units_of<T>(a, q, begin) : 0u;
+  };
+  uint32_t sum = 0, tiles, units;
+  int begin = 0;
+  for (int i = 0; i < per && lane * per + i < a.sequences; ++i) {
+    sizes(lane * per + i, tiles, units, begin);
+    sum += tiles * units;
+  }
+  const uint32_t all = (uint32_t)uniform(
+      (int)__shfl((int)wave_scan(sum), kWave - 1, kWave));
+  const uint32_t heads = (uint32_t)a.heads, room = (uint32_t)a.shares - (uint32_t)a.tiles * heads;
+  const uint64_t need = ((uint64_t)all * heads + room - 1u) / room;
+  const uint32_t least = max(256 / T >> a.unit, 1);
+  const uint32_t chunk = need > least ? (uint32_t)need : least;
+  auto chunks_of = [&](uint32_t n) { return (n + chunk - 1u) / chunk; };
+  auto entries = [&](int b) {
+    sizes(b, tiles, units, begin);
+    return tiles * heads * (kJoin ? 1u : chunks_of(units));
+  };
+  uint32_t place;
+  if (!find_entry(a, slot, false, entries, r.b, place)) return false;
+  rows_of(a, r.b, r.first, r.count);
+  r.first = uniform(r.first);
+  r.count = uniform(r.count);
+  tiles = tiles_for(a, r.count);
+  units = (uint32_t)uniform((int)units_of<T>(a, r, begin));
+  r.tile = (int)(place % tiles);
+  share.head = (int)(place / tiles % heads);
+  share.chunk = (int)(place / tiles / heads);
+  share.chunks = (int)chunks_of(units);
+  share.apart = (int)(tiles * heads);
+  const int64_t from = ((int64_t)share.chunk * chunk << a.unit) + uniform(begin);
+  share.begin = (int)min(from, (int64_t)INT32_MAX);
+  share.end = (int)min(from + ((int64_t)chunk << a.unit), (int64_t)INT32_MAX);
+  if constexpr (kJoin) {
+    uint32_t before = 0;  // shares of the sequences before
+    for (int i = 0; i < per && lane * per + i < r.b; ++i) {
+      sizes(lane * per + i, tiles, units, begin);
+      before += tiles * heads * chunks_of(units);
+    }
+    share.first = uniform(__shfl((int)wave_scan(before), kWave - 1, kWave)) + (int)place;
+  }
   return true;
 }
 
@@ -187,32 +296,39 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
   constexpr int T = Tile::kTokens, kGroups = T / 16, kLoads = D / 32;
   constexpr int kOwn = T == 64 ? 2 : 1;  // tensors of which a wave loads 16 rows a tile
   constexpr int kMarks = (D / 32 + 1) / 2;
+  // Of the two waves of a SIMD the one in its products goes first, so that the
+  // other's softmax runs beside them (16384 tokens, head_dim 128, 2300 -> 2180 us);
+  // where the softmax takes longer it goes first (head_dim 64, 8192 tokens of 16
+  // heads, 218 -> 204 us).
+  constexpr bool kProductsFirst = D > 64;
   __shared__ alignas(16) char smem[2][Tile::kBytes];
   __shared__ uint32_t marks[2][kMarks][kPromptThreads];  // outputs that kUp and kDown found
-  const int head = (int)(blockIdx.x % (uint32_t)a.heads);
-  const uint32_t slot = blockIdx.x / (uint32_t)a.heads;
-  PromptRows rows;
-  if (!find_tile(a, slot, rows)) {
-    if (a.zero_rest && (int)slot == a.tiles && blockIdx.y == 0) zero_rows<D>(a, head);
+  const uint32_t last = gridDim.x - (a.zero_rest ? (uint32_t)a.heads : 0u);
+  if (blockIdx.x >= last) {
+    zero_rows<D>(a, (int)(blockIdx.x - last));
     return;
   }
+  PromptRows rows;
+  Share share{(int)(blockIdx.x % (uint32_t)a.heads), 0, 1, 0, INT32_MAX, 0, 0};
+  // A chunk's tiles go to one XCD (workgroups go to the 8 in turn), whose L2 then
+  // has the keys of the second from the first.
+  const uint32_t each = (uint32_t)a.shares / 8u;
+  const uint32_t slot = blockIdx.x < each * 8u ? blockIdx.x % 8u * each + blockIdx.x / 8u
+                                               : blockIdx.x;
+  if (!(a.shares ? find_share<T, false>(a, slot, rows, share)
+                 : find_tile(a, blockIdx.x / (uint32_t)a.heads, rows)))
+    return;
+  const int head = share.head;
   const int lane = threadIdx.x % kWave, wave = uniform((int)threadIdx.x / kWave);
   const int l32 = lane & 31, h = lane >> 5;
 
   // ---- the sequence's keys
-  int length, key_first = 0;
-  bool bad = false;
-  if (a.table) {
-    length = scalar_at(a.lengths, rows.b);
-    bad = length > 0 && (length - 1) >> a.shift >= a.max_blocks;
-    length = bad || length < 0 ? 0 : length;
-  } else if (a.key_starts) {
-    key_first = min(max(scalar_at(a.key_starts, rows.b), 0), a.key_tokens);
-    length = min(max(scalar_at(a.key_starts, rows.b + 1), key_first), a.key_tokens) - key_first;
-  } else {
-    key_first = rows.first;
-    length = rows.count;
-  }
+  int key_first;
+  bool bad;
+  int length = keys_of(a, rows, key_first, bad);
+  length = uniform(length);
+  key_first = uniform(key_first);
+  bad = uniform(bad);
   int prefix = a.prefix ? scalar_at(a.prefix, rows.b) : 0;
   prefix = min(max(prefix, 0), length);
 
@@ -244,12 +360,8 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
     whole_end = p0 < 0 ? 0 : max(p0 + 1, prefix);
     whole_begin = p1 >= a.window ? p1 - a.window + 1 : 0;
   }
-  int tile_begin = wg_begin / T, tile_end = (wg_end + T - 1) / T;
-  if (a.splits > 1) {
-    const int64_t n = max(tile_end - tile_begin, 0), s = blockIdx.y;
-    tile_end = tile_begin + (int)(n * (s + 1) / a.splits);
-    tile_begin += (int)(n * s / a.splits);
-  }
+  const int tile_begin = max(wg_begin / T, share.begin);
+  const int tile_end = min((int)(((int64_t)wg_end + T - 1) / T), share.end);
 
   // ---- the query rows
   U32x4 q[D / 16];
@@ -356,6 +468,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
       }
       const int t0 = tile * T;
       if (t0 < wave_end && t0 + T > wave_begin) {
+        __builtin_amdgcn_s_setprio(kProductsFirst ? 1 : 0);
         // ---- scores
         F32x16 s[T / 32];
 #pragma unroll
@@ -363,22 +476,42 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
 #pragma unroll
           for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
           const char* keys = buffer + (32 * u + l32) * Tile::kKeyRow + 16 * h;
+          // (4 reads ahead of the products)
+          constexpr int kAhead = 4;
+          U32x4 k[D / 16];
 #pragma unroll
-          for (int j = 0; j < D / 16; ++j)
-            s[u] = mma32<kHalf>(*reinterpret_cast<const U32x4*>(keys + 32 * j), q[j], s[u]);
+          for (int j = 0; j < D / 16; ++j) k[j] = *reinterpret_cast<const U32x4*>(keys + 32 * j);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) s[u] = mma32<kHalf>(k[j], q[j], s[u]);
+          __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            if (j + kAhead < D / 16) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
         }
+        __builtin_amdgcn_s_setprio(kProductsFirst ? 0 : 1);
         auto token = [&](int u, int i) { return t0 + 32 * u + 8 * (i / 4) + 4 * h + i % 4; };
         if constexpr (kScores) {
           const float by = a.cap > 0.0f ? a.per_cap : a.scale;
 #pragma unroll
-          for (int u = 0; u < T / 32; ++u)
+          for (int u = 0; u < T / 32; ++u) s[u] *= by;
+          if (a.cap > 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float x = s[u][i] * by;
-              if (a.cap > 0.0f) x = tanh_hw(x) * a.cap;
-              if (a.slopes) x -= slope * __builtin_fabsf((float)(pos - token(u, i)));
-              s[u][i] = x;
-            }
+            for (int u = 0; u < T / 32; ++u)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[u][i] = tanh_hw(s[u][i]) * a.cap;
+          }
+          if (a.slopes) {
+            // the distances of a lane's keys from that of its first
+            const float far = (float)(pos - token(0, 0));
+#pragma unroll
+            for (int u = 0; u < T / 32; ++u)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                s[u][i] = __builtin_fmaf(
+                    -slope, __builtin_fabsf(far - (float)(32 * u + 8 * (i / 4) + i % 4)), s[u][i]);
+          }
         }
         const float scale = kScores ? 1.0f : a.scale;
         if (t0 + T > whole_end || t0 < whole_begin) {
@@ -435,6 +568,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
               p[2 * u + i / 8][i % 8 / 2] = (seen(i) ? kOne : 0u) | (seen(i + 1) ? kOne << 16 : 0u);
             }
         }
+        __builtin_amdgcn_s_setprio(kProductsFirst ? 1 : 0);
         // ---- products
         const int l16 = lane & 15;
         const char* values = buffer + Tile::kValueAt + (4 * h + l16 / 4) * Tile::kValueRow +
@@ -455,6 +589,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
             }
             acc[n] = mma32<kHalf>(v, p[c], acc[n]);
           }
+        __builtin_amdgcn_s_setprio(0);
       }
       if (more) store(smem[(tile + 1 - tile_begin) & 1]);
       __syncthreads();
@@ -500,8 +635,8 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
   if (!mine) return;
   if (bad) l = __builtin_nanf("");
   const int64_t row = (int64_t)(rows.first + in_seq) * (a.heads * a.group) + head * a.group + g;
-  if (a.splits > 1) {
-    const int64_t at = (int64_t)blockIdx.y * a.tokens * (a.heads * a.group) + row;
+  if (share.chunks > 1) {
+    const int64_t at = (int64_t)slot * kTileRows + (pair - pair0);
     float* to = a.part_acc + at * D + 4 * h;
 #pragma unroll
     for (int n = 0; n < D / 32; ++n)
@@ -526,17 +661,19 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
     }
 }
 
-// Joins the parts of a tile's rows, each D / 4 threads one row at a time.
+// Joins the parts of a tile's rows: workgroup (tile and head, y) every
+// gridDim.y-th 256 / (D / 4) of them, D / 4 threads a row.
 template <int D, bool kHalf>
 __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs a) {
   using E = typename Type16<kHalf>::E;
   constexpr int kAcross = D / 4, kRows = kPromptThreads / kAcross;
-  const int head = (int)(blockIdx.x % (uint32_t)a.heads);
   PromptRows rows;
-  if (!find_tile(a, blockIdx.x / (uint32_t)a.heads, rows)) return;
+  Share share;
+  if (!find_share<PromptTile<D>::kTokens, true>(a, blockIdx.x, rows, share) || share.chunks == 1)
+    return;
+  const int head = share.head;
   const int c = (int)threadIdx.x % kAcross, in = (int)threadIdx.x / kAcross;
   const int pairs = min(rows.count * a.group - rows.tile * kTileRows, kTileRows);
-  const int64_t all = (int64_t)a.tokens * (a.heads * a.group);
   for (int i = (int)blockIdx.y * kRows + in; in < kRows && i < pairs;
        i += kRows * (int)gridDim.y) {
     const int pair = rows.tile * kTileRows + i;
@@ -544,10 +681,13 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
                         head * a.group + pair % a.group;
     float m = kNegInf, l = 0.0f;
     F32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    fold_parts(0u, 1u, (uint32_t)a.splits, m, l, o,
-               [&](uint32_t j) { return a.part_ml[j * all + row]; },
+    auto part_at = [&](uint32_t j) {
+      return ((int64_t)share.first + (int64_t)j * share.apart) * kTileRows + i;
+    };
+    fold_parts(0u, 1u, (uint32_t)share.chunks, m, l, o,
+               [&](uint32_t j) { return a.part_ml[part_at(j)]; },
                [&](uint32_t j) {
-                 return *reinterpret_cast<const float4*>(a.part_acc + (j * all + row) * D + 4 * c);
+                 return *reinterpret_cast<const float4*>(a.part_acc + part_at(j) * D + 4 * c);
                });
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     typedef E E4 __attribute__((ext_vector_type(4)));
@@ -559,26 +699,25 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
 }
 
 struct PromptPlan {
-  int tiles = 0, splits = 1;
+  int tiles = 0, shares = 0, unit = 0;
   size_t acc_off = 0, total = 0;
 };
 
-// Tiles: at most those of all rows together and one more a sequence.  Few
-// tiles share their keys out until the device has two workgroups a CU, 256 keys
-// each at least.
+// Tiles: at most those of all rows together and one more a sequence.  Where
+// they leave half of the workgroups that the device holds at a time (two a CU)
+// idle, that many share the tiles' keys.
 PromptPlan prompt_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t group, int64_t dim,
                        int64_t most_keys) {
   PromptPlan P;
   const int64_t some = tokens < sequences ? tokens : sequences;
   P.tiles = (int)(tokens * group / kTileRows + some);
-  const int64_t blocks = P.tiles * heads, want = 2 * compute_units();
-  int64_t splits = blocks > 0 && blocks < want ? want / blocks : 1;
-  const int64_t most = (most_keys + 255) / 256;
-  splits = splits < most ? splits : most;
-  P.splits = (int)(splits > 1 ? splits : 1);
-  if (P.splits > 1) {
-    const size_t rows = (size_t)(tokens * heads * group) * P.splits;
-    P.acc_off = (rows * sizeof(float2) + 255) & ~(size_t)255;
+  const int64_t want = 2 * compute_units();
+  if (P.tiles > 0 && P.tiles * heads * 2 <= want && most_keys > 256) {
+    P.shares = (int)want;
+    // (tiles times units are summed in 32 bits)
+    while ((most_keys / 32 >> P.unit) + 2 > ((int64_t(1) << 32) - 1) / want) ++P.unit;
+    const size_t rows = (size_t)want * kTileRows;
+    P.acc_off = rows * sizeof(float2);
     P.total = P.acc_off + rows * dim * sizeof(float);
   }
   return P;
@@ -646,20 +785,23 @@ int prompt(const char* who, PromptArgs& a, int dtype, int64_t tokens, int64_t se
   a.out = static_cast<char*>(output);
   a.zero_rest = zero_rest;
   a.tiles = P.tiles;
-  a.splits = P.splits;
+  a.shares = P.shares;
+  a.unit = P.unit;
   // (a window alone changes no score; a scale of 0 times a hidden score would)
   const bool plain = !(a.cap > 0.0f) && !a.slopes && a.scale > 0.0f && a.scale < kPosInf;
-  const dim3 grid((unsigned)((P.tiles + (zero_rest ? 1 : 0)) * heads), (unsigned)P.splits);
-  const dim3 join((unsigned)(P.tiles * heads), 8), threads(kPromptThreads);
+  const int64_t blocks = P.shares ? P.shares : P.tiles * heads;
+  // (the last `heads` workgroups: rows of no sequence)
+  const dim3 grid((unsigned)(blocks + (zero_rest ? heads : 0)));
+  const dim3 join((unsigned)(P.tiles * heads), 16), threads(kPromptThreads);
   RKV_DISPATCH_DIM(dim, D, {
     if (dtype == RKV_F16) {
       if (plain) prompt_kernel<D, true, false><<<grid, threads, 0, stream>>>(a);
       else prompt_kernel<D, true, true><<<grid, threads, 0, stream>>>(a);
-      if (P.splits > 1) prompt_join_kernel<D, true><<<join, threads, 0, stream>>>(a);
+      if (P.shares) prompt_join_kernel<D, true><<<join, threads, 0, stream>>>(a);
     } else {
       if (plain) prompt_kernel<D, false, false><<<grid, threads, 0, stream>>>(a);
       else prompt_kernel<D, false, true><<<grid, threads, 0, stream>>>(a);
-      if (P.splits > 1) prompt_join_kernel<D, false><<<join, threads, 0, stream>>>(a);
+      if (P.shares) prompt_join_kernel<D, false><<<join, threads, 0, stream>>>(a);
     }
   });
   return check_launch("prompt_kernel");
