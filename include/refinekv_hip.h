@@ -337,7 +337,7 @@ int rkv_paged_read(const rkv_paged_cache* cache, int64_t tokens, const int32_t* 
 
 /* What an attention's scores are besides scaled products x = scale q . k, in
  * this order; NULL, or all fields 0, for nothing:
- *   softcap > 0:  softcap * tanh(x / softcap);
+ *   softcap > 0:  softcap * tanh(x / softcap), 1e-30..1e30;
  *   slopes:       fp32 per query head (device, 4-byte aligned), x - slope *
  *                 |position of q - position of k|;
  *   window > 0:   a query sees the last `window` tokens up to its own. */

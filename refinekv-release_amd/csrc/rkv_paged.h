@@ -127,8 +127,8 @@ inline int scores_window(const rkv_scores* s) {
 
 inline int check_scores(const char* who, const rkv_scores* s) {
   if (!s) return kOk;
-  if (!(s->softcap >= 0.0f) || s->softcap > 3.0e38f)
-    return set_error(kInvalidArgument, "%s: softcap must be finite, and 0 for none", who);
+  if (s->softcap != 0.0f && !(s->softcap >= 1e-30f && s->softcap <= 1e30f))
+    return set_error(kInvalidArgument, "%s: softcap must be in 1e-30..1e30, or 0 for none", who);
   if (s->window < 0) return set_error(kInvalidArgument, "%s: negative window", who);
   if (!aligned(s->slopes, 4)) return set_error(kInvalidArgument, "%s: unaligned slopes", who);
   return kOk;

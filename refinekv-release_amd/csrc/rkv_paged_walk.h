@@ -408,7 +408,9 @@ __device__ __forceinline__ void walk(const typename Store::Args& a) {
         top = __builtin_fmaxf(u, w);
         // (kScaleLate: the scores are multiplied on the way into the exponential)
         constexpr bool kLate = Store::kScaleLate && !kScores;
-        const float late = kLate ? store.unit(q) * a.scale : 1.0f;
+        // (never 0: a hidden score times it would be NaN)
+        const float late =
+            kLate ? __builtin_fmaxf(store.unit(q) * a.scale, __FLT_MIN__) : 1.0f;
         if constexpr (kLate) top *= late;
         if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
           const float mn = __builtin_fmaxf(m, top);

@@ -671,6 +671,8 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
   Share share;
   if (!find_share<PromptTile<D>::kTokens, true>(a, blockIdx.x, rows, share) || share.chunks == 1)
     return;
+  // (starts that overlap ask for more shares than there are)
+  if ((int64_t)share.first + (int64_t)(share.chunks - 1) * share.apart >= a.shares) return;
   const int head = share.head;
   const int c = (int)threadIdx.x % kAcross, in = (int)threadIdx.x / kAcross;
   const int pairs = min(rows.count * a.group - rows.tile * kTileRows, kTileRows);
@@ -697,6 +699,9 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
     *reinterpret_cast<E4*>(a.out + (row * D + 4 * c) * 2) = v;
   }
 }
+
+// Keys of a sequence: their numbers, and those of two tiles behind them, are ints.
+constexpr int64_t kMostKeys = (int64_t(1) << 31) - 512;
 
 struct PromptPlan {
   int tiles = 0, shares = 0, unit = 0;
@@ -837,8 +842,7 @@ extern "C" int rkv_prompt_attention(const void* query, int64_t q_token_stride,
   clear_error();
   int rc = check_prompt(who, dtype, tokens, sequences, heads, group, dim);
   if (rc) return rc;
-  const int64_t lim = (int64_t(1) << 31) - 1;
-  if (key_tokens < 0 || key_tokens > lim)
+  if (key_tokens < 0 || key_tokens > kMostKeys)
     return set_error(kInvalidArgument, "%s: bad key count", who);
   if (!token_starts && (sequences != 1 || key_starts))
     return set_error(kInvalidArgument, "%s: several sequences need token_starts", who);
@@ -889,6 +893,8 @@ extern "C" int rkv_paged_prompt(const rkv_paged_cache* cache, const void* query,
   if (rc) return rc;
   if (!token_starts && tokens != cache->sequences)
     return set_error(kInvalidArgument, "%s: without token_starts one token per sequence", who);
+  if (cache->max_blocks * cache->page_size > kMostKeys)
+    return set_error(kUnsupported, "%s: the block table covers too many tokens", who);
   PromptArgs a{};
   a.k_ps = read_stride(cache->key_page_stride, cache->pages);
   a.k_hs = read_stride(cache->key_head_stride, cache->heads);

@@ -970,8 +970,8 @@ extern "C" int rkv_quantized_decode(const rkv_quantized_cache* cache, const void
   a.value_codes = static_cast<const char*>(cache->value_codes);
   a.value_scales = static_cast<const char*>(cache->value_scales);
   const dim3 grid((unsigned)P.grid), join((unsigned)P.grid, (unsigned)group);
-  // (a scale of 0 times a hidden score would be NaN where scores are scaled late)
-  const bool plain = !scores_any(scores) && a.scale != 0.0f;
+  // (scores that are scaled late are scaled by a number above 0)
+  const bool plain = !scores_any(scores) && a.scale != 0.0f && a.scale - a.scale == 0.0f;
   const size_t parts = part_bytes(group, cache->dim);
   RKV_DISPATCH_DIM(cache->dim, D, {
     if (cache->dtype == RKV_F16) {

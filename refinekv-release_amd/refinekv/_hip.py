@@ -807,15 +807,15 @@ _prompt_sizes = {}
 
 
 def _prompt_scratch(workspace, tokens, sequences, heads, group, dim, most_keys, device):
-    """(buffer or None, bytes) for a prompt's call: sizes are rounded up to powers
-    of two, so that a workspace keeps few buffers (none ever replaced: a
-    captured graph keeps using the one it was captured with)."""
+    """(buffer or None, bytes) for a prompt's call: one size for a head_dim and
+    device (none is ever replaced: a captured graph keeps using the one it was
+    captured with)."""
     shape = (tokens, sequences, heads, group, dim, most_keys, device.index)
     nbytes = _prompt_sizes.get(shape)
     if nbytes is None:
         found = _size()
         _check(lib().rkv_prompt_plan(*shape[:6], ctypes.byref(found)), "rkv_prompt_plan")
-        nbytes = 1 << max(found.value - 1, (1 << 20) - 1).bit_length() if found.value else 0
+        nbytes = found.value
         if len(_prompt_sizes) >= 4096:
             _prompt_sizes.clear()
         _prompt_sizes[shape] = nbytes

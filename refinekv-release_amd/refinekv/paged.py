@@ -20,7 +20,6 @@ Inference only, as the whole package: the results carry no gradient.
 """
 
 from dataclasses import dataclass, field
-import math
 
 import torch
 
@@ -29,6 +28,7 @@ from .quantized import PAGE_SIZES, QuantizedCache
 from .rotary import DTYPES, check_out, overlaps_itself, pick_backend, rows_overlap
 
 MAX_ROW_STRIDE = 1 << 25  # elements between a page's rows, at most
+MOST_TOKENS = 2 ** 31 - 1  # positions are int32
 
 
 @dataclass(frozen=True, eq=False)
@@ -212,6 +212,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     elif query_out is not None:
         raise ValueError("query_out without a query")
     quantized = isinstance(cache, QuantizedCache)
+    if quantized and query_out is not None and _meet_pages(query_out, cache):
+        raise ValueError("query_out overlaps the cache")
     why = None if key.dtype in DTYPES else "the HIP append needs a bf16, fp16 or fp32 cache"
     if pick_backend(key, backend, why is None, why) == "hip":
         hip = _hip.quantized_append if quantized else _hip.paged_append
@@ -277,8 +279,8 @@ def check_scores(softcap, slopes, window, q_heads, device):
     """The checked options of a call, or None where they ask for nothing."""
     if softcap is None and slopes is None and window is None:
         return None
-    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
-        raise ValueError("softcap must be finite and positive")
+    if softcap is not None and not 1e-30 <= softcap <= 1e30:
+        raise ValueError("softcap must be in 1e-30..1e30")
     if window is not None and (not isinstance(window, int) or isinstance(window, bool)
                                or window <= 0):
         raise ValueError("window must be a positive integer")
@@ -287,7 +289,7 @@ def check_scores(softcap, slopes, window, q_heads, device):
             raise ValueError("slopes must be float32 with shape (q_heads,)")
         if slopes.device != device or not slopes.is_contiguous():
             raise ValueError("slopes must be contiguous on the query's device")
-    return Scores(0.0 if softcap is None else float(softcap), slopes, window or 0)
+    return Scores(0.0 if softcap is None else float(softcap), slopes, min(window or 0, MOST_TOKENS))
 
 
 def _decode_support(cache, group):

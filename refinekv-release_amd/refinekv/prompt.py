@@ -25,6 +25,7 @@ from .paged import (MAX_ROW_STRIDE, _check_capture, _check_starts, _meet_pages, 
 from .quantized import QuantizedCache
 from .rotary import pick_backend, rows_overlap
 
+MOST_KEYS = 2 ** 31 - 512
 HIP_DTYPES = (torch.bfloat16, torch.float16)
 
 
@@ -68,6 +69,8 @@ def _why_not_cache(cache):
                 why = "the HIP prompt attention needs a cache of 16-byte aligned rows"
             elif t.stride(2) > MAX_ROW_STRIDE:
                 why = "the HIP prompt attention needs a cache whose rows are not too far apart"
+        if cache.capacity > MOST_KEYS:
+            why = "the HIP prompt attention needs a block table of fewer tokens"
     return why
 
 

@@ -320,3 +320,45 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         with torch.cuda.graph(graph):
             paged_prompt(q, cache)
+
+
+def test_starts_that_overlap():
+    """Several sequences whose device starts overlap ask for more tiles than the
+    rows have: whatever is written lies inside, and later calls are right."""
+    gen = torch.Generator().manual_seed(12)
+    _, query, key, value = ragged([40], 1, 2, 64, BF16, gen, behind=0)
+    rows = [t.to(DEV) for t in (query, key, value)]
+    many = torch.tensor([0, 40] * 33, dtype=torch.int32, device=DEV)
+    far = torch.tensor([0, 2 ** 31 - 1] * 33, dtype=torch.int32, device=DEV)
+    long_keys = [torch.randn(4000, 1, 64, generator=gen).to(BF16).to(DEV) for _ in range(2)]
+    workspace = {}
+    for starts in (many, far):
+        guard = torch.full((42, 2, 64), 7.0, dtype=BF16, device=DEV)
+        prompt_attention(*rows, token_starts=starts, output=guard[1:41], backend="hip")
+        prompt_attention(rows[0], *long_keys, token_starts=starts,
+                         key_starts=torch.tensor([0, 4000] * 33, dtype=torch.int32, device=DEV),
+                         output=guard[1:41], workspace=workspace, backend="hip")
+        assert bool((guard[0] == 7.0).all()) and bool((guard[41] == 7.0).all())
+    ends = torch.tensor([0, 40])
+    got = prompt_attention(*rows, backend="hip")
+    want, room = prompt64(query, key, value, ends, ends)
+    assert_rows(got, want, room)
+
+
+def test_more_sequences_than_lanes():
+    """More sequences than a wave has lanes, most of them empty or of a row."""
+    gen = torch.Generator().manual_seed(13)
+    counts = [(b * 7) % 4 if b % 5 else 0 for b in range(200)]
+    counts[150] = 130
+    starts, query, key, value = ragged(counts, 1, 2, 64, BF16, gen)
+    got = prompt_attention(*(t.to(DEV) for t in (query, key, value)),
+                           token_starts=starts.to(DEV), backend="hip")
+    want, room = prompt64(query, key, value, starts, starts)
+    assert_rows(got, want, room)
+    # over longer keys, which are shared out
+    lengths = [n + (b * 37) % 300 for b, n in enumerate(counts)]
+    ends, _, key, value = ragged(lengths, 1, 1, 64, BF16, gen)
+    got = prompt_attention(query.to(DEV), key.to(DEV), value.to(DEV), backend="hip",
+                           token_starts=starts.to(DEV), key_starts=ends.to(DEV), window=200)
+    want, room = prompt64(query, key, value, starts, ends, window=200)
+    assert_rows(got, want, room)

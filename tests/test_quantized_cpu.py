@@ -284,7 +284,7 @@ def test_call_refusals():
         with pytest.raises(ValueError):
             paged_read(cache, tokens, token_starts=starts)
     query = torch.zeros(3, 4, 64, dtype=BF16)
-    for options in (dict(softcap=0.0), dict(softcap=-1.0), dict(softcap=math.inf),
+    for options in (dict(softcap=0.0), dict(softcap=-1.0), dict(softcap=math.inf), dict(softcap=1e-40),
                     dict(softcap=math.nan), dict(window=0), dict(window=2.0), dict(window=True),
                     dict(slopes=torch.zeros(3)), dict(slopes=torch.zeros(4).double()),
                     dict(slopes=torch.zeros(8)[::2]), dict(output=query[:2]),

@@ -472,3 +472,28 @@ def test_refusals():
     with pytest.raises(ValueError):  # codes at an odd address
         QuantizedCache(raw[8:].view(4, 2, 16, 32), cache.value_codes, cache.key_scales,
                        cache.value_scales, cache.block_table, cache.lengths)
+
+
+def test_scales_of_nothing():
+    """A scale of 0, one that vanishes against a zero query's, negative ones."""
+    gen = torch.Generator().manual_seed(31)
+    lengths = [40, 17, 0]
+    on_cpu, wide = quantized_pages(lengths, 16, 1, 64, BF16, gen)
+    query = torch.randn(3, 4, 64, generator=gen).to(BF16)
+    query[0, 1] = 0.0
+    for scaling in (0.0, 1e-20, -0.2):
+        got = paged_decode(query.to(DEV), to(on_cpu, DEV), scaling=scaling, backend="hip")
+        want, room = decode64_quantized(query, *wide, on_cpu.block_table, lengths, scaling)
+        assert_within(got, want, room, str(scaling))
+
+
+def test_query_out_among_the_pages():
+    """Refused, at an odd address as well (where a copy would be made first)."""
+    cache = QuantizedCache.empty(64, 1, 16, 64, 2, 2, device=DEV)
+    rows = torch.zeros(2, 1, 64, dtype=BF16, device=DEV)
+    rotary = Rotary(RotaryConfig(head_dim=64), DEV)
+    pool = cache.value_codes.view(-1).view(BF16)
+    for first in (0, 1):
+        with pytest.raises(ValueError):
+            paged_append(rows, rows, cache, query=rows, rotary=rotary,
+                         query_out=pool[first:first + 128].view(2, 1, 64))
