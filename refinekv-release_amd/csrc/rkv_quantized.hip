@@ -28,7 +28,9 @@
 namespace rkv {
 namespace {
 
-constexpr float kLargest = 4096.0f;  // in magnitude, of a group's values
+// In magnitude, of a group's values: 64 times a scale (at most 8192 / 15, and 1/64
+// more) stays in fp16's range.
+constexpr float kLargest = 4096.0f;
 constexpr int kGroupDims = 32;
 
 typedef _Float16 Half2 __attribute__((ext_vector_type(2)));
@@ -192,6 +194,11 @@ __device__ __forceinline__ void store_value(const QuantRows& a, int64_t row, int
 // parts of two; or (the whole head turns) in the thread's second item.
 enum Partner : int { kWithin, kWhole, kParts, kHalves };
 
+// Memory and vector issue bound it together: 18 K tokens' rows of 28 + 4 + 4 heads
+// (d 128, fp16, 150 MB in and out) in 33 us, 4.5 TB/s, of which some 23 us are
+// vector instructions (a cos and sin costs 30, a coded value 8).  Coding in the
+// same pass as the queries 42 us, with a division a value 50, each half of a row
+// in a thread of its own (which works out the other's cos and sin again) 77.
 // A thread holds 8 dims of a token's rows (kHalves: twice 8, half a row apart):
 // it works out their cos and sin once and applies them to every slots-th head,
 // queries, then keys, then values, the next head's row on its way while one is
@@ -413,9 +420,8 @@ __device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t view, uint32_t
   }
 }
 
-// Entry m of 4 that a word holds: the two codes as fp16 numbers 64 + code (in
-// fp16, 64 + code / 16 times 16 units of the last bit: the code shifted to
-// bits 4 .. 7 of 64).
+// Entry m of 4 that a word holds: the two codes as fp16 numbers 64 + code (the
+// code in bits 4 .. 7 of 64, whose last bit is 1/16).
 // Mask and 64 come in registers: as literals they take an instruction each.
 struct CodeBits {
   uint32_t mask = 0x00f000f0u, sixty_four = 0x54005400u;
@@ -690,6 +696,12 @@ struct Pages4 {
 template <int D>
 constexpr int kPerCu4 = D <= 64 ? 3 : D <= 128 ? 2 : 1;
 
+// HBM and vector issue bound it together: 1.34 GB of 8 x 131072 tokens (8 KV heads,
+// group 4, d 128) in 222-245 us, 5.5-6.0 TB/s; 313 vector instructions a tile of 32
+// tokens (176 of them turn its 8192 codes into fp16) keep the ALUs busy for 138 us
+// of it.  (378 when masks and biases were literals and every tile had the selects
+// of a row's end, and 258 us.)  A call of few tokens is paged_kernel's chain of
+// latencies: one sequence of 2003 tokens 7.7 us, then 4.5 for the join.
 template <int D, bool kHalf, bool kScores>
 __global__ __launch_bounds__(kThreads)
 __attribute__((amdgpu_waves_per_eu(kPerCu4<D>))) void quantized_kernel(QuantArgs a) {
