@@ -279,7 +279,7 @@ __device__ __forceinline__ uint32_t value_words(uint32_t w, int pass) {
 // The matrix cores and the softmax's vector issue bound it, one after the other
 // more than side by side: 16384 tokens (8 KV heads, group 4, d 128) in 2160-2190
 // us, 1010 TFLOP/s of the visible products (a bf16 product of 8192^3 reaches 1257
-// here), the matrix cores busy for 48 % of it and the vector ALUs for 52 %.
+// here), the matrix cores busy for 47 % of it and the vector ALUs for 51 %.
 // (Scores of the next tile computed beside the softmax of this one, keys two tiles
 // ahead: 2610 us; tiles of 32 keys 2380; reads of all a product's operands in
 // groups of 8: 2300 against 2255.)  Few rows over many keys are bound by the keys

@@ -692,6 +692,15 @@ def paged_append(key, value, cache, query=None, table=None, token_starts=None, q
     return query_out
 
 
+def _whole_rows(t):
+    """(tokens, heads, dim) rows of a 16-bit type whose addresses are multiples of
+    16 bytes (a copy where they are not)."""
+    token, head, dim = t.stride()
+    if dim == 1 and not (t.data_ptr() | 2 * (token | head)) & 15:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def quantized_append(key, value, cache, query=None, table=None, token_starts=None,
                      query_out=None):
     """rkv_quantized_append on checked rows; returns the turned query or None."""
@@ -699,10 +708,10 @@ def quantized_append(key, value, cache, query=None, table=None, token_starts=Non
     if _elsewhere(device):
         with torch.cuda.device(device):
             return quantized_append(key, value, cache, query, table, token_starts, query_out)
-    key, value = _row_aligned(key, 16), _row_aligned(value, 16)
+    key, value = _whole_rows(key), _whole_rows(value)
     rows, target = (0, 0, 0, 0, 0, 0, 0), query_out
     if query is not None:
-        query = _row_aligned(query, 16)
+        query = _whole_rows(query)
         # (the kernel writes whole vectors, and not over the query)
         if query_out is None or not _takes_rows(query_out) or _spans_meet(query, query_out):
             target = _like(query)
@@ -838,7 +847,7 @@ def prompt_attention(query, key, value, sequences, token_starts, key_starts, pre
         with torch.cuda.device(device):
             return prompt_attention(query, key, value, sequences, token_starts, key_starts,
                                     prefix, scaling, scores, workspace, output)
-    query, key, value = (_row_aligned(t, 16) for t in (query, key, value))
+    query, key, value = _whole_rows(query), _whole_rows(key), _whole_rows(value)
     key, value = (t.contiguous() if t.stride(0) > MAX_ROW_STRIDE else t for t in (key, value))
     if output is not None and output.data_ptr() % 16:  # (the kernel stores whole vectors)
         return output.copy_(prompt_attention(query, key, value, sequences, token_starts,
@@ -870,7 +879,7 @@ def paged_prompt(query, cache, token_starts, prefix, scaling, scores, workspace=
         with torch.cuda.device(device):
             return paged_prompt(query, cache, token_starts, prefix, scaling, scores, workspace,
                                 output)
-    query = _row_aligned(query, 16)
+    query = _whole_rows(query)
     if output is not None and output.data_ptr() % 16:  # (the kernel stores whole vectors)
         return output.copy_(paged_prompt(query, cache, token_starts, prefix, scaling, scores,
                                          workspace, output.clone()))

@@ -497,3 +497,28 @@ def test_query_out_among_the_pages():
         with pytest.raises(ValueError):
             paged_append(rows, rows, cache, query=rows, rotary=rotary,
                          query_out=pool[first:first + 128].view(2, 1, 64))
+
+
+@pytest.mark.parametrize("scores", [{}, dict(softcap=20.0)])
+@pytest.mark.parametrize("four", [True, False])
+def test_widest_group_and_head(four, scores):
+    """The most LDS that a workgroup's parts take: 16 query heads of 256 dims, rows
+    that several waves and workgroups hold parts of."""
+    gen = torch.Generator().manual_seed(37)
+    lengths = [700, 3, 41000]
+    query = torch.randn(3, 16, 256, generator=gen).to(BF16)
+    if four:
+        on_cpu, wide = quantized_pages(lengths, 64, 1, 256, BF16, gen)
+        got = paged_decode(query.to(DEV), to(on_cpu, DEV), backend="hip", **scores)
+        want, room = decode64_quantized(query, *wide, on_cpu.block_table, lengths, 1 / 16, **scores)
+        assert_within(got, want, room)
+        return
+    keys, values, table = pages_for(lengths, 64, 1, 256, BF16, gen)
+    cache = PagedCache(*(t.to(DEV) for t in (keys, values, table)),
+                       torch.tensor(lengths, dtype=torch.int32, device=DEV))
+    got = paged_decode(query.to(DEV), cache, backend="hip", **scores).cpu()
+    for b, n in enumerate(lengths):
+        k, v = (t[table[b, :-(-n // 64)].long(), 0].reshape(-1, 256)[:n] for t in (keys, values))
+        want, room = attend64(query[b], k, v, torch.full((16,), n - 1), 1 / 16, BF16,
+                              scores.get("softcap", 0.0))
+        assert_within(got[b], want, room, str(b))
