@@ -191,7 +191,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
     here belongs to one sequence, and a cache whose keys and values share
     memory is refused.  Rows that are views of the cache's pages are copied
     first: the call stores what they hold before it.  To a ``QuantizedCache``
-    the rows go in 4 bits, keys turned and rounded to their type before.
+    the rows go in 4 bits, keys turned and rounded to their type before;
+    views of its tensors are refused as rows.
 
     (A prompt's own attention needs its turned keys as well: turn both with
     rotate_heads, then append without ``rotary``.)
@@ -224,6 +225,8 @@ def paged_append(key, value, cache, *, query=None, rotary=None, token_starts=Non
 
     if not quantized and _keys_meet_values(cache):
         raise ValueError("the cache's keys and values share memory")
+    if quantized and any(_meet_pages(t, cache) for t in (key, value, query) if t is not None):
+        raise ValueError("rows overlap the cache")
     if query_out is not None and _meet_pages(query_out, cache):
         raise ValueError("query_out overlaps the cache")
     with torch.no_grad():

@@ -294,3 +294,13 @@ def test_call_refusals():
     with pytest.raises(ValueError):
         paged_decode(query[:, :3], cache)
     assert not bool(paged_decode(query, cache).any())  # every place is idle
+
+
+def test_rows_in_the_cache_are_refused():
+    cache = QuantizedCache.empty(16, 2, 16, 64, 3, 2)
+    inside = cache.key_codes.view(-1).view(BF16)[:384].view(3, 2, 64)
+    rows = torch.zeros(3, 2, 64, dtype=BF16)
+    for change in (dict(key=inside), dict(value=inside),
+                   dict(query=inside, rotary=Rotary(RotaryConfig(head_dim=64)))):
+        with pytest.raises(ValueError, match="overlap the cache"):
+            paged_append(**{**dict(key=rows, value=rows, cache=cache), **change})

@@ -522,3 +522,12 @@ def test_widest_group_and_head(four, scores):
         want, room = attend64(query[b], k, v, torch.full((16,), n - 1), 1 / 16, BF16,
                               scores.get("softcap", 0.0))
         assert_within(got[b], want, room, str(b))
+
+
+def test_rows_in_the_cache_are_refused():
+    cache = QuantizedCache.empty(16, 2, 16, 64, 3, 2, device=DEV)
+    inside = cache.value_codes.view(-1).view(BF16)[:384].view(3, 2, 64)
+    rows = torch.zeros(3, 2, 64, dtype=BF16, device=DEV)
+    for change in (dict(key=inside), dict(value=inside)):
+        with pytest.raises(ValueError, match="overlap the cache"):
+            paged_append(**{**dict(key=rows, value=rows, cache=cache, backend="hip"), **change})
