@@ -4,6 +4,8 @@
 // over the tokens j of i's sequence that i sees: those up to i, and those of
 // the sequence's prefix, at most `window` back; f caps the scores and biases
 // them by distance.
+#include <algorithm>
+
 #include "rkv_paged_walk.h"
 
 namespace rkv {
@@ -50,7 +52,8 @@ struct PromptArgs {
   const float* slopes;
   int window;
   char* out;                   // (tokens, H G, D) dense
-  int zero_rest;               // rows of no sequence become zeros (else: as they were)
+  int zero_rest;               // workgroups a head for the rows of no sequence, which
+                               // become zeros (0: they stay as they were)
   int tiles;                   // at most so many in the grid
   // few tiles: so many workgroups share all tiles' keys (0: each has a tile of
   // its own); keys are counted in units of 2^unit LDS tiles
@@ -134,12 +137,12 @@ __device__ __forceinline__ bool find_entry(const PromptArgs& a, uint32_t slot, b
   const uint32_t at = from_end ? total - 1u - slot : slot;
   const int owner = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
   place = at - (uint32_t)uniform(__shfl((int)(upto - sum), owner, kWave));
-  for (b = owner * per; b + 1 < a.sequences; ++b) {
+  for (b = owner * per; b < a.sequences; ++b) {
     const uint32_t here = (uint32_t)uniform((int)entries(b));
-    if (place < here) break;
+    if (place < here) return true;
     place -= here;
   }
-  return true;
+  return false;  // (starts that overlap so often that their sum passed 32 bits)
 }
 
 // The slot-th of the tiles, the last ones of the last sequence first: a
@@ -238,16 +241,17 @@ __device__ __forceinline__ bool find_share(const PromptArgs& a, uint32_t slot, P
   return true;
 }
 
-// Rows of no sequence: this head group's part of them becomes zeros.
+// Rows of no sequence: the part-th part of them becomes zeros, for one head's group.
 template <int D>
-__device__ __forceinline__ void zero_rows(const PromptArgs& a, int head) {
+__device__ __forceinline__ void zero_rows(const PromptArgs& a, int head, int part) {
   int first, count, last;
   rows_of(a, 0, first, count);
   rows_of(a, a.sequences - 1, last, count);
   last += count;
   const int per_row = a.group * (D / 8);
   const int64_t n = (int64_t)(a.tokens - last + first) * per_row;
-  for (int64_t i = threadIdx.x; i < n; i += kPromptThreads) {
+  for (int64_t i = (int64_t)part * kPromptThreads + threadIdx.x; i < n;
+       i += (int64_t)a.zero_rest * kPromptThreads) {
     const int64_t row = i / per_row, token = row < first ? row : row - first + last;
     reinterpret_cast<U32x4*>(a.out)[(token * a.heads + head) * per_row + i % per_row] =
         U32x4{0u, 0u, 0u, 0u};
@@ -313,9 +317,10 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
   constexpr bool kProductsFirst = D > 64;
   __shared__ alignas(16) char smem[2][Tile::kBytes];
   __shared__ uint32_t marks[2][kMarks][kPromptThreads];  // outputs that kUp and kDown found
-  const uint32_t last = gridDim.x - (a.zero_rest ? (uint32_t)a.heads : 0u);
+  const uint32_t last = gridDim.x - (uint32_t)(a.zero_rest * a.heads);
   if (blockIdx.x >= last) {
-    zero_rows<D>(a, (int)(blockIdx.x - last));
+    const int rest = (int)(blockIdx.x - last);
+    zero_rows<D>(a, rest % a.heads, rest / a.heads);
     return;
   }
   PromptRows rows;
@@ -682,7 +687,7 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
   if (!find_share<PromptTile<D>::kTokens, true>(a, blockIdx.x, rows, share) || share.chunks == 1)
     return;
   // (starts that overlap ask for more shares than there are)
-  if ((int64_t)share.first + (int64_t)(share.chunks - 1) * share.apart >= a.shares) return;
+  if ((uint32_t)share.first + (int64_t)(share.chunks - 1) * share.apart >= a.shares) return;
   const int head = share.head;
   const int c = (int)threadIdx.x % kAcross, in = (int)threadIdx.x / kAcross;
   const int pairs = min(rows.count * a.group - rows.tile * kTileRows, kTileRows);
@@ -749,9 +754,10 @@ int check_prompt(const char* who, int dtype, int64_t tokens, int64_t sequences, 
   if (tokens < 0 || sequences <= 0 || heads <= 0 || group <= 0 || sequences > lim ||
       heads > 65535 || group > 65535)
     return set_error(kInvalidArgument, "%s: empty or oversized shape", who);
-  // (pairs of a sequence, and the grid, are counted in 32 bits)
+  // (pairs of a sequence are counted in 32 bits, and so are a launch's threads)
+  const int64_t most = (int64_t(1) << 32) / kPromptThreads - 1;
   if (tokens > lim / group - kTileRows || heads * group > lim ||
-      (tokens * group / kTileRows + (tokens < sequences ? tokens : sequences) + 1) > lim / heads)
+      (tokens * group / kTileRows + (tokens < sequences ? tokens : sequences) + 32) > most / heads)
     return set_error(kUnsupported, "%s: too many rows", who);
   return kOk;
 }
@@ -798,15 +804,17 @@ int prompt(const char* who, PromptArgs& a, int dtype, int64_t tokens, int64_t se
     }
   }
   a.out = static_cast<char*>(output);
-  a.zero_rest = zero_rest;
+  // (rows behind the last sequence may be most of a padded batch: a workgroup for
+  // every 256 of them, up to 32 a head)
+  a.zero_rest = zero_rest ? (int)std::min<int64_t>(1 + tokens / 256, 32) : 0;
   a.tiles = P.tiles;
   a.shares = P.shares;
   a.unit = P.unit;
   // (a window alone changes no score; a scale of 0 times a hidden score would)
   const bool plain = !(a.cap > 0.0f) && !a.slopes && a.scale > 0.0f && a.scale < kPosInf;
   const int64_t blocks = P.shares ? P.shares : P.tiles * heads;
-  // (the last `heads` workgroups: rows of no sequence)
-  const dim3 grid((unsigned)(blocks + (zero_rest ? heads : 0)));
+  // (the last workgroups: rows of no sequence)
+  const dim3 grid((unsigned)(blocks + a.zero_rest * heads));
   const dim3 join((unsigned)(P.tiles * heads), 16), threads(kPromptThreads);
   RKV_DISPATCH_DIM(dim, D, {
     if (dtype == RKV_F16) {

@@ -345,6 +345,27 @@ def test_starts_that_overlap():
     assert_rows(got, want, room)
 
 
+@pytest.mark.parametrize("before,behind", [(0, 9001), (1300, 700), (5000, 4000)])
+def test_rows_of_no_sequence(before, behind):
+    """A padded batch: zeros in a new tensor, left alone in `output`."""
+    gen = torch.Generator().manual_seed(before)
+    counts, heads, group, dim = (50, 0, 33), 3, 2, 64
+    _, query, key, value = ragged(counts, heads, group, dim, F16, gen, behind=before + behind)
+    starts = torch.tensor([before, before + 50, before + 50, before + 83]).int()
+    rows = [t.to(DEV) for t in (query, key, value)]
+    poison = torch.full_like(rows[0], 7.0)  # (memory that the new tensor may take)
+    del poison
+    got = prompt_attention(*rows, token_starts=starts.to(DEV), backend="hip")
+    want, room = prompt64(query, key, value, starts, starts)
+    assert_rows(got, want, room, "padded")
+    assert not bool(got[:before].any()) and not bool(got[before + 83:].any())
+    kept = torch.full_like(rows[0], 7.0)
+    prompt_attention(*rows, token_starts=starts.to(DEV), backend="hip", output=kept)
+    inside = slice(before, before + 83)
+    assert torch.equal(bits(kept[inside]), bits(got[inside]))
+    assert bool((kept[:before] == 7.0).all()) and bool((kept[before + 83:] == 7.0).all())
+
+
 def test_more_sequences_than_lanes():
     """More sequences than a wave has lanes, most of them empty or of a row."""
     gen = torch.Generator().manual_seed(13)
