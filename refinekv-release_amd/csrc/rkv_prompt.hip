@@ -390,9 +390,21 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
       for (int i = 0; i < 4; ++i) q[j][i] ^= a.flip;
     }
   }
-  float slope = 0.0f;
-  if constexpr (kScores)
+  // Scores without a cap are scaled on the way into the exponential, slopes divided
+  // by the scale for it; of tiles before all the wave's rows a key's bias is that of
+  // the tile's first and its place's, one operation a score (23 documents, head_dim
+  // 64, 119 -> 111 us).  Not with slopes or scales whose products could overflow.
+  float slope = 0.0f, unit_slope = 0.0f, scale = a.scale;
+  bool late = true;
+  int biased_end = 0;  // tokens up to every row of the wave
+  if constexpr (kScores) {
     if (a.slopes) slope = a.slopes[head * a.group + g] * kLog2e;
+    const bool tame = __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(slope) < 1e20f)) == 0;
+    late = tame && !(a.cap > 0.0f) && a.scale > 0x1p-20f && a.scale < 0x1p20f;
+    unit_slope = late ? slope / a.scale : slope;
+    scale = late ? a.scale : 1.0f;
+    if (tame) biased_end = position_of(pair0 + wave * kWaveRows) + 1;
+  }
 
   int pass = kPlain;
 
@@ -507,10 +519,13 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
         }
         __builtin_amdgcn_s_setprio(kProductsFirst ? 0 : 1);
         auto token = [&](int u, int i) { return t0 + 32 * u + 8 * (i / 4) + 4 * h + i % 4; };
+        float bias = 0.0f;  // of the lane's first key, apart from the scores
         if constexpr (kScores) {
           const float by = a.cap > 0.0f ? a.per_cap : a.scale;
+          if (!late) {
 #pragma unroll
-          for (int u = 0; u < T / 32; ++u) s[u] *= by;
+            for (int u = 0; u < T / 32; ++u) s[u] *= by;
+          }
           if (a.cap > 0.0f) {
 #pragma unroll
             for (int u = 0; u < T / 32; ++u)
@@ -518,17 +533,27 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
               for (int i = 0; i < 16; ++i) s[u][i] = tanh_hw(s[u][i]) * a.cap;
           }
           if (a.slopes) {
-            // the distances of a lane's keys from that of its first
+            // the distance of a lane's first key, and its others' from that
             const float far = (float)(pos - token(0, 0));
+            if (t0 + T <= biased_end) {
+              bias = -slope * far;
 #pragma unroll
-            for (int u = 0; u < T / 32; ++u)
+              for (int u = 0; u < T / 32; ++u)
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                s[u][i] = __builtin_fmaf(
-                    -slope, __builtin_fabsf(far - (float)(32 * u + 8 * (i / 4) + i % 4)), s[u][i]);
+                for (int i = 0; i < 16; ++i)
+                  s[u][i] = __builtin_fmaf(unit_slope, (float)(32 * u + 8 * (i / 4) + i % 4),
+                                           s[u][i]);
+            } else {
+#pragma unroll
+              for (int u = 0; u < T / 32; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  s[u][i] = __builtin_fmaf(
+                      -unit_slope, __builtin_fabsf(far - (float)(32 * u + 8 * (i / 4) + i % 4)),
+                      s[u][i]);
+            }
           }
         }
-        const float scale = kScores ? 1.0f : a.scale;
         if (t0 + T > whole_end || t0 < whole_begin) {
 #pragma unroll
           for (int u = 0; u < T / 32; ++u)
@@ -542,9 +567,10 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
         for (int u = 0; u < T / 32; ++u)
 #pragma unroll
           for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[u][i]);
+        top = kScores ? __builtin_fmaf(top, scale, bias) : top * scale;
         float x, y;
         xor32_pair(top, x, y);
-        top = __builtin_fmaxf(x, y) * scale;
+        top = __builtin_fmaxf(x, y);
         // (the maximum may lag by 2^8: weights up to that, and fewer rescalings)
         if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {
           const float mn = __builtin_fmaxf(m, top);
@@ -556,7 +582,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
         }
         // (fp16 weights start from 2^7: those under 2^-24 of the largest, many
         // in a long context, do not all round to zero)
-        const float base = m == kNegInf ? 0.0f : kHalf ? m - 7.0f : m;
+        const float base = (m == kNegInf ? 0.0f : kHalf ? m - 7.0f : m) - bias;
         U32x4 p[T / 16];
 #pragma unroll
         for (int u = 0; u < T / 32; ++u)

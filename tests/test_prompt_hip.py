@@ -345,6 +345,31 @@ def test_starts_that_overlap():
     assert_rows(got, want, room)
 
 
+@pytest.mark.parametrize("dim,group,dtype", [(64, 1, BF16), (128, 3, F16)])
+def test_slopes_of_all_sizes(dim, group, dtype):
+    """Slopes below zero, of nothing and too large for a shared bias; scales that
+    are too small or large for one, or 1; caps beside them."""
+    gen = torch.Generator().manual_seed(dim)
+    counts = (300, 65)
+    starts, query, key, value = ragged(counts, 2, group, dim, dtype, gen)
+    rows = [t.to(DEV) for t in (query, key, value)]
+    slopes = torch.logspace(-9, 0, 2 * group, base=2.0)
+    prefix = torch.tensor([130, 3]).int()
+    one = math.log(2.0)  # (times log2 e: about 1)
+    mixed = slopes.clone()
+    mixed[0] = 1e25
+    for options in (dict(slopes=-slopes), dict(slopes=slopes * 0), dict(slopes=mixed),
+                    dict(slopes=slopes, scaling=2.0 ** -24), dict(slopes=slopes, scaling=-0.1),
+                    dict(slopes=slopes, scaling=one), dict(softcap=3.0, scaling=one),
+                    dict(slopes=-slopes, softcap=3.0, window=100),
+                    dict(slopes=slopes, prefix=prefix, window=70)):
+        got = prompt_attention(*rows, token_starts=starts.to(DEV), backend="hip",
+                               **on_gpu(options))
+        want, room = prompt64(query, key, value, starts, starts, **options)
+        what = str({k: v if isinstance(v, float) else str(v) for k, v in options.items()})
+        assert_rows(got, want, room, what)
+
+
 @pytest.mark.parametrize("before,behind", [(0, 9001), (1300, 700), (5000, 4000)])
 def test_rows_of_no_sequence(before, behind):
     """A padded batch: zeros in a new tensor, left alone in `output`."""
