@@ -574,7 +574,10 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
         // (the maximum may lag by 2^8: weights up to that, and fewer rescalings)
         if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {
           const float mn = __builtin_fmaxf(m, top);
-          const float by = mn == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+          // (kUp and kDown count: a count does not shrink)
+          const float by = mn == kNegInf || pass == kUp || pass == kDown
+                               ? 1.0f
+                               : __builtin_amdgcn_exp2f(m - mn);
           m = mn;
           l *= by;
 #pragma unroll
