@@ -208,11 +208,17 @@ struct Shares {
 };
 
 // Folds parts j = first, first + step, .. of n into (m, l, o): in batches whose
-// loads are all in flight before the first use.
-template <typename Ml, typename Acc>
+// loads are all in flight before the first use.  kKeep: infinite and NaN sums
+// count whatever their part weighs (else one that weighs 0 is NaN).
+template <bool kKeep = false, typename Ml, typename Acc>
 __device__ __forceinline__ void fold_parts(uint32_t first, uint32_t step, uint32_t n, float& m,
                                            float& l, F32x4& o, Ml load_ml, Acc load_acc) {
   constexpr uint32_t kBatch = 8;
+  auto weighed = [](F32x4 x, float w) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = kKeep && !__builtin_isfinite(x[i]) ? x[i] : x[i] * w;
+    return x;
+  };
   for (uint32_t j0 = first; j0 < n; j0 += step * kBatch) {
     float2 ml[kBatch];
     float4 x[kBatch];
@@ -227,7 +233,7 @@ __device__ __forceinline__ void fold_parts(uint32_t first, uint32_t step, uint32
     for (uint32_t i = 0; i < kBatch; ++i) mn = __builtin_fmaxf(mn, ml[i].x);
     const float old = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
     l *= old;
-    o *= old;
+    o = weighed(o, old);
     m = mn;
 #pragma unroll
     for (uint32_t i = 0; i < kBatch; ++i) {
@@ -235,7 +241,8 @@ __device__ __forceinline__ void fold_parts(uint32_t first, uint32_t step, uint32
       const float w = ml[i].x == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - mn);
       // (a NaN sum stays one, whatever its weight)
       l += there ? ml[i].y * w : 0.0f;
-      o += there ? F32x4{x[i].x, x[i].y, x[i].z, x[i].w} * w : F32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      o += there ? weighed(F32x4{x[i].x, x[i].y, x[i].z, x[i].w}, w)
+                 : F32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
   }
 }

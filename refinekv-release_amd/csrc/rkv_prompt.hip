@@ -730,11 +730,12 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
     auto part_at = [&](uint32_t j) {
       return ((int64_t)share.first + (int64_t)j * share.apart) * kTileRows + i;
     };
-    fold_parts(0u, 1u, (uint32_t)share.chunks, m, l, o,
-               [&](uint32_t j) { return a.part_ml[part_at(j)]; },
-               [&](uint32_t j) {
-                 return *reinterpret_cast<const float4*>(a.part_acc + part_at(j) * D + 4 * c);
-               });
+    fold_parts<true>(
+        0u, 1u, (uint32_t)share.chunks, m, l, o,
+        [&](uint32_t j) { return a.part_ml[part_at(j)]; },
+        [&](uint32_t j) {
+          return *reinterpret_cast<const float4*>(a.part_acc + part_at(j) * D + 4 * c);
+        });
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     typedef E E4 __attribute__((ext_vector_type(4)));
     E4 v;

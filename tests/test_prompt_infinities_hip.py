@@ -65,3 +65,20 @@ def test_values_far_behind(dim, dtype):
     query[..., :2], key[..., :2] = 1.0, 0.0
     key[:, :, 0] = (torch.arange(287) % 250)[:, None]
     check(query, key, value, starts, starts, scaling=1.0)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16), (160, BF16)])
+def test_values_far_behind_in_shares(dim, dtype):
+    """Few rows, whose keys several workgroups share: a part that weighs e^-600
+    beside another, infinite or NaN."""
+    gen = torch.Generator().manual_seed(dim)
+    starts = torch.tensor([0, 40, 45], dtype=torch.int32)
+    key_starts = torch.tensor([0, 3000, 4000], dtype=torch.int32)
+    query = rows(45, 4, dim, dtype, gen)
+    key, value = (rows(4000, 2, dim, dtype, gen) for _ in range(2))
+    early(value, 0)
+    early(value, 2988)  # (and the last rows of the first sequence alone)
+    slopes = torch.tensor([0.2, 0.15, 0.1, 0.05])
+    check(query, key, value, starts, key_starts, slopes=slopes)
+    check(query, key, value, starts, key_starts, slopes=-slopes)
+    check(query, key, value, starts, key_starts, slopes=slopes, window=2975)
