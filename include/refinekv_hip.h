@@ -414,8 +414,9 @@ int rkv_quantized_plan(const rkv_quantized_cache* cache, int64_t group, size_t* 
  * (key_tokens, heads, dim) keys and values; the query rows are the last ones of
  * the key rows.  A row sees the keys up to its own, all of the sequence's first
  * prefix[b] (device int32 per sequence, null: none), and of these at most
- * scores->window back; one that sees nothing is zeros.  An infinite or NaN value
- * counts for the rows that see it.  Query heads h group .. + group - 1 belong
+ * scores->window back; one that sees nothing is zeros, one whose scores are -inf
+ * alone NaN, as a softmax is.  An infinite or NaN value counts for the rows that
+ * see it, whatever it weighs.  Query heads h group .. + group - 1 belong
  * to KV head h.  output: dense (tokens, heads group, dim); rows of no sequence
  * become zeros with zero_rest, else stay as they were.  bf16 or fp16, head_dim
  * 32..256 in steps of 32, 16-byte aligned rows, strides in multiples of 8.

@@ -258,6 +258,12 @@ __device__ __forceinline__ void zero_rows(const PromptArgs& a, int head, int par
   }
 }
 
+// What a row's sums are multiplied with: 0 for one that sees nothing, NaN for one
+// whose scores are -inf alone or NaN.
+__device__ __forceinline__ float weight_of(bool sees, float l) {
+  return !sees ? 0.0f : l > 0.0f ? 1.0f / l : __builtin_nanf("");
+}
+
 // An infinite or NaN value makes NaN of every row whose products it is in, those
 // that do not see it as well.  A workgroup that ends with such rows goes over
 // its keys again: once for the outputs that see +inf or NaN, once for those that
@@ -691,7 +697,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
     if (h == 0) a.part_ml[at] = make_float2(m, l);
     return;
   }
-  const float by = l == 0.0f ? 0.0f : 1.0f / l;  // (a row that sees nothing: zeros)
+  const float by = weight_of(sees || bad, l);
   char* to = a.out + row * (D * 2) + 8 * h;
 #pragma unroll
   for (int n = 0; n < D / 32; ++n)
@@ -720,6 +726,9 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
   const int head = share.head;
   const int c = (int)threadIdx.x % kAcross, in = (int)threadIdx.x / kAcross;
   const int pairs = min(rows.count * a.group - rows.tile * kTileRows, kTileRows);
+  int key_first;
+  bool bad;  // (never: such a row has no shares)
+  const int pos0 = keys_of(a, rows, key_first, bad) - rows.count;
   for (int i = (int)blockIdx.y * kRows + in; in < kRows && i < pairs;
        i += kRows * (int)gridDim.y) {
     const int pair = rows.tile * kTileRows + i;
@@ -736,7 +745,7 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
         [&](uint32_t j) {
           return *reinterpret_cast<const float4*>(a.part_acc + part_at(j) * D + 4 * c);
         });
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    const float by = weight_of(pos0 + pair / a.group >= 0, l);
     typedef E E4 __attribute__((ext_vector_type(4)));
     E4 v;
 #pragma unroll

@@ -82,3 +82,39 @@ def test_values_far_behind_in_shares(dim, dtype):
     check(query, key, value, starts, key_starts, slopes=slopes)
     check(query, key, value, starts, key_starts, slopes=-slopes)
     check(query, key, value, starts, key_starts, slopes=slopes, window=2975)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, F16), (256, BF16)])
+def test_scores_of_minus_infinity(dim, dtype):
+    """Rows whose seen keys all score -inf are NaN, as a softmax's; such keys
+    weigh nothing beside others; rows that see no key are zeros."""
+    gen = torch.Generator().manual_seed(dim)
+    query, key, value = (rows(150, n, dim, dtype, gen) for n in (4, 2, 2))
+    query[..., 0] = 1.0
+    key[:3, :, 0] = -math.inf
+    key[149, :, 0] = -math.inf
+    value[149, :, 5] = math.inf  # (a NaN row has no infinities)
+    on_gpu = [t.to(DEV) for t in (query, key, value)]
+    starts = torch.tensor([0, 149], dtype=torch.int32)
+    at = starts.to(DEV)
+    got = prompt_attention(*on_gpu, token_starts=at, backend="hip")
+    assert bool(got[:3].isnan().all())
+    want, room = prompt64(query, key, value, [3, 149], [3, 149])
+    assert_rows(got[3:149], want[3:149], room[3:149])
+    got = prompt_attention(*on_gpu, window=1, backend="hip")  # each row its own token
+    alone = torch.tensor([0, 1, 2, 149], device=DEV)
+    assert bool(got[alone].isnan().all()) and bool(got[3:149].isfinite().all())
+    # 5 rows over 3000 keys and 700 over 600, which are shared out
+    counts, lengths = [5, 700], [3000, 600]
+    starts, ends = (torch.tensor([0] + n).cumsum(0).int() for n in (counts, lengths))
+    query = rows(705, 1, dim, dtype, gen)
+    key, value = (rows(3600, 1, dim, dtype, gen) for _ in range(2))
+    query[..., 0] = 1.0
+    key[:3000, 0, 0] = -math.inf
+    value[1000, 0, 7] = math.inf
+    got = prompt_attention(*(t.to(DEV) for t in (query, key, value)), token_starts=starts.to(DEV),
+                           key_starts=ends.to(DEV), backend="hip")
+    assert bool(got[:5].isnan().all())
+    want, room = prompt64(query, key, value, [5, 705], [3000, 3600])
+    assert_rows(got[5:], want[5:], room[5:])
+    assert not bool(got[5:105].any())
