@@ -114,6 +114,16 @@ def read(cache, tokens, token_starts):
     return tuple(found)
 
 
+def score(x, scores, distance, heads):
+    """Scaled products capped and biased by the tokens' distance; ``heads``: the
+    slopes' shape beside them."""
+    if scores.softcap:
+        x = torch.tanh(x / scores.softcap) * scores.softcap
+    if scores.slopes is not None:
+        x = x - scores.slopes.view(heads) * distance
+    return x
+
+
 def attend(q, k, v, position, scaling, scores, prefix=0):
     """(heads, group, rows, dim) outputs of query rows at their positions over
     (heads, tokens, dim) keys and values, in the inputs' type (32 bits or
@@ -123,10 +133,7 @@ def attend(q, k, v, position, scaling, scores, prefix=0):
     x = torch.matmul(q, k[:, None].transpose(2, 3).contiguous()) * scaling
     seen = ((distance >= 0) | (token < prefix)) & (position >= 0)[:, None]
     if scores is not None:
-        if scores.softcap:
-            x = torch.tanh(x / scores.softcap) * scores.softcap
-        if scores.slopes is not None:
-            x = x - scores.slopes.view(q.shape[0], q.shape[1], 1, 1) * distance.abs()
+        x = score(x, scores, distance.abs(), (*q.shape[:2], 1, 1))
         if scores.window:
             seen &= distance < scores.window
     p = torch.softmax(x.masked_fill(~seen, -math.inf), -1)
@@ -214,24 +221,24 @@ def decode(query, cache, scaling, scores=None):
     for b, length in enumerate(cache.lengths.tolist()):
         if length <= 0:
             continue
-        # (pages before the window may be gone)
-        first = 0
+        # (tokens before the window are hidden, their pages may be gone)
+        hidden = 0
         if scores is not None and scores.window:
-            first = max(length - scores.window, 0) // cache.page_size
+            hidden = max(length - scores.window, 0)
+        first = hidden // cache.page_size
         pages = cache.block_table[b, first:-(-length // cache.page_size)].long()
         if length > cache.capacity or not bool(((pages >= 0) & (pages < cache.pages)).all()):
             out[b] = math.nan
             continue
         first *= cache.page_size
         # (blocks, heads, page, dim) -> (heads, length, dim)
-        k, v = (x.transpose(0, 1).reshape(heads, -1, dim)[:, :length - first]
+        k, v = (x.transpose(0, 1).reshape(heads, -1, dim)[:, hidden - first:length - first]
                 for x in pages_of(cache, pages))
         q = _wide(query[b].reshape(heads, group, dim))
-        if scores is None:
-            p = torch.softmax(torch.matmul(q, k.transpose(1, 2)) * scaling, -1)
-            out[b] = torch.matmul(p, v).reshape(heads * group, dim).to(query.dtype)
-            continue
-        position = torch.full((1,), length - 1 - first, device=query.device)
-        rows = attend(q[:, :, None], k, v, position, scaling, scores)
-        out[b] = rows.reshape(heads * group, dim).to(query.dtype)
+        x = torch.matmul(q, k.transpose(1, 2)) * scaling
+        if scores is not None:
+            distance = torch.arange(k.shape[1] - 1, -1, -1, device=query.device)
+            x = score(x, scores, distance, (heads, group, 1))
+        p = torch.softmax(x, -1)
+        out[b] = torch.matmul(p, v).reshape(heads * group, dim).to(query.dtype)
     return out
