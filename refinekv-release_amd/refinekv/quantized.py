@@ -23,6 +23,7 @@ from . import _hip
 PAGE_SIZES = (16, 32, 64, 128, 256)
 GROUP_DIMS = 32
 LARGEST = 4096.0
+LARGEST_SCALE = 552.0  # a 15th of a span of 2 LARGEST, rounded up to 7 significant bits
 
 
 def _tables(table, lengths, device):
@@ -37,6 +38,22 @@ def _tables(table, lengths, device):
         raise ValueError("lengths must be contiguous")
     if table.device != device or lengths.device != device:
         raise ValueError("block_table and lengths must be on the cache's device")
+
+
+def _check_held(codes, scales):
+    """Codes of 4 bits, and on a GPU scales and zeros that the kernels' products hold
+    exactly."""
+    if int(codes.max()) > 15:
+        raise ValueError("codes must be 0 to 15")
+    if scales.device.type != "cuda":
+        return
+    scale, zero = scales.unbind(-1)
+    odd = (scale.view(torch.int16) & 15 != 0) | (scale < 0) | (scale > LARGEST_SCALE)
+    if bool((odd & ~scale.isnan()).any()):
+        raise ValueError(f"scales must be NaN, or 0 to {LARGEST_SCALE:g} of 7 significant bits (their "
+                         "last 4 bits 0)")
+    if bool(zero.isinf().any()):
+        raise ValueError("zeros must not be infinite")
 
 
 def _meet(a, b):
@@ -130,8 +147,12 @@ class QuantizedCache:
                dtype=torch.bfloat16):
         """A cache of codes (pages, kv_heads, page_size, head_dim) uint8, one a
         byte, and (scale, zero) pairs (pages, kv_heads, page_size,
-        head_dim / 32, 2) float16.  Scales must have 7 significant bits (their
-        last 4 bits 0); codes and scales are copied."""
+        head_dim / 32, 2) float16; both are copied.
+
+        On a GPU scales must have 7 significant bits (their last 4 bits 0) and
+        lie in 0..552, or be NaN, and zeros not be infinite, in every page: the
+        kernels' products hold no others (the torch operations on a CPU take
+        them all; a cache that is moved to a GPU is not looked at again)."""
         for codes, scales in ((key_codes, key_scales), (value_codes, value_scales)):
             if codes.ndim != 4 or codes.dtype != torch.uint8 or codes.shape[3] % GROUP_DIMS or (
                     codes.shape[2] % 16):
@@ -141,6 +162,8 @@ class QuantizedCache:
                     *codes.shape[:3], codes.shape[3] // GROUP_DIMS, 2):
                 raise ValueError("scales must be float16 with shape (pages, kv_heads, page_size, "
                                  "head_dim / 32, 2)")
+            if codes.numel():
+                _check_held(codes, scales)
         return cls(pack_keys(key_codes), pack_values(value_codes), key_scales.clone(
             memory_format=torch.contiguous_format), pack_scales(value_scales), block_table,
             lengths, dtype)
