@@ -133,6 +133,8 @@ class QuantizedCache:
     def empty(cls, pages, kv_heads, page_size, head_dim, sequences, max_blocks, *,
               dtype=torch.bfloat16, device=None):
         """A new cache of zeros with no pages assigned (block_table -1)."""
+        if head_dim not in _hip.SUPPORTED_DIMS:
+            raise ValueError("a cache in 4 bits needs head_dim in 32..256 (multiple of 32)")
         shape = (pages, kv_heads, page_size)
         codes = [torch.zeros(*shape, head_dim // 2, dtype=torch.uint8, device=device)
                  for _ in range(2)]

@@ -1,5 +1,5 @@
-"""What QuantizedCache.packed takes: codes of 4 bits, scales as the kernels'
-products hold them exactly."""
+"""What QuantizedCache.packed and empty take: codes of 4 bits, scales as the
+kernels' products hold them exactly, whole groups."""
 
 import math
 
@@ -31,6 +31,13 @@ def test_codes_are_of_4_bits(which):
     for code in (16, 200):
         with pytest.raises(ValueError, match="codes"):
             packed_with("cpu", which, (1, 2, 7, 40), code)
+
+
+def test_head_dims_between_groups():
+    for dim in (33, 48, 65, 100, 127, 257):
+        with pytest.raises(ValueError, match="head_dim"):
+            QuantizedCache.empty(2, 1, 16, dim, 1, 1)
+    assert QuantizedCache.empty(2, 1, 16, 96, 1, 1).head_dim == 96
 
 
 @pytest.mark.gpu
