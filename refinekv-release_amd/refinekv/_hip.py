@@ -701,6 +701,16 @@ def _whole_rows(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _rows_apart(t, cache):
+    """_whole_rows, of rows that are no views of a 4-bit cache (the C entry looks
+    at those that need no copy)."""
+    rows = _whole_rows(t)
+    if rows is not t and any(_spans_meet(t, p) for p in (
+            cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales)):
+        raise ValueError("rkv_quantized_append: rows overlap the cache")
+    return rows
+
+
 def quantized_append(key, value, cache, query=None, table=None, token_starts=None,
                      query_out=None):
     """rkv_quantized_append on checked rows; returns the turned query or None."""
@@ -708,10 +718,10 @@ def quantized_append(key, value, cache, query=None, table=None, token_starts=Non
     if _elsewhere(device):
         with torch.cuda.device(device):
             return quantized_append(key, value, cache, query, table, token_starts, query_out)
-    key, value = _whole_rows(key), _whole_rows(value)
+    key, value = _rows_apart(key, cache), _rows_apart(value, cache)
     rows, target = (0, 0, 0, 0, 0, 0, 0), query_out
     if query is not None:
-        query = _whole_rows(query)
+        query = _rows_apart(query, cache)
         # (the kernel writes whole vectors, and not over the query)
         if query_out is None or not _takes_rows(query_out) or _spans_meet(query, query_out):
             target = _like(query)
