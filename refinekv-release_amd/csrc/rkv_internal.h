@@ -46,6 +46,11 @@ inline int check_launch(const char* what) {
   return kOk;
 }
 
+// Whether a launch has fewer than 2^32 threads, which is how far they are counted.
+inline bool launch_fits(int64_t blocks, int64_t threads) {
+  return blocks < (int64_t(1) << 32) / threads;
+}
+
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 }  // namespace rkv

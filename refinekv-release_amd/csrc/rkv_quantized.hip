@@ -819,13 +819,14 @@ int rows_args(const char* who, QuantRows& a, const rkv_quantized_cache* c, int64
 // Heads that a token's threads hold at a time, and the grid: `heads` rows a
 // token, `items` threads a row.  Few tokens: all threads of a workgroup, for
 // latency.
-int rows_grid(QuantRows& a, int heads, int items, int64_t& blocks) {
+int rows_grid(const char* who, QuantRows& a, int heads, int items, int64_t& blocks) {
   a.slots = kRowThreads / items;
   if (a.tokens * items * a.slots >= kManyRowThreads) a.slots = items < kWave / 2 ? kWave / 2 / items : 1;
   a.slots = a.slots < heads ? a.slots : heads;
   a.per_block = kRowThreads / (items * a.slots);
   blocks = (a.tokens + a.per_block - 1) / a.per_block;
-  return blocks <= 0x7fffffff ? kOk : set_error(kInvalidArgument, "too many tokens");
+  return launch_fits(blocks, kRowThreads) ? kOk
+                                          : set_error(kInvalidArgument, "%s: too many tokens", who);
 }
 
 }  // namespace
@@ -896,7 +897,7 @@ extern "C" int rkv_quantized_append(const rkv_quantized_cache* cache, const void
   a.scale = scale;
   int64_t blocks;
   const bool halves = !a.interleaved && rotary_dim == cache->dim && rotary_dim / 2 % kGroupDims == 0;
-  rc = rows_grid(a, a.q_heads + 2 * a.heads, a.dim / (halves ? 2 * kItem : kItem), blocks);
+  rc = rows_grid(who, a, a.q_heads + 2 * a.heads, a.dim / (halves ? 2 * kItem : kItem), blocks);
   if (rc) return rc;
   const dim3 grid((unsigned)blocks), threads(kRowThreads);
   const bool half = cache->dtype == RKV_F16;
@@ -938,7 +939,7 @@ extern "C" int rkv_quantized_read(const rkv_quantized_cache* cache, int64_t toke
   a.dst[1] = static_cast<char*>(key_out);
   a.dst[2] = static_cast<char*>(value_out);
   int64_t blocks;
-  rc = rows_grid(a, 2 * a.heads, a.dim / kItem, blocks);
+  rc = rows_grid(who, a, 2 * a.heads, a.dim / kItem, blocks);
   if (rc) return rc;
   const dim3 grid((unsigned)blocks), threads(kRowThreads);
   if (cache->dtype == RKV_F16) quantized_read_kernel<_Float16><<<grid, threads, 0, stream>>>(a);

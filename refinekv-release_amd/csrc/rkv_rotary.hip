@@ -220,7 +220,8 @@ int launch_w(RotaryArgs& a, hipStream_t stream) {
   a.slots = a.slots < kThreads / wide ? a.slots : kThreads / wide;
   a.per_block = kThreads / (wide * a.slots);
   const int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
-  if (blocks > 0x7fffffff) return set_error(kInvalidArgument, "rotary: too many tokens");
+  if (!launch_fits(blocks, kThreads))
+    return set_error(kInvalidArgument, "rotary: too many tokens");
   const int64_t bytes = a.tokens * a.heads * a.dim * (int64_t)sizeof(T);
   if (bytes >= kStreamBytes)
     rotary_kernel<T, W, kAdjacent, true><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
@@ -296,9 +297,10 @@ __global__ __launch_bounds__(kThreads) void paged_read_kernel(ReadArgs a) {
 template <typename V>
 int launch_read(const ReadArgs& a, hipStream_t stream) {
   const int64_t each = 2 * (int64_t)a.heads * (a.row_bytes / (int)sizeof(V));
-  if (a.tokens > INT64_MAX / each || (a.tokens * each + kThreads - 1) / kThreads > 0x7fffffff)
+  const bool fits = launch_fits(a.tokens, each);
+  const int64_t blocks = fits ? (a.tokens * each + kThreads - 1) / kThreads : 0;
+  if (!fits || !launch_fits(blocks, kThreads))
     return set_error(kInvalidArgument, "rkv_paged_read: too many tokens");
-  const int64_t blocks = (a.tokens * each + kThreads - 1) / kThreads;
   paged_read_kernel<V><<<dim3((unsigned)blocks), dim3(kThreads), 0, stream>>>(a);
   return check_launch("paged_read_kernel");
 }
