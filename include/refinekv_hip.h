@@ -416,10 +416,11 @@ int rkv_quantized_plan(const rkv_quantized_cache* cache, int64_t group, size_t* 
  * prefix[b] (device int32 per sequence, null: none), and of these at most
  * scores->window back; one that sees nothing is zeros, one whose scores are -inf
  * alone NaN, as a softmax is.  An infinite or NaN value counts for the rows that
- * see it, whatever it weighs.  Query heads h group .. + group - 1 belong
- * to KV head h.  output: dense (tokens, heads group, dim); rows of no sequence
- * become zeros with zero_rest, else stay as they were.  bf16 or fp16, head_dim
- * 32..256 in steps of 32, 16-byte aligned rows, strides in multiples of 8.
+ * see it, whatever it weighs.  Query heads h group .. + group - 1 belong to KV
+ * head h.  output: dense (tokens, heads group, dim); rows of no sequence (all,
+ * with token_starts that decrease) become zeros with zero_rest, else stay as they
+ * were.  bf16 or fp16, head_dim 32..256 in steps of 32, 16-byte aligned rows,
+ * strides in multiples of 8.
  * Calls with few rows share out their keys and join them through the workspace
  * (rkv_prompt_plan; 0 bytes: none needed; most_keys: key_tokens, or the tokens
  * a row of the block table can address).

@@ -83,7 +83,8 @@ struct PromptRows {
   int tile;             // of kTileRows (row, head of the group) pairs
 };
 
-__device__ __forceinline__ void rows_of(const PromptArgs& a, int b, int& first, int& count) {
+// Sequence b's rows, inside the tensor.  False: its starts decrease.
+__device__ __forceinline__ bool rows_of(const PromptArgs& a, int b, int& first, int& count) {
   int from, to;
   if (a.step) {
     from = b;
@@ -97,6 +98,7 @@ __device__ __forceinline__ void rows_of(const PromptArgs& a, int b, int& first, 
   }
   first = min(max(from, 0), a.tokens);
   count = min(max(to, first), a.tokens) - first;
+  return from <= to;
 }
 
 __device__ __forceinline__ uint32_t tiles_for(const PromptArgs& a, int count) {
@@ -122,36 +124,39 @@ __device__ __forceinline__ int keys_of(const PromptArgs& a, const PromptRows& r,
   return r.count;
 }
 
-// The slot-th of the entries that the sequences have `entries(b)` of, with its
-// sequence and its place among that one's entries.  False: there are fewer.
+// The slot-th of the entries that the sequences have `entries(b, odd)` of, with its
+// sequence and its place among that one's entries.  False: there are fewer, or a
+// sequence's starts decrease (odd): overlapping sequences could have more entries
+// than the grid, so that then no row is any sequence's.
 template <typename Entries>
 __device__ __forceinline__ bool find_entry(const PromptArgs& a, uint32_t slot, bool from_end,
                                            Entries entries, int& b, uint32_t& place) {
   const int lane = threadIdx.x % kWave;
   const int per = (a.sequences + kWave - 1) / kWave;
   uint32_t sum = 0;
-  for (int i = 0; i < per && lane * per + i < a.sequences; ++i) sum += entries(lane * per + i);
+  bool odd = false;
+  for (int i = 0; i < per && lane * per + i < a.sequences; ++i) sum += entries(lane * per + i, odd);
   const uint32_t upto = wave_scan(sum);
   const uint32_t total = (uint32_t)uniform((int)__shfl((int)upto, kWave - 1, kWave));
-  if (slot >= total) return false;
+  if (slot >= total || __builtin_amdgcn_ballot_w64(odd) != 0) return false;
   const uint32_t at = from_end ? total - 1u - slot : slot;
   const int owner = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > at));
   place = at - (uint32_t)uniform(__shfl((int)(upto - sum), owner, kWave));
   for (b = owner * per; b < a.sequences; ++b) {
-    const uint32_t here = (uint32_t)uniform((int)entries(b));
+    const uint32_t here = (uint32_t)uniform((int)entries(b, odd));
     if (place < here) return true;
     place -= here;
   }
-  return false;  // (starts that overlap so often that their sum passed 32 bits)
+  return false;  // (starts that change under the call)
 }
 
 // The slot-th of the tiles, the last ones of the last sequence first: a
 // sequence's later tiles have more keys.
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, uint32_t slot, PromptRows& r) {
   uint32_t place;
-  auto tiles = [&](int b) {
+  auto tiles = [&](int b, bool& odd) {
     int first, count;
-    rows_of(a, b, first, count);
+    odd |= !rows_of(a, b, first, count);
     return tiles_for(a, count);
   };
   if (!find_entry(a, slot, true, tiles, r.b, place)) return false;
@@ -194,9 +199,10 @@ __device__ __forceinline__ bool find_share(const PromptArgs& a, uint32_t slot, P
   auto sizes = [&](int b, uint32_t& tiles, uint32_t& units, int& begin) {
     PromptRows q;
     q.b = b;
-    rows_of(a, b, q.first, q.count);
+    const bool odd = !rows_of(a, b, q.first, q.count);
     tiles = tiles_for(a, q.count);
     units = tiles ? units_of<T>(a, q, begin) : 0u;
+    return odd;
   };
   uint32_t sum = 0, tiles, units;
   int begin = 0;
@@ -211,8 +217,8 @@ __device__ __forceinline__ bool find_share(const PromptArgs& a, uint32_t slot, P
   const uint32_t least = max(256 / T >> a.unit, 1);
   const uint32_t chunk = need > least ? (uint32_t)need : least;
   auto chunks_of = [&](uint32_t n) { return (n + chunk - 1u) / chunk; };
-  auto entries = [&](int b) {
-    sizes(b, tiles, units, begin);
+  auto entries = [&](int b, bool& odd) {
+    odd |= sizes(b, tiles, units, begin);
     return tiles * heads * (kJoin ? 1u : chunks_of(units));
   };
   uint32_t place;
@@ -241,13 +247,18 @@ __device__ __forceinline__ bool find_share(const PromptArgs& a, uint32_t slot, P
   return true;
 }
 
-// Rows of no sequence: the part-th part of them becomes zeros, for one head's group.
+// Rows of no sequence (all, where starts decrease): the part-th part of them becomes
+// zeros, for one head's group.
 template <int D>
 __device__ __forceinline__ void zero_rows(const PromptArgs& a, int head, int part) {
   int first, count, last;
+  bool odd = false;
+  for (int b = (int)threadIdx.x % kWave; b < a.sequences; b += kWave)
+    odd |= !rows_of(a, b, first, count);
   rows_of(a, 0, first, count);
   rows_of(a, a.sequences - 1, last, count);
   last += count;
+  if (__builtin_amdgcn_ballot_w64(odd) != 0) last = first;
   const int per_row = a.group * (D / 8);
   const int64_t n = (int64_t)(a.tokens - last + first) * per_row;
   for (int64_t i = (int64_t)part * kPromptThreads + threadIdx.x; i < n;
@@ -721,7 +732,7 @@ __global__ __launch_bounds__(kPromptThreads) void prompt_join_kernel(PromptArgs 
   Share share;
   if (!find_share<PromptTile<D>::kTokens, true>(a, blockIdx.x, rows, share) || share.chunks == 1)
     return;
-  // (starts that overlap ask for more shares than there are)
+  // (starts or lengths that change under the call)
   if ((uint32_t)share.first + (int64_t)(share.chunks - 1) * share.apart >= a.shares) return;
   const int head = share.head;
   const int c = (int)threadIdx.x % kAcross, in = (int)threadIdx.x / kAcross;

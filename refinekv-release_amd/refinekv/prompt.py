@@ -90,7 +90,8 @@ def prompt_attention(query, key, value, *, token_starts=None, key_starts=None, p
     takes the distance either way).
 
     Returns a new tensor, or ``output``: rows that see nothing are zeros, rows of
-    no sequence zeros in a new tensor and left as they were in ``output``.
+    no sequence (all, with token_starts that decrease) zeros in a new tensor and
+    left as they were in ``output``.
     An infinite or NaN key or value counts for the rows that see it alone; a row
     whose scores are -inf alone is NaN.
     ``workspace`` (a dict) keeps the buffers in which calls with few rows join

@@ -160,6 +160,8 @@ def _prompt(query, heads, starts, keys_of, scaling, scores, prefix, output):
     group = q_heads // heads
     out = torch.zeros_like(query, memory_format=torch.contiguous_format) if output is None \
         else output
+    if any(a > b for a, b in zip(starts, starts[1:])):
+        return out
     for b in range(len(starts) - 1):
         first = min(max(starts[b], 0), tokens)
         end = min(max(starts[b + 1], first), tokens)
