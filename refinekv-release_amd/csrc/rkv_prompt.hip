@@ -298,14 +298,14 @@ __device__ __forceinline__ uint32_t value_words(uint32_t w, int pass) {
 }
 
 // The matrix cores and the softmax's vector issue bound it, one after the other
-// more than side by side: 16384 tokens (8 KV heads, group 4, d 128) in 2160-2190
-// us, 1010 TFLOP/s of the visible products (a bf16 product of 8192^3 reaches 1257
+// more than side by side: 16384 tokens (8 KV heads, group 4, d 128) in 2170-2240
+// us, 980-1010 TFLOP/s of the visible products (a bf16 product of 8192^3 reaches 1257
 // here), the matrix cores busy for 47 % of it and the vector ALUs for 51 %.
 // (Scores of the next tile computed beside the softmax of this one, keys two tiles
 // ahead: 2610 us; tiles of 32 keys 2380; reads of all a product's operands in
 // groups of 8: 2300 against 2255.)  Few rows over many keys are bound by the keys
 // on their way into LDS: 3 x 33 rows over 134 K tokens of 4 heads (274 MB) 104-120
-// us, then 11 for the join.  One tile alone takes 10 us: finding it, its first
+// us, then 12 for the join.  One tile alone takes 10 us: finding it, its first
 // loads and its code.
 // A workgroup has 128 (row, head of the group) pairs of one sequence and KV
 // head, 32 a wave, and goes over the keys they see in tiles that two LDS buffers
@@ -410,7 +410,7 @@ __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_kernel(Prompt
   // Scores without a cap are scaled on the way into the exponential, slopes divided
   // by the scale for it; of tiles before all the wave's rows a key's bias is that of
   // the tile's first and its place's, one operation a score (23 documents, head_dim
-  // 64, 119 -> 111 us).  Not with slopes or scales whose products could overflow.
+  // 64, 119 -> 111 us then, 108 now).  Not with slopes or scales whose products could overflow.
   float slope = 0.0f, unit_slope = 0.0f, scale = a.scale;
   bool late = true;
   int biased_end = 0;  // tokens up to every row of the wave

@@ -697,7 +697,7 @@ template <int D>
 constexpr int kPerCu4 = D <= 64 ? 3 : D <= 128 ? 2 : 1;
 
 // HBM and vector issue bound it together: 1.34 GB of 8 x 131072 tokens (8 KV heads,
-// group 4, d 128) in 222-245 us, 5.5-6.0 TB/s; 313 vector instructions a tile of 32
+// group 4, d 128) in 222-264 us, 5.1-6.0 TB/s; 313 vector instructions a tile of 32
 // tokens (176 of them turn its 8192 codes into fp16) keep the ALUs busy for 138 us
 // of it.  (378 when masks and biases were literals and every tile had the selects
 // of a row's end, and 258 us.)  A call of few tokens is paged_kernel's chain of
